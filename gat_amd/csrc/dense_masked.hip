@@ -1427,9 +1427,8 @@ struct MSrcState8 {
     float df2;
 };
 
-// <a, b> over eight floats as four packed two-float multiply-adds and one add.  Written on two-float vectors so
-// that the products of ONE entry share the packed instructions: left to itself the compiler pairs the products of
-// two entries instead and spends two register moves per packed instruction on bringing their operands together.
+// <a, b> over eight floats in two chains of four multiply-adds and one add.  The library is compiled without the
+// packed fp32 instructions (Makefile); the two-float vectors only say which sums belong together.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float dot8_pairs(float4 a0, float4 a1, float4 b0, float4 b1) {
     f32x2 s = (f32x2){a0.x, a0.y} * (f32x2){b0.x, b0.y};

@@ -186,9 +186,8 @@ __device__ __forceinline__ float coef_drop_scale(uint64_t seed, int64_t b, int N
     return keep_mask(seed, idx, keep) ? 1.0f / keep : 0.f;
 }
 
-// float4 arithmetic of the row kernels (one float4 of a feature row per lane)
-// Written on two-element vectors so that the compiler can use the packed fp32 instructions of
-// CDNA3/4 (v_pk_fma_f32, v_pk_mul_f32, v_pk_add_f32: two lanes' worth of fp32 per issue slot).
+// float4 arithmetic of the row kernels (one float4 of a feature row per lane), on two-element vectors; the library is
+// compiled without the packed fp32 instructions (Makefile), so each element is an instruction of its own.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float4 f4_fma(float a, float4 x, float4 y) {
     const f32x2_t s = {a, a};
