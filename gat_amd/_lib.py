@@ -12,7 +12,7 @@ import os
 # that owns torch's device memory and streams; loading libgatmi first would map a second runtime.
 import torch  # noqa: F401  (isort: keep above the CDLL call)
 
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgatmi.so")
@@ -97,6 +97,17 @@ _SIGNATURES = {
     "gatmi_bnf_attn_bwd": (c_int, [c_int64, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, P, P, P, c_float, P, P, c_int, P, P, P, P, c_int32, P]),
     "gatmi_ipd_fwd": (c_int, [c_int64, c_int32, c_int32, P, c_int32, c_float, c_uint64, P, P]),
     "gatmi_ipd_bwd": (c_int, [c_int64, c_int32, c_int32, P, P, P, c_int32, c_float, c_uint64, P, P]),
+    "gatmi_dot_attn_fwd_ws_floats": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "gatmi_dot_attn_fwd": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, c_int64, c_int64, P, P, c_float,
+                                   P, P, P, P]),
+    "gatmi_dot_attn_bwd": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, P, P, P, P, c_int64, c_int64, P, P,
+                                   c_float, P, P, P, P, P]),
+    "gatmi_embed_fwd": (c_int, [P, c_int32, c_int64, P, c_int64, c_int64, c_int32, c_int32, c_float, P, P]),
+    "gatmi_embed_bwd_ws_floats": (c_size_t, [c_int64, c_int64, c_int32]),
+    "gatmi_embed_bwd": (c_int, [P, c_int32, c_int64, P, c_int64, c_int64, c_int32, c_int32, c_float, P, P, P]),
+    "gatmi_newton_schulz_ws_floats": (c_size_t, [c_int64, c_int64, c_int64]),
+    "gatmi_newton_schulz": (c_int, [c_int64, c_int64, c_int64, P, c_int64, c_int64, c_int32, c_int32, c_double, c_double, c_double, c_double,
+                                    P, c_int64, c_int64, P, P]),
     "gatmi_halo_pack": (c_int, [P, P, c_int64, c_int32, P, P]),
     "gatmi_halo_unpack_add": (c_int, [P, P, c_int64, c_int32, P, P]),
     "gatmi_halo_unpack_sum": (c_int, [P, P, P, P, c_int64, c_int32, P, P]),

@@ -1,0 +1,625 @@
+// Orthogonalised updates: `steps` Newton-Schulz steps X <- a X + b (X X^T) X + c (X X^T)^2 X of every matrix of a batch,
+// from X = x / (|x|_F + eps).  Each step applies the odd polynomial a s + b s^3 + c s^5 to the singular values.
+//
+// The polynomial's slope at 0 is a, so what a step rounds off in the directions of small singular values is multiplied by
+// a in every step that follows (3.44^5 = 485 for the usual coefficients): with 16-bit operands five steps leave errors
+// of 2 to 10 %.  Two ways keep fp32's accuracy, by the length n of the shorter side:
+//
+// n <= 64 (`narrow`): with G = X^T X (n x n; the longer side is summed over), all factors are polynomials in G and
+//   commute: the result is X Q(G) with an n x n matrix Q.  Three launches: G, Q, X Q, whatever the longer side.  Squaring the
+//   singular values doubles the digits that small ones need, so G, Q and the last product are formed in fp64 on
+//   v_mfma_f64_16x16x4_f64 (128 flop / clock / CU): for n <= 64 they are small.  |x|_F is the root of G's trace.
+//
+// n > 64 (`wide`): the steps themselves, three products each, on the 16-bit matrix instructions at fp32 accuracy: an
+//   operand v is kept as hi + lo, two fp16 numbers of 11 bits each, and hi hi + hi lo + lo hi is summed in fp32 (relative error 2^-22;
+//   the missing lo lo is below it).  fp16 has few exponent bits, but the iteration bounds its operands: entries of X, X X^T and of the
+//   polynomial are below kMaxEntry (checked on the host for the given coefficients), so that one fixed scale
+//   2^13 keeps hi in range and lo of every entry that matters above the subnormals.  Where |x|_F is not far above eps, X is tiny: it is
+//   then kept times 2^e with e falling from step to step as X can grow (NsShift).  3 products at 16 times the rate of fp32's.
+//   X X^T and its square are symmetric: only tiles on and above the diagonal are formed, each is stored twice.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+#include "device_common.h"
+
+namespace gatmi {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNarrow = 64;
+constexpr int kNarrowThreads = 512;          // of the polynomial kernel
+constexpr int kGramParts = 256;              // partial sums of G per matrix, at most
+constexpr int kMaxSteps = 32;
+constexpr int64_t kBatchAtOnce = 32768;      // matrices of one set of launches (grid.y, grid.z)
+constexpr int64_t kMaxSide = 1 << 20;        // of a wide matrix
+constexpr float kPlaneScale = 8192.f;        // 2^13
+constexpr double kMaxEntry = 7.5;            // kPlaneScale * kMaxEntry < 65504
+
+struct NsMatrix {                            // the batch as given: element (i, j) of matrix b at x + b * batch + i * row + j
+    const void *x;
+    void *out;
+    int64_t x_batch, x_row, out_batch, out_row;
+    int64_t m, n;
+};
+
+template <typename T>
+__device__ __forceinline__ float ns_load(const T *p) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float *>(p);
+    else return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t *>(p) << 16);
+}
+template <typename T>
+__device__ __forceinline__ void ns_store(T *p, float v) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float *>(p) = v;
+    else *reinterpret_cast<uint16_t *>(p) = (uint16_t)pack_bf16x2(v, 0.f);
+}
+
+// ---- narrow ------------------------------------------------------------------------------------------------------------
+// S = index along the short side (0..n), L = along the long side.  TALL: the long side is the row of x.
+template <typename T, bool TALL>
+__device__ __forceinline__ int64_t ns_at(int64_t row, int64_t s, int64_t l) {
+    return TALL ? l * row + s : s * row + l;
+}
+
+struct NarrowArgs {
+    NsMatrix a;
+    int n;                     // short side
+    int64_t len;               // long side
+    int parts;
+    int64_t per_part;          // a multiple of 16
+    double *gram;              // [batch][parts][np * np], upper tiles
+    double *q;                 // [batch][np * np]
+    int steps;
+    double ca, cb, cc, eps;
+};
+
+// One wave per part of the long side: all upper tiles of G in registers, each loaded value is both operands.
+template <typename T, bool TALL, int TILES>
+__global__ __launch_bounds__(64) void ns_gram_kernel(NarrowArgs a) {
+    constexpr int NP = 16 * TILES;
+    const int lane = threadIdx.x, i = lane & 15, kq = lane >> 4;
+    const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.y * a.a.x_batch;
+    const int64_t l0 = blockIdx.x * a.per_part, l1 = min(a.len, l0 + a.per_part);
+    f64x4 acc[TILES][TILES];
+#pragma unroll
+    for (int p = 0; p < TILES; ++p)
+#pragma unroll
+        for (int q = p; q < TILES; ++q) acc[p][q] = (f64x4){0, 0, 0, 0};
+    for (int64_t l = l0; l < l1; l += 16) {
+        float v[TILES][4];
+#pragma unroll
+        for (int p = 0; p < TILES; ++p)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int64_t at = l + 4 * kq + t;                // slot kq of product t: any order of the sum, the same for both operands
+                const int s = 16 * p + i;
+                v[p][t] = s < a.n && at < l1 ? ns_load<T>(x + ns_at<T, TALL>(a.a.x_row, s, at)) : 0.f;
+            }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int p = 0; p < TILES; ++p)
+#pragma unroll
+                for (int q = p; q < TILES; ++q)
+                    acc[p][q] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v[p][t], (double)v[q][t], acc[p][q], 0, 0, 0);
+    }
+    double *g = a.gram + ((size_t)blockIdx.y * a.parts + blockIdx.x) * (NP * NP);
+#pragma unroll
+    for (int p = 0; p < TILES; ++p)
+#pragma unroll
+        for (int q = p; q < TILES; ++q)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) g[(16 * p + kq + 4 * r) * NP + 16 * q + i] = acc[p][q][r];      // C: row kq + 4 r, column i
+}
+
+// C = A B for symmetric commuting A and B in LDS: the waves share the upper tiles, results stay in registers
+// until every wave has read its operands.
+template <int TILES>
+struct NsProduct {
+    static constexpr int NP = 16 * TILES, LD = NP + 2, COUNT = TILES * (TILES + 1) / 2, WAVES = kNarrowThreads / 64, PER = (COUNT + WAVES - 1) / WAVES;
+    f64x4 acc[PER];
+    __device__ static void tile(int t, int &p, int &q) {
+        p = 0;
+        while (t >= TILES - p) { t -= TILES - p; ++p; }
+        q = p + t;
+    }
+    __device__ __forceinline__ void multiply(const double *A, const double *B) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            acc[u] = (f64x4){0, 0, 0, 0};
+            const int t = wave + u * WAVES;
+            if (t < COUNT) {
+                int p, q;
+                tile(t, p, q);
+                const double *ar = A + (16 * p + i) * LD + kq, *br = B + (16 * q + i) * LD + kq;        // B symmetric: its column is its row
+#pragma unroll
+                for (int k = 0; k < NP; k += 4) acc[u] = __builtin_amdgcn_mfma_f64_16x16x4f64(ar[k], br[k], acc[u], 0, 0, 0);
+            }
+        }
+    }
+    // C_ij = alpha acc_ij + beta D_ij + diag, written to both halves
+    __device__ __forceinline__ void store(double *C, double alpha, double beta, const double *D, double diag) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int t = wave + u * WAVES;
+            if (t < COUNT) {
+                int p, q;
+                tile(t, p, q);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * p + kq + 4 * r, col = 16 * q + i;
+                    if (row <= col) {                             // of a tile on the diagonal only one half is stored, to both places
+                        double v = alpha * acc[u][r];
+                        if (D) v += beta * D[row * LD + col];
+                        if (row == col) v += diag;
+                        C[row * LD + col] = v;
+                        C[col * LD + row] = v;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Q of one matrix per block: P_k = a I + b A_k + c A_k^2, Q = P_0 P_1 ..., A_{k+1} = A_k P_k^2, from A_0 = G / (|x|_F + eps)^2.
+// The scale of x goes into Q.
+template <int TILES>
+__global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
+    using Product = NsProduct<TILES>;
+    constexpr int NP = Product::NP, LD = Product::LD;
+    extern __shared__ double lds[];
+    double *A = lds, *P = A + NP * LD, *Q = P + NP * LD;
+    const double *g = a.gram + (size_t)blockIdx.x * a.parts * (NP * NP);
+    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) {
+        const int row = e / NP, col = e % NP;
+        const int up = row / 16 <= col / 16 ? e : col * NP + row;          // tiles below the diagonal are not formed
+        double s = 0;
+        for (int p = 0; p < a.parts; ++p) s += g[(size_t)p * (NP * NP) + up];
+        A[row * LD + col] = s;
+    }
+    __syncthreads();
+    double trace = 0;
+    for (int d = 0; d < a.n; ++d) trace += A[d * LD + d];
+    const double inv = 1.0 / (sqrt(trace) + a.eps);
+    __syncthreads();
+    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) A[e / NP * LD + e % NP] *= inv * inv;
+    if (a.steps == 0)
+        for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) Q[e / NP * LD + e % NP] = e / NP == e % NP ? 1.0 : 0.0;
+    __syncthreads();
+    Product pr;
+    for (int step = 0; step < a.steps; ++step) {
+        pr.multiply(A, A);
+        pr.store(P, a.cc, a.cb, A, a.ca);
+        __syncthreads();
+        if (step == 0) {
+            for (int e = threadIdx.x; e < NP * LD; e += kNarrowThreads) Q[e] = P[e];
+        } else {
+            pr.multiply(Q, P);
+            __syncthreads();
+            pr.store(Q, 1.0, 0.0, nullptr, 0.0);
+        }
+        if (step + 1 < a.steps) {
+            for (int half = 0; half < 2; ++half) {
+                pr.multiply(A, P);
+                __syncthreads();
+                pr.store(A, 1.0, 0.0, nullptr, 0.0);
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+    double *q = a.q + (size_t)blockIdx.x * (NP * NP);
+    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) q[e] = Q[e / NP * LD + e % NP] * inv;
+}
+
+// out = X Q, 16 places of the long side per wave
+template <typename T, bool TALL, int TILES>
+__global__ __launch_bounds__(256) void ns_apply_kernel(NarrowArgs a) {
+    constexpr int NP = 16 * TILES, LD = NP + 2;
+    extern __shared__ double lds[];
+    const double *q = a.q + (size_t)blockIdx.y * (NP * NP);
+    for (int e = threadIdx.x; e < NP * NP; e += 256) lds[e / NP * LD + e % NP] = q[e];
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, kq = lane >> 4;
+    const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.y * a.a.x_batch;
+    T *out = reinterpret_cast<T *>(a.a.out) + (int64_t)blockIdx.y * a.a.out_batch;
+    for (int64_t l0 = (blockIdx.x * 4 + wave) * (int64_t)16; l0 < a.len; l0 += (int64_t)gridDim.x * 64) {
+        float v[TILES][4];
+#pragma unroll
+        for (int c = 0; c < TILES; ++c)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int s = 16 * c + 4 * kq + t;
+                v[c][t] = s < a.n && l0 + i < a.len ? ns_load<T>(x + ns_at<T, TALL>(a.a.x_row, s, l0 + i)) : 0.f;
+            }
+#pragma unroll
+        for (int p = 0; p < TILES; ++p) {
+            f64x4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < TILES; ++c)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const double qv = lds[(16 * p + i) * LD + 16 * c + 4 * kq + t];
+                    // the contiguous direction of `out` lies across the lanes of a row of C
+                    acc = TALL ? __builtin_amdgcn_mfma_f64_16x16x4f64((double)v[c][t], qv, acc, 0, 0, 0)
+                               : __builtin_amdgcn_mfma_f64_16x16x4f64(qv, (double)v[c][t], acc, 0, 0, 0);
+                }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t l = l0 + (TALL ? kq + 4 * r : i);
+                const int s = 16 * p + (TALL ? i : kq + 4 * r);
+                if (l < a.len && s < a.n) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, s, l), (float)acc[r]);
+            }
+        }
+    }
+}
+
+// ---- wide --------------------------------------------------------------------------------------------------------------
+constexpr int kWT = 128;          // rows and columns of a tile
+constexpr int kWK = 32;           // depth of a step
+constexpr int kNormBlocks = 64;   // partial sums of squares per matrix
+
+struct Planes { _Float16 *hi, *lo; };     // value = (hi + lo) / kPlaneScale
+
+struct WideArgs {
+    NsMatrix a;
+    int64_t n, len;               // short and long side
+    int64_t np, lp;               // padded to whole tiles (zeros)
+    Planes x, xt, g, p;           // X [np][lp], X^T [lp][np], X X^T and the polynomial [np][np]; per matrix
+    Planes xt_new;                // a step's X^T: other blocks still read the old one
+    int64_t x_plane, g_plane;     // elements of one matrix
+    double *norm;                 // [batch][kNormBlocks]
+    int32_t *shift;               // [batch]: e of the first step
+    float ca, cb, cc;
+    double eps;
+    int step, growth;             // a step multiplies X by at most 2^growth
+};
+
+// X is stored times 2^e, e = max(0, e_0 - step growth): |X| 2^e_0 is in [1/2, 1) before the first step where eps makes X small, and
+// e_0 = 0 otherwise.
+struct NsShift {
+    float now, next;
+};
+__device__ __forceinline__ NsShift ns_shift(const WideArgs &a, int64_t b) {
+    const int e0 = a.shift[b];
+    return NsShift{ldexpf(1.f, max(0, e0 - a.step * a.growth)), ldexpf(1.f, max(0, e0 - (a.step + 1) * a.growth))};
+}
+
+__device__ __forceinline__ void split16(float v, _Float16 &hi, _Float16 &lo) {
+    const float s = v * kPlaneScale;
+    hi = (_Float16)s;
+    lo = (_Float16)(s - (float)hi);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void ns_norm_kernel(WideArgs a) {
+    __shared__ double part[4];
+    const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.y * a.a.x_batch;
+    double s = 0;
+    for (int64_t i = blockIdx.x; i < a.a.m; i += gridDim.x)
+        for (int64_t j = threadIdx.x; j < a.a.n; j += 256) {
+            const double v = ns_load<T>(x + i * a.a.x_row + j);
+            s += v * v;
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.norm[blockIdx.y * kNormBlocks + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// X and X^T as planes, zero in the padding: 32 x 32 tiles through LDS
+template <typename T, bool TALL>
+__global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
+    __shared__ float tile[32][33];
+    double s = 0;
+    for (int k = 0; k < kNormBlocks; ++k) s += a.norm[blockIdx.z * kNormBlocks + k];
+    double inv = 1.0 / (sqrt(s) + a.eps);
+    const double unit = sqrt(s) * inv;                                     // |X|_F
+    const int e0 = unit > 0.0 && unit < 0.5 ? min(120, -ilogb(unit) - 1) : 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.shift[blockIdx.z] = e0;
+    inv = ldexp(inv, e0);
+    const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.z * a.a.x_batch;
+    const int64_t i0 = blockIdx.y * 32ll, j0 = blockIdx.x * 32ll;          // rows and columns of x
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t rows = TALL ? a.lp : a.np, cols = TALL ? a.np : a.lp;
+    Planes straight = TALL ? a.xt : a.x, turned = TALL ? a.x : a.xt;
+    straight.hi += blockIdx.z * a.x_plane; straight.lo += blockIdx.z * a.x_plane;
+    turned.hi += blockIdx.z * a.x_plane; turned.lo += blockIdx.z * a.x_plane;
+#pragma unroll
+    for (int r = 0; r < 32; r += 8) {
+        const int64_t i = i0 + ty + r, j = j0 + tx;
+        const float v = i < a.a.m && j < a.a.n ? (float)((double)ns_load<T>(x + i * a.a.x_row + j) * inv) : 0.f;
+        tile[ty + r][tx] = v;
+        _Float16 hi, lo;
+        split16(v, hi, lo);
+        straight.hi[i * cols + j] = hi;
+        straight.lo[i * cols + j] = lo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 32; r += 8) {
+        const int64_t j = j0 + ty + r, i = i0 + tx;
+        _Float16 hi, lo;
+        split16(tile[tx][ty + r], hi, lo);
+        turned.hi[j * rows + i] = hi;
+        turned.lo[j * rows + i] = lo;
+    }
+}
+
+// C = U V^T over depth K for planes U [.][K] and V [.][K], a 128 x 128 tile per block, 64 x 64 per wave.
+// MODE: what becomes of C.
+constexpr int kNsGram = 0, kNsPoly = 1, kNsStep = 2, kNsLast = 3;
+template <int MODE, typename T, bool TALL>
+__global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
+    __shared__ __attribute__((aligned(16))) _Float16 buf[2][4][kWT * kWK];        // two stages of U.hi U.lo V.hi V.lo
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t b = blockIdx.z;
+    int ti, tj;
+    if constexpr (MODE == kNsGram || MODE == kNsPoly) {
+        int t = blockIdx.x, tiles = (int)(a.np / kWT);                             // upper tiles, row by row
+        ti = 0;
+        while (t >= tiles - ti) { t -= tiles - ti; ++ti; }
+        tj = ti + t;
+    } else {
+        ti = blockIdx.x;
+        tj = blockIdx.y;
+    }
+    const int64_t K = MODE == kNsGram ? a.lp : a.np;
+    const int64_t uoff = MODE == kNsGram ? b * a.x_plane : b * a.g_plane;
+    const int64_t voff = MODE == kNsPoly ? b * a.g_plane : b * a.x_plane;
+    const Planes U = MODE == kNsGram ? a.x : (MODE == kNsPoly ? a.g : a.p);
+    const Planes V = MODE == kNsGram ? a.x : (MODE == kNsPoly ? a.g : a.xt);
+    const _Float16 *src[4] = {U.hi + uoff + ti * (int64_t)kWT * K, U.lo + uoff + ti * (int64_t)kWT * K,
+                              V.hi + voff + tj * (int64_t)kWT * K, V.lo + voff + tj * (int64_t)kWT * K};
+    // a wave stages one operand's tile: 128 rows of 64 bytes, eight loads of 64 lanes x 16 bytes straight into LDS
+    const _Float16 *mine = src[wave] + (lane >> 2) * K + (lane & 3) * 8;
+    auto stage = [&](int s, int64_t k) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(mine + c * 16 * K + k),
+                                             (__attribute__((address_space(3))) void *)(&buf[s][wave][c * 16 * kWK]), 16, 0, 0);
+    };
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+    const int frag = (lane & 15) * kWK + (lane >> 4) * 8;
+    // the loads of the other waves have to be in LDS too: each waits for its own before the barrier
+    auto arrived = [] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    stage(0, 0);
+    arrived();
+    int s = 0;
+    for (int64_t k = 0; k < K; k += kWK, s ^= 1) {
+        if (k + kWK < K) stage(s ^ 1, k + kWK);
+        f16x8 uh[4], ul[4], vh[4], vl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uh[i] = *reinterpret_cast<const f16x8 *>(&buf[s][0][(wi + 16 * i) * kWK + frag]);
+            ul[i] = *reinterpret_cast<const f16x8 *>(&buf[s][1][(wi + 16 * i) * kWK + frag]);
+            vh[i] = *reinterpret_cast<const f16x8 *>(&buf[s][2][(wj + 16 * i) * kWK + frag]);
+            vl[i] = *reinterpret_cast<const f16x8 *>(&buf[s][3][(wj + 16 * i) * kWK + frag]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[i], vh[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
+            }
+        arrived();
+    }
+    constexpr float kInv = 1.0f / (kPlaneScale * kPlaneScale);
+    const NsShift sh = ns_shift(a, b);
+    const float unscale = MODE == kNsGram ? kInv / sh.now / sh.now : (MODE == kNsStep ? kInv * (sh.next / sh.now) : (MODE == kNsLast ? kInv / sh.now : kInv));
+    const int n0 = lane & 15, m0 = (lane >> 4) * 4;                               // C: row m0 + r, column n0
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t row = ti * (int64_t)kWT + wi + 16 * i + m0, col = tj * (int64_t)kWT + wj + 16 * j + n0;
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * unscale;
+            if constexpr (MODE == kNsLast) {
+                T *out = reinterpret_cast<T *>(a.a.out) + b * a.a.out_batch;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row + r < a.n && col < a.len) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, row + r, col), v[r]);
+            } else {
+                const bool sym = MODE != kNsStep;
+                const Planes C = MODE == kNsGram ? a.g : (MODE == kNsPoly ? a.p : a.x);
+                const Planes Ct = MODE == kNsStep ? a.xt_new : C;
+                const int64_t off = sym ? b * a.g_plane : b * a.x_plane, ld = sym ? a.np : a.lp;
+                if constexpr (MODE == kNsPoly) {                                  // a I + b G + c G^2
+                    const int64_t at = off + col * a.np + row;                    // G is symmetric: four consecutive entries of its row `col`
+                    const f16x4 gh = *reinterpret_cast<const f16x4 *>(a.g.hi + at), gl = *reinterpret_cast<const f16x4 *>(a.g.lo + at);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        v[r] = a.cc * v[r] + a.cb * (((float)gh[r] + (float)gl[r]) * (1.0f / kPlaneScale)) + (row + r == col ? a.ca : 0.f);
+                }
+                f16x4 hi, lo;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    _Float16 h, l;
+                    split16(v[r], h, l);
+                    hi[r] = h;
+                    lo[r] = l;
+                    C.hi[off + (row + r) * ld + col] = h;
+                    C.lo[off + (row + r) * ld + col] = l;
+                }
+                if (!sym || ti != tj) {
+                    *reinterpret_cast<f16x4 *>(Ct.hi + off + col * a.np + row) = hi;
+                    *reinterpret_cast<f16x4 *>(Ct.lo + off + col * a.np + row) = lo;
+                }
+            }
+        }
+}
+
+// ---- entry points ------------------------------------------------------------------------------------------------------
+}  // namespace gatmi
+
+using namespace gatmi;
+
+static int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+static int gram_parts(int64_t batch, int64_t len) {
+    const int64_t per_matrix = std::max<int64_t>(1, 512 / std::max<int64_t>(1, batch));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kGramParts, per_matrix), (len + 127) / 128));
+}
+
+// Largest entry that X, X X^T or the polynomial can reach: |X|_2 <= s with s_0 = 1 and s_{k+1} = max over t in [0, s_k] of
+// |a t + b t^3 + c t^5|.  Extremes lie at the ends or where a derivative vanishes: g = t^2 = -b / 2c for the polynomial
+// a + b g + c g^2, the roots of a + 3 b g + 5 c g^2 for t times it.
+static double ns_bound(int steps, double a, double b, double c) {
+    double s = 1.0, worst = 1.0;
+    const double disc = 9 * b * b - 20 * a * c, root = std::sqrt(std::max(0.0, disc));
+    const double at[4] = {-b / (2 * c), (-3 * b + root) / (10 * c), (-3 * b - root) / (10 * c), -a / (3 * b)};      // the last for c = 0
+    for (int k = 0; k < steps; ++k) {
+        const double top = s * s;
+        auto poly = [&](double g) { return std::fabs(a + b * g + c * g * g); };
+        double next = s * poly(top);
+        worst = std::max(worst, std::max(poly(0.0), poly(top)));
+        for (double g : at)
+            if (g > 0.0 && g < top) {                             // false for the quotients by zero
+                next = std::max(next, std::sqrt(g) * poly(g));
+                worst = std::max(worst, poly(g));
+            }
+        s = next;
+        worst = std::max(worst, std::max(s, s * s));
+        if (!(worst < 1e6)) return 1e6;
+    }
+    return worst;
+}
+
+static size_t narrow_ws(int64_t batch, int64_t n, int64_t len) {
+    const size_t np = (size_t)round_up(n, 16);
+    return 2 * (size_t)batch * (gram_parts(batch, len) + 1) * np * np;
+}
+static size_t wide_head(int64_t batch) { return 2 * (size_t)batch * kNormBlocks + ((size_t)batch + 3) / 4 * 4; }      // norms and shifts
+static size_t wide_ws(int64_t batch, int64_t n, int64_t len) {
+    const size_t np = (size_t)round_up(n, kWT), lp = (size_t)round_up(len, kWT);
+    return wide_head(batch) + (size_t)batch * (3 * np * lp + 2 * np * np);      // planes of X, X^T twice, G, P: two fp16 a float
+}
+
+extern "C" size_t gatmi_newton_schulz_ws_floats(int64_t batch, int64_t m, int64_t n) {
+    if (batch <= 0 || m <= 0 || n <= 0) return 0;
+    const int64_t s = std::min(m, n), l = std::max(m, n);
+    const int64_t at_once = std::min<int64_t>(batch, kBatchAtOnce);
+    return s <= kNarrow ? narrow_ws(at_once, s, l) : wide_ws(at_once, s, l);
+}
+
+template <typename T, bool TALL>
+static int run_narrow(const NsMatrix &mat, int64_t batch, int steps, double ca, double cb, double cc, double eps, float *ws, hipStream_t st) {
+    NarrowArgs a;
+    a.a = mat;
+    a.n = (int)std::min(mat.m, mat.n);
+    a.len = std::max(mat.m, mat.n);
+    a.parts = gram_parts(batch, a.len);
+    a.per_part = round_up((a.len + a.parts - 1) / a.parts, 16);
+    a.steps = steps; a.ca = ca; a.cb = cb; a.cc = cc; a.eps = eps;
+    const int tiles = (a.n + 15) / 16, np = 16 * tiles;
+    a.gram = reinterpret_cast<double *>(ws);
+    a.q = a.gram + (size_t)batch * a.parts * np * np;
+    hipError_t e = hipSuccess;
+    const unsigned apply = (unsigned)std::min<int64_t>(1024, (a.len + 63) / 64);
+#define RUN(t)                                                                                                                              \
+    if (tiles == t) {                                                                                                                       \
+        const size_t one = (size_t)(16 * t) * (16 * t + 2) * sizeof(double);                                                                \
+        hipLaunchKernelGGL((ns_gram_kernel<T, TALL, t>), dim3(a.parts, (unsigned)batch), dim3(64), 0, st, a);                               \
+        if (3 * one > 48 * 1024) e = hipFuncSetAttribute(reinterpret_cast<const void *>(&ns_poly_kernel<t>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * one)); \
+        if (e != hipSuccess) return fail(GATMI_EHIP, "newton_schulz: %s", hipGetErrorString(e));                                            \
+        hipLaunchKernelGGL((ns_poly_kernel<t>), dim3((unsigned)batch), dim3(kNarrowThreads), 3 * one, st, a);                               \
+        hipLaunchKernelGGL((ns_apply_kernel<T, TALL, t>), dim3(apply, (unsigned)batch), dim3(256), one, st, a);                             \
+    }
+    RUN(1) RUN(2) RUN(3) RUN(4)
+#undef RUN
+    GATMI_LAUNCH_CHECK("newton_schulz");
+    return GATMI_OK;
+}
+
+template <typename T, bool TALL>
+static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, double cb, double cc, double eps, float *ws, hipStream_t st) {
+    WideArgs a;
+    a.a = mat;
+    a.n = std::min(mat.m, mat.n);
+    a.len = std::max(mat.m, mat.n);
+    a.np = round_up(a.n, kWT);
+    a.lp = round_up(a.len, kWT);
+    a.x_plane = a.np * a.lp;
+    a.g_plane = a.np * a.np;
+    a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.eps = eps;
+    a.growth = std::max(1, (int)std::ceil(std::log2(ns_bound(steps, ca, cb, cc))));
+    a.norm = reinterpret_cast<double *>(ws);
+    a.shift = reinterpret_cast<int32_t *>(ws + 2 * (size_t)batch * kNormBlocks);
+    _Float16 *p = reinterpret_cast<_Float16 *>(ws + wide_head(batch));
+    const size_t xs = (size_t)batch * a.x_plane, gs = (size_t)batch * a.g_plane;
+    a.x = {p, p + xs};
+    a.xt = {p + 2 * xs, p + 3 * xs};
+    a.xt_new = {p + 4 * xs, p + 5 * xs};
+    a.g = {p + 6 * xs, p + 6 * xs + gs};
+    a.p = {p + 6 * xs + 2 * gs, p + 6 * xs + 3 * gs};
+    hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);
+    const int64_t rows = TALL ? a.lp : a.np, cols = TALL ? a.np : a.lp;
+    hipLaunchKernelGGL((ns_split_kernel<T, TALL>), dim3((unsigned)(cols / 32), (unsigned)(rows / 32), (unsigned)batch), dim3(256), 0, st, a);
+    const unsigned tn = (unsigned)(a.np / kWT), tl = (unsigned)(a.lp / kWT), sym = tn * (tn + 1) / 2;
+    for (int k = 0; k < steps; ++k) {
+        a.step = k;
+        hipLaunchKernelGGL((ns_gemm_kernel<kNsGram, T, TALL>), dim3(sym, 1, (unsigned)batch), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((ns_gemm_kernel<kNsPoly, T, TALL>), dim3(sym, 1, (unsigned)batch), dim3(256), 0, st, a);
+        if (k + 1 < steps) {
+            hipLaunchKernelGGL((ns_gemm_kernel<kNsStep, T, TALL>), dim3(tn, tl, (unsigned)batch), dim3(256), 0, st, a);
+            std::swap(a.xt, a.xt_new);
+        } else {
+            hipLaunchKernelGGL((ns_gemm_kernel<kNsLast, T, TALL>), dim3(tn, tl, (unsigned)batch), dim3(256), 0, st, a);
+        }
+    }
+    GATMI_LAUNCH_CHECK("newton_schulz");
+    return GATMI_OK;
+}
+
+extern "C" int gatmi_newton_schulz(int64_t batch, int64_t m, int64_t n, const void *x, int64_t x_batch, int64_t x_row, int32_t dtype, int32_t steps,
+                                   double a, double b, double c, double eps, void *out, int64_t out_batch, int64_t out_row, float *ws, void *stream) {
+    GATMI_REQUIRE(batch >= 0 && m >= 0 && n >= 0, GATMI_EINVAL, "newton_schulz: batch = %lld, m = %lld, n = %lld", (long long)batch, (long long)m, (long long)n);
+    GATMI_REQUIRE(dtype == GATMI_DTYPE_F32 || dtype == GATMI_DTYPE_BF16, GATMI_EINVAL, "newton_schulz: dtype %d", dtype);
+    GATMI_REQUIRE(steps >= 1 && steps <= kMaxSteps, GATMI_EINVAL, "newton_schulz: %d steps (1 to %d)", steps, kMaxSteps);
+    GATMI_REQUIRE(eps > 0.0 && eps < 1.0, GATMI_EINVAL, "newton_schulz: eps = %g (above 0, below 1)", eps);
+    GATMI_REQUIRE(std::isfinite(a) && std::isfinite(b) && std::isfinite(c), GATMI_EINVAL, "newton_schulz: coefficients %g, %g, %g", a, b, c);
+    const double worst = ns_bound(steps, a, b, c);
+    GATMI_REQUIRE(worst <= kMaxEntry, GATMI_EUNSUPPORTED,
+                  "newton_schulz: with a = %g, b = %g, c = %g the iteration can reach %g in %d steps (at most %g): the coefficients do not keep the singular values bounded",
+                  a, b, c, worst, steps, kMaxEntry);
+    if (batch == 0 || m == 0 || n == 0) return GATMI_OK;
+    GATMI_REQUIRE(x && out && ws, GATMI_EINVAL, "newton_schulz: null pointer");
+    GATMI_REQUIRE_ALIGNED(ws);
+    GATMI_REQUIRE(x_row >= n || m == 1, GATMI_EINVAL, "newton_schulz: row stride %lld below n = %lld", (long long)x_row, (long long)n);
+    GATMI_REQUIRE(out_row >= n || m == 1, GATMI_EINVAL, "newton_schulz: row stride %lld of the result below n = %lld", (long long)out_row, (long long)n);
+    const bool tall = m > n, narrow = std::min(m, n) <= kNarrow;
+    GATMI_REQUIRE(narrow || std::max(m, n) <= kMaxSide, GATMI_ERANGE, "newton_schulz: a side of %lld (at most %lld)", (long long)std::max(m, n), (long long)kMaxSide);
+    hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int64_t size = dtype == GATMI_DTYPE_F32 ? 4 : 2;
+    for (int64_t b0 = 0; b0 < batch; b0 += kBatchAtOnce) {
+        NsMatrix mat{static_cast<const char *>(x) + b0 * x_batch * size, static_cast<char *>(out) + b0 * out_batch * size, x_batch, x_row, out_batch, out_row, m, n};
+        const int64_t now = std::min(kBatchAtOnce, batch - b0);
+        int rc;
+#define RUN(T)                                                                                                                                  rc = narrow ? (tall ? run_narrow<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_narrow<T, false>(mat, now, steps, a, b, c, eps, ws, st))                 : (tall ? run_wide<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_wide<T, false>(mat, now, steps, a, b, c, eps, ws, st))
+        if (dtype == GATMI_DTYPE_F32) RUN(float);
+        else RUN(uint16_t);
+#undef RUN
+        if (rc) return rc;
+    }
+    return GATMI_OK;
+}

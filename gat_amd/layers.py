@@ -250,13 +250,16 @@ class VariableStore(nn.Module):
     def begin(self):
         self._cursor = 0
 
-    def next_heads(self, f_in, heads, width, residual, device):
+    def next_heads(self, f_in, heads, width, residual, device, kind=None):
+        kind = GATHeads if kind is None else kind
         if self._cursor == len(self.layers):
-            self.layers.append(GATHeads(f_in, heads, width, residual, device))
+            self.layers.append(kind(f_in, heads, width, residual=residual, device=device))
         m = self.layers[self._cursor]
         if (m.f_in, m.heads, m.width) != (f_in, heads, width):
             raise ValueError("variable %d was created for (f_in,heads,width)=%s, now asked for %s"
                              % (self._cursor, (m.f_in, m.heads, m.width), (f_in, heads, width)))
+        if type(m) is not kind:
+            raise ValueError("variable %d was created as %s, now asked for as %s" % (self._cursor, type(m).__name__, kind.__name__))
         self._cursor += 1
         return m
 
@@ -313,6 +316,83 @@ def sp_attn_head(seq, out_sz, adj_mat, activation, nb_nodes, in_drop=0.0, coef_d
     (indices, values, shape) triple of preprocess_adj_bias (utils/process.py:188) or a CSRGraph."""
     training = in_drop != 0.0 or coef_drop != 0.0
     return sp_attn_heads(seq, out_sz, adj_mat, activation, nb_nodes, 1, "concat", in_drop, coef_drop, residual, training)
+
+
+class DotHeads(nn.Module):
+    """Attention heads scored by dot products over the same additive mask as GATHeads (utils/layers.py:16-18 with
+    scale <q_i, k_j> in place of f_1 + f_2):  act(softmax(q k^T / sqrt(D) + bias_mat) v + bias).
+    W [F, H + 2 G, D]: the query kernels of the H heads, then the key and the value kernels of the G = kv_heads shared heads (H
+    unless given); bias [H, D]; W_res / b_res as in GATHeads.  One projection, one attention launch for all heads.
+    storage="bf16": the rows the attention reads are rounded to bf16 (sums and softmax stay fp32)."""
+
+    def __init__(self, f_in, heads, width, kv_heads=None, residual=False, device=None, storage="f32"):
+        super().__init__()
+        if storage not in ("f32", "bf16"):
+            raise ValueError("storage must be 'f32' or 'bf16'")
+        self.f_in, self.heads, self.width = int(f_in), int(heads), int(width)
+        self.kv_heads = self.heads if kv_heads is None else int(kv_heads)
+        if self.kv_heads < 1 or self.heads % self.kv_heads:
+            raise ValueError("%d query heads do not share %d key/value heads evenly" % (self.heads, self.kv_heads))
+        self.storage = storage
+        kw = {"device": device, "dtype": torch.float32}
+        self.W = nn.Parameter(torch.empty(f_in, self.heads + 2 * self.kv_heads, width, **kw))
+        self.bias = nn.Parameter(torch.zeros(heads, width, **kw))
+        self.has_res = bool(residual) and f_in != width
+        if self.has_res:
+            self.W_res = nn.Parameter(torch.empty(f_in, heads, width, **kw))
+            self.b_res = nn.Parameter(torch.zeros(heads, width, **kw))
+        lim = math.sqrt(6.0 / (self.f_in + self.width))
+        with torch.no_grad():
+            self.W.uniform_(-lim, lim)
+            if self.has_res:
+                self.W_res.uniform_(-lim, lim)
+
+    def forward(self, seq, bias_mat, activation="elu", reduce="concat", sizes=None):
+        """seq [B,N,F], bias_mat [B or 1,N,N] or None, sizes int32 [B]: nodes of each graph (rows behind them give act(bias))."""
+        act = _activation_name(activation)
+        if reduce not in ("concat", "mean"):
+            raise ValueError("reduce must be 'concat' or 'mean'")
+        if act != "identity" and reduce == "mean":
+            raise ValueError("mean over heads is defined for the identity activation (models/sp_gat.py:30-32)")
+        B, N, F = seq.shape
+        H, G, D = self.heads, self.kv_heads, self.width
+        rows = ops.tall_linear(seq, self.W.reshape(F, -1).t()).reshape(B, N, H + 2 * G, D)
+        if self.storage == "bf16":
+            rows = rows.to(torch.bfloat16)
+        q, k, v = rows[:, :, :H], rows[:, :, H:H + G], rows[:, :, H + G:]
+        out = ops.dot_attention(q, k, v, bias_mat, key_sizes=sizes, query_sizes=sizes).to(seq.dtype).reshape(B, N, H * D)
+        if self.has_res:
+            out = out + ops.tall_linear(seq, self.W_res.reshape(F, -1).t(), self.b_res.reshape(-1))
+        out = ops.add_row_bias(out, self.bias.reshape(-1), act)
+        return out.reshape(B, N, H, D).mean(2) if reduce == "mean" else out
+
+
+def dot_attn_heads(seq, out_sz, bias_mat, activation, n_heads, reduce="concat", in_drop=0.0, residual=False, sizes=None):
+    """n_heads dot-product heads over bias_mat, variables from the active VariableStore; a non-zero in_drop drops seq."""
+    if in_drop != 0.0:
+        seq = torch.nn.functional.dropout(seq, in_drop, True)
+    m = default_store().next_heads(seq.shape[-1], n_heads, out_sz, residual, seq.device, DotHeads)
+    return m(seq, bias_mat, activation, reduce, sizes)
+
+
+def dot_attn_head(seq, out_sz, bias_mat, activation, in_drop=0.0, residual=False):
+    """attn_head (utils/layers.py:6) with dot-product scores: seq [B,N,F], bias_mat [B,N,N] additive mask; returns [B,N,out_sz]."""
+    return dot_attn_heads(seq, out_sz, bias_mat, activation, 1, "concat", in_drop, residual)
+
+
+class NodeEmbedding(nn.Module):
+    """Learned input rows of nodes without features (or beside them): scale * weight[ids], ids of any shape; an id outside
+    [0, rows) is a padded node: zeros and no gradient.  Equal to one-hot SparseFeatures times weight, without the CSR of them."""
+
+    def __init__(self, rows, width, scale=1.0, device=None, dtype=torch.float32):
+        super().__init__()
+        self.scale = float(scale)
+        self.weight = nn.Parameter(torch.empty(rows, width, device=device, dtype=dtype))
+        with torch.no_grad():
+            self.weight.normal_(0.0, 1.0 / math.sqrt(width))
+
+    def forward(self, ids):
+        return ops.embedding(ids, self.weight, self.scale)
 
 
 class BNFAttention(nn.Module):

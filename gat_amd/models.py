@@ -85,6 +85,78 @@ class TFAdam(torch.optim.Optimizer):
         return loss
 
 
+def matrix_parameters(module):
+    """(matrices, others) of a module built from this package's layers and torch.nn.Linear: `matrices` lists (parameter, head axis)
+    of every kernel that multiplies rows — the axis along which a 3-d kernel holds one matrix per head, None for a plain
+    [out, in] weight — and `others` what is left (biases, logit vectors, embeddings, normalisation)."""
+    found = {}
+    for m in module.modules():
+        if isinstance(m, torch.nn.Linear):
+            found[id(m.weight)] = (m.weight, None)
+        elif isinstance(m, (layers.GATHeads, layers.DotHeads, layers.BNFAttention)):
+            for name in ("W", "W_res"):
+                if getattr(m, name, None) is not None:
+                    found[id(getattr(m, name))] = (getattr(m, name), 1)
+        elif isinstance(m, layers.AttnE2VBNFV2):
+            for w in m.head_w:
+                found[id(w)] = (w, 0)
+    return list(found.values()), [p for p in module.parameters() if id(p) not in found]
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update of every matrix is orthogonalised (ops.newton_schulz) before it is applied:
+        m = momentum m + g;  u = g + momentum m (nesterov) or m;  W -= lr sqrt(max(1, out / in)) orth(u);  W *= 1 - lr weight_decay first.
+    params: (parameter, head axis) pairs as matrix_parameters gives them, or plain 2-d [out, in] parameters.  A 3-d kernel
+    [F, H, D] (head axis 1) is one F x D matrix per head, as the reference creates them (tf.layers.conv1d per head,
+    utils/layers.py:11); [H, F, D] has head axis 0.  Matrices of one shape share one call.  What is not a matrix goes to TFAdam.
+    step() only enqueues: it can be captured (gat_amd.graphs.capture); lr is then frozen."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
+        if lr < 0.0 or not 0.0 <= momentum < 1.0 or weight_decay < 0.0 or steps < 1:
+            raise ValueError("Muon: lr = %r, momentum = %r, weight_decay = %r, steps = %r" % (lr, momentum, weight_decay, steps))
+        by_axis = {}
+        for entry in params:
+            p, axis = entry if isinstance(entry, (tuple, list)) else (entry, None)
+            if p.dim() != (2 if axis is None else 3) or axis not in (None, 0, 1):
+                raise ValueError("Muon: a parameter of shape %s with head axis %r is not a matrix or a set of them" % (tuple(p.shape), axis))
+            by_axis.setdefault(axis, []).append(p)
+        super().__init__([dict(params=ps, head_axis=axis) for axis, ps in by_axis.items()],
+                         dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            for p in ps:
+                if "m" not in self.state[p]:
+                    self.state[p]["m"] = torch.zeros_like(p)
+            gs, ms = [p.grad for p in ps], [self.state[p]["m"] for p in ps]
+            torch._foreach_mul_(ms, group["momentum"])
+            torch._foreach_add_(ms, gs)
+            us = torch._foreach_add(gs, ms, alpha=group["momentum"]) if group["nesterov"] else ms
+            if group["weight_decay"]:
+                torch._foreach_mul_(ps, 1.0 - group["lr"] * group["weight_decay"])
+            axis = group["head_axis"]
+            same = {}
+            for p, u in zip(ps, us):
+                if axis is not None:                      # one [in, out] matrix per head
+                    p, u = p.movedim(axis, 0), u.movedim(axis, 0)
+                same.setdefault((u.shape, u.dtype, u.device), []).append((p, u))
+            for (shape, _, _), pairs in same.items():
+                out, inp = (shape[-2], shape[-1]) if axis is None else (shape[-1], shape[-2])
+                u = pairs[0][1][None] if len(pairs) == 1 else torch.stack([u for _, u in pairs])
+                o = ops.newton_schulz(u, steps=group["steps"])
+                rate = -group["lr"] * max(1.0, out / inp) ** 0.5
+                torch._foreach_add_([p for p, _ in pairs], list(o.unbind(0)), alpha=rate)
+        return loss
+
+
 class _L2Penalty(torch.autograd.Function):
     """coef * sum_v 0.5 ||v||^2 over a list of tensors with a handful of launches in each direction
     (horizontally fused norms forward, one fused scaling backward: d/dv = coef * v).  Written per

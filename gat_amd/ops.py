@@ -5,6 +5,9 @@ the autograd tape; every floating-point operation of the layer runs in the HIP k
 Math and reference lines: utils/layers.py:6-34 (one head), models/sp_gat.py:12-17,27-32 (heads
 concatenated or averaged).
 """
+import ctypes
+import math
+
 import torch
 
 from . import _lib
@@ -851,3 +854,196 @@ def inner_product_decoder(z, activation="sigmoid", dropout=0.0, seed=None):
     if seed is None:
         seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if keep < 1.0 else 0
     return InnerProductDecoderFn.apply(z, act, keep, int(seed))
+
+
+# ------------------------------------------------------------------------------------------------
+# dot-product attention, learned rows, orthogonalised updates
+# ------------------------------------------------------------------------------------------------
+_FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _float_type(what, *ts):
+    """Code of the one dtype (fp32 or bf16) that all tensors share."""
+    if ts[0].dtype not in _FLOATS or any(t.dtype != ts[0].dtype for t in ts):
+        raise TypeError("%s: fp32 or bf16 tensors of one type expected, got %s" % (what, ", ".join(str(t.dtype) for t in ts)))
+    return _FLOATS[ts[0].dtype]
+
+
+def _same_device(what, *ts):
+    _require_cuda(*ts)
+    devs = {t.device for t in ts if t is not None}
+    if len(devs) > 1:
+        raise ValueError("%s: tensors on different devices: %s" % (what, ", ".join(sorted(map(str, devs)))))
+    return ts[0].device
+
+
+def _strides(t):
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _attn_rows(t, width):
+    """t [B, N, heads, D] as rows the kernels take: D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
+    if t.shape[-1] != width:
+        return torch.nn.functional.pad(t, (0, width - t.shape[-1]))
+    unit = 16 // t.element_size()
+    if t.stride(3) == 1 and all(s % unit == 0 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class DotAttentionFn(torch.autograd.Function):
+    """out = softmax(scale q k^T + bias) v per graph and head (gatmi_dot_attn_fwd / _bwd); see dot_attention."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, key_sizes, query_sizes, scale):
+        B, Nq, H, D = q.shape
+        Nk, Hkv = k.shape[1], k.shape[2]
+        dtype = _FLOATS[q.dtype]
+        unit = 4 if dtype == _lib.DTYPE_F32 else 8
+        width = (D + unit - 1) // unit * unit
+        qr, kr, vr = (_attn_rows(t, width) for t in (q, k, v))
+        out = torch.empty((B, Nq, H, width), dtype=q.dtype, device=q.device)
+        need = any(ctx.needs_input_grad[:3])
+        lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if need else None
+        floats = _lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, Hkv, width)
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        bb, br = (0, Nk) if bias is None else (bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1))
+        with torch.cuda.device(q.device):
+            _lib.call("gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, ptr(qr), _strides(qr), ptr(kr), _strides(kr), ptr(vr), _strides(vr),
+                      ptr(bias), bb, br, ptr(key_sizes), ptr(query_sizes), scale, ptr(out), ptr(lse), ptr(ws), _lib.current_stream())
+        if need:
+            ctx.save_for_backward(qr, kr, vr, out, lse, bias, key_sizes, query_sizes)
+            ctx.scale, ctx.D, ctx.bias_strides = scale, D, (bb, br)
+        return out[..., :D] if width != D else out
+
+    @staticmethod
+    def backward(ctx, dout):
+        qr, kr, vr, out, lse, bias, key_sizes, query_sizes = ctx.saved_tensors
+        B, Nq, H, width = qr.shape
+        Nk, Hkv = kr.shape[1], kr.shape[2]
+        D = ctx.D
+        dr = _attn_rows(dout, width)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (qr, kr, vr))
+        delta = torch.empty_like(lse)
+        with torch.cuda.device(qr.device):
+            _lib.call("gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], ptr(qr), _strides(qr), ptr(kr), _strides(kr), ptr(vr), _strides(vr),
+                      ptr(out), ptr(dr), _strides(dr), ptr(lse), ptr(bias), *ctx.bias_strides, ptr(key_sizes), ptr(query_sizes), ctx.scale,
+                      ptr(dq), ptr(dk), ptr(dv), ptr(delta), _lib.current_stream())
+        if width != D:
+            dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
+        return dq, dk, dv, None, None, None, None
+
+
+def _sizes(what, sizes, B, device):
+    if sizes is None:
+        return None
+    if not torch.is_tensor(sizes) or sizes.dtype != torch.int32 or tuple(sizes.shape) != (B,):
+        raise ValueError("%s: an int32 tensor of %d sizes expected" % (what, B))
+    if sizes.device != device:
+        raise ValueError("%s is on %s, the rows are on %s" % (what, sizes.device, device))
+    return sizes.contiguous()
+
+
+def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, scale=None):
+    """Dot-product attention with the additive mask of utils/process.py:14-25:
+        out[b,i,h] = sum_j softmax_j(scale <q[b,i,h], k[b,j,g]> + bias_mat[b,i,j]) v[b,j,g],   g = h // (H / Hkv)
+    q [B,Nq,H,D], k and v [B,Nk,Hkv,D] (H a multiple of Hkv, D at most 128), fp32 or bf16; any strides (rows that are not
+    16-byte aligned are copied once).  Nq = 1 answers for single nodes.  scale: D ** -0.5 unless given.
+    bias_mat [B or 1, Nq, Nk] fp32 (or None): an entry not above -1e8 is not attended; it takes no gradient.
+    key_sizes, query_sizes: int32 [B] on the same device: rows behind a graph's own nodes are neither read nor given a
+    gradient, and their outputs are zeros.  A row without an attended key gives zeros.  Rows of k and v inside key_sizes have to be
+    finite also where the mask leaves them out.  The backward recomputes the probabilities and adds in a fixed order."""
+    what = "dot_attention"
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not torch.is_tensor(t) or t.dim() != 4:
+            raise ValueError("%s: %s is [batch, nodes, heads, width], got %s" % (what, name, tuple(t.shape) if torch.is_tensor(t) else type(t)))
+    _float_type(what, q, k, v)
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("%s: q %s, k %s, v %s do not belong together" % (what, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if Hkv < 1 or H % Hkv:
+        raise ValueError("%s: %d query heads do not share %d key/value heads evenly" % (what, H, Hkv))
+    if not 1 <= D <= 128:
+        raise ValueError("%s: head width %d is not in 1..128" % (what, D))
+    dev = _same_device(what, q, k, v, bias_mat)
+    if bias_mat is not None:
+        if bias_mat.dtype != torch.float32 or bias_mat.dim() != 3 or bias_mat.shape[0] not in (1, B) or tuple(bias_mat.shape[1:]) != (Nq, Nk):
+            raise ValueError("%s: bias_mat is fp32 [%d or 1, %d, %d], got %s %s" % (what, B, Nq, Nk, bias_mat.dtype, tuple(bias_mat.shape)))
+        if bias_mat.requires_grad:
+            raise ValueError("%s: bias_mat takes no gradient; detach it" % what)
+        if bias_mat.stride(2) != 1 or bias_mat.stride(1) < Nk:
+            bias_mat = bias_mat.contiguous()
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    return DotAttentionFn.apply(q, k, v, bias_mat, _sizes("key_sizes", key_sizes, B, dev), _sizes("query_sizes", query_sizes, B, dev), scale)
+
+
+class EmbeddingFn(torch.autograd.Function):
+    """scale * table[ids] and the table's gradient by sorted ids (gatmi_embed_fwd / _bwd); see embedding."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale):
+        rows, width = table.shape
+        dtype = _FLOATS[table.dtype]
+        flat = ids.reshape(-1)
+        flat = flat if flat.is_contiguous() else flat.contiguous()
+        tb = table if table.stride(1) == 1 and table.stride(0) >= width else table.contiguous()
+        out = torch.empty((flat.numel(), width), dtype=table.dtype, device=table.device)
+        with torch.cuda.device(table.device):
+            _lib.call("gatmi_embed_fwd", ptr(flat), 8 * flat.element_size(), flat.numel(), ptr(tb), tb.stride(0), rows, width, dtype, scale, ptr(out),
+                      _lib.current_stream())
+        ctx.save_for_backward(flat)
+        ctx.scale, ctx.rows = scale, rows
+        return out.reshape(*ids.shape, width)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (flat,) = ctx.saved_tensors
+        n, rows, width = flat.numel(), ctx.rows, dout.shape[-1]
+        d = dout.reshape(n, width)
+        d = d if d.stride(1) == 1 and d.stride(0) >= width else d.contiguous()
+        grad = torch.empty((rows, width), dtype=dout.dtype, device=dout.device)
+        ws = torch.empty(_lib.lib.gatmi_embed_bwd_ws_floats(n, rows, width), dtype=torch.float32, device=dout.device)
+        with torch.cuda.device(dout.device):
+            _lib.call("gatmi_embed_bwd", ptr(flat), 8 * flat.element_size(), n, ptr(d), d.stride(0), rows, width, _FLOATS[dout.dtype], ctx.scale,
+                      ptr(grad), ptr(ws), _lib.current_stream())
+        return None, grad, None
+
+
+def embedding(ids, table, scale=1.0):
+    """scale * table[ids]: a learned row per id.  ids int32 or int64 of any shape, table [rows, width] fp32 or bf16; returns
+    [*ids.shape, width].  An id outside [0, rows) stands for padding: a row of zeros, no gradient.  The gradient of the table is
+    summed in fp32 in the order of the tokens of each row (the ids are sorted with their positions): the same bits every run."""
+    if not torch.is_tensor(ids) or ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("embedding: ids are int32 or int64, got %s" % (ids.dtype if torch.is_tensor(ids) else type(ids)))
+    if not torch.is_tensor(table) or table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError("embedding: table is [rows, width], got %s" % (tuple(table.shape) if torch.is_tensor(table) else type(table),))
+    _float_type("embedding", table)
+    _same_device("embedding", table, ids)
+    return EmbeddingFn.apply(ids, table, float(scale))
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # a, b, c of the quintic usual for orthogonalised updates: steep at 0, and [0.7, 1.2] maps into itself
+
+
+@torch.no_grad()
+def newton_schulz(x, steps=5, eps=1e-7, coefficients=NEWTON_SCHULZ):
+    """Every m x n matrix of x [..., m, n] (fp32 or bf16) with its singular values driven towards 1: from X = x / (|x|_F + eps), `steps`
+    times X <- a X + b (X X^T) X + c (X X^T)^2 X, at fp32 accuracy whatever the type (gatmi_newton_schulz).  Outside autograd."""
+    if not torch.is_tensor(x) or x.dim() < 2:
+        raise ValueError("newton_schulz: x is [..., m, n], got %s" % (tuple(x.shape) if torch.is_tensor(x) else type(x),))
+    dtype = _float_type("newton_schulz", x)
+    _require_cuda(x)
+    m, n = x.shape[-2:]
+    x3 = x.reshape(math.prod(x.shape[:-2]), m, n)
+    if x3.stride(2) != 1 or x3.stride(1) < n:
+        x3 = x3.contiguous()
+    out = torch.empty(x3.shape, dtype=x.dtype, device=x.device)
+    a, b, c = (float(v) for v in coefficients)
+    batch = x3.shape[0]
+    ws = torch.empty(_lib.lib.gatmi_newton_schulz_ws_floats(batch, m, n), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.call("gatmi_newton_schulz", batch, m, n, ptr(x3), x3.stride(0), x3.stride(1), dtype, int(steps), a, b, c, float(eps),
+                  ptr(out), m * n, n, ptr(ws), _lib.current_stream())
+    return out.reshape(x.shape)

@@ -551,6 +551,52 @@ int gatmi_ipd_fwd(int64_t B, int32_t N, int32_t F, const float *Z, int32_t activ
 int gatmi_ipd_bwd(int64_t B, int32_t N, int32_t F, const float *dOut, const float *out,
                   const float *Z, int32_t activation, float keep, uint64_t seed, float *dZ, void *stream);
 
+/* Scaled dot-product attention over the additive mask of utils/process.py:14-25 (the scoring of attn_head,
+ * utils/layers.py:15-18, replaced by scale * <q_i, k_j>), forward and backward.
+ *   q [B, Nq, H, D], k, v [B, Nk, Hkv, D] fp32 or bf16 (dtype), given by the element strides of graph, node and head (three
+ *   int64 each); D contiguous, D a multiple of 4 (fp32) or 8 (bf16), at most 128; rows 16-byte aligned.  Query head h reads the
+ *   key/value head h / (H / Hkv).  out contiguous [B, Nq, H, D].
+ *   bias: optional fp32 [B, Nq, Nk] with strides bias_batch (0: one mask for all graphs), bias_row, 1.  An entry whose bias is
+ *   not above -1e8 is not attended.  key_sizes, query_sizes: optional int32 [B] on the device, clamped to [0, Nk] / [0, Nq]; keys behind
+ *   theirs are not read, queries behind theirs give zeros and take no part in the gradients.  A row without an
+ *   attended key gives zeros.
+ *   fwd: lse [B, H, Nq] (log2 of the row's sum of exponentials; NULL when no backward follows).  ws: gatmi_dot_attn_fwd_ws_floats
+ *   (0: may be NULL); few rows on many keys are split over the keys and joined.
+ *   bwd: the probabilities are formed again from lse; dq [B, Nq, H, D], dk, dv [B, Nk, Hkv, D] contiguous, written whole; delta
+ *   [B, H, Nq] is scratch.  No atomics: the same bits every run. */
+size_t gatmi_dot_attn_fwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D);
+int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype,
+                       const void *q, const int64_t *q_stride, const void *k, const int64_t *k_stride,
+                       const void *v, const int64_t *v_stride, const float *bias, int64_t bias_batch, int64_t bias_row,
+                       const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse,
+                       float *ws, void *stream);
+int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype,
+                       const void *q, const int64_t *q_stride, const void *k, const int64_t *k_stride,
+                       const void *v, const int64_t *v_stride, const void *out, const void *dout, const int64_t *dout_stride,
+                       const float *lse, const float *bias, int64_t bias_batch, int64_t bias_row,
+                       const int32_t *key_sizes, const int32_t *query_sizes, float scale,
+                       void *dq, void *dk, void *dv, float *delta, void *stream);
+
+/* Learned rows by id.  ids: int32 or int64 (id_bits 32 / 64) [tokens]; an id outside [0, rows) is padding.
+ *   fwd: out[t, :] = scale * table[ids[t], :] (zeros for padding); table rows ld_table elements apart, out contiguous.
+ *   bwd: dtable [rows, width] (contiguous, written whole) = scale * sum over the tokens of each row of dout[t, :] (rows ld_dout
+ *   elements apart), summed in fp32 in token order: the same bits every run.  ws: gatmi_embed_bwd_ws_floats.
+ *   tokens and rows below 2^31, width at most 65536; dtype of table / out / dout / dtable: fp32 or bf16. */
+int gatmi_embed_fwd(const void *ids, int32_t id_bits, int64_t tokens, const void *table, int64_t ld_table, int64_t rows,
+                    int32_t width, int32_t dtype, float scale, void *out, void *stream);
+size_t gatmi_embed_bwd_ws_floats(int64_t tokens, int64_t rows, int32_t width);
+int gatmi_embed_bwd(const void *ids, int32_t id_bits, int64_t tokens, const void *dout, int64_t ld_dout, int64_t rows,
+                    int32_t width, int32_t dtype, float scale, void *dtable, float *ws, void *stream);
+
+/* Newton-Schulz orthogonalisation of a batch of m x n matrices (an update's singular values driven towards 1): from
+ * X = x / (|x|_F + eps), `steps` (1..32) times X <- a X + b (X X^T) X + c (X X^T)^2 X.  x, out: fp32 or bf16, element
+ * (i, j) of matrix b at b * batch stride + i * row stride + j; fp32 accuracy throughout, one rounding at the end.
+ * GATMI_EUNSUPPORTED when (a, b, c) let the iteration's entries pass 7.5 within `steps`. */
+size_t gatmi_newton_schulz_ws_floats(int64_t batch, int64_t m, int64_t n);
+int gatmi_newton_schulz(int64_t batch, int64_t m, int64_t n, const void *x, int64_t x_batch, int64_t x_row, int32_t dtype,
+                        int32_t steps, double a, double b, double c, double eps,
+                        void *out, int64_t out_batch, int64_t out_row, float *ws, void *stream);
+
 /* Halo exchange helpers (row-partitioned multi-GPU).  pack: dst[k, :] = src[idx[k], :] for
  * k < n_idx, rows of `width` floats (send buffer of Wh / f2 rows requested by a peer); rows are
  * moved 16 bytes per lane when width is a multiple of 4, one float per lane otherwise.

@@ -1,0 +1,292 @@
+"""GPU parity of ops.dot_attention, forward and gradients, against its 64-bit form within counted rounding bounds: types, head
+layouts, lengths from one row to long ones, masks that leave rows empty, padded graphs, strides, streams and captured graphs."""
+import numpy as np
+import pytest
+import torch
+
+from tests import attn_ref
+from tests.attn_ref import within
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _case(B, Nq, Nk, H, G, D, dtype, density=None, shared_mask=False, sizes=False, seed=0, soft=False):
+    rng = np.random.default_rng(seed)
+    dev = torch.device("cuda:0")
+    t = lambda *s: torch.tensor(rng.normal(0, 1, s), dtype=torch.float32).to(TYPES[dtype]).to(dev)
+    c = {"q": t(B, Nq, H, D), "k": t(B, Nk, G, D), "v": t(B, Nk, G, D), "dout": t(B, Nq, H, D), "bias": None, "ks": None, "qs": None}
+    if density is not None:
+        bm = np.where(rng.random((1 if shared_mask else B, Nq, Nk)) < density, 0.0, -1e9)
+        if soft:
+            bm = np.where(bm == 0.0, rng.normal(0, 2, bm.shape), bm)
+        if Nq > 2:
+            bm[:, 1] = -1e9                                              # a row that the mask leaves empty
+        c["bias"] = torch.tensor(bm, dtype=torch.float32, device=dev)
+    if sizes:
+        ks = rng.integers(0, Nk + 1, B)
+        ks[0] = Nk
+        if B > 2:
+            ks[1], ks[2] = 0, 1
+        c["ks"] = torch.tensor(ks, dtype=torch.int32, device=dev)
+        c["qs"] = c["ks"] if Nq == Nk else torch.tensor(rng.integers(0, Nq + 1, B), dtype=torch.int32, device=dev)
+    return c
+
+
+def _np(x):
+    return None if x is None else x.detach().double().cpu().numpy()
+
+
+def _run(c, grad=True, scale=None):
+    from gat_amd import ops
+    leaves = [c[n].detach().requires_grad_(grad) for n in ("q", "k", "v")]
+    out = ops.dot_attention(*leaves, c["bias"], key_sizes=c["ks"], query_sizes=c["qs"], scale=scale)
+    res = {"out": out.detach()}
+    if grad:
+        res.update(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, c["dout"])))
+    return res
+
+
+def _check(c, dtype, grad=True, scale=None, what=""):
+    got = _run(c, grad, scale)
+    ref = attn_ref.attention(_np(c["q"]), _np(c["k"]), _np(c["v"]), _np(c["bias"]), _np(c["ks"]), _np(c["qs"]), scale,
+                             _np(c["dout"]) if grad else None, dtype == "bf16")
+    for n, (value, bound) in ref.items():
+        assert got[n].dtype == TYPES[dtype]
+        within(got[n].double().cpu().numpy(), value, bound, "%s %s" % (what, n))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [8, 16, 20, 32, 64, 100, 128])
+def test_every_width(D, dtype):
+    _check(_case(2, 70, 70, 4, 2, D, dtype, density=0.3, seed=D), dtype, what="D=%d" % D)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [1, 3, 7, 13])
+def test_widths_that_no_vector_divides(D, dtype):
+    _check(_case(2, 33, 33, 2, 2, D, dtype, density=0.5, seed=D), dtype, what="D=%d" % D)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("Nq,Nk", [(1, 1), (1, 2), (2, 1), (1, 64), (1, 65), (15, 17), (16, 16), (17, 63), (63, 64), (64, 63), (65, 65), (127, 129),
+                                   (128, 128), (129, 127), (1, 300), (300, 1), (246, 246), (264, 264)])
+def test_lengths(Nq, Nk, dtype):
+    _check(_case(2, Nq, Nk, 2, 2, 16, dtype, density=0.4 if Nk > 8 else None, seed=Nq + Nk), dtype, what="%dx%d" % (Nq, Nk))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("H,G", [(1, 1), (3, 1), (6, 6), (6, 2), (8, 2), (12, 4), (5, 5), (16, 1)])
+def test_head_layouts(H, G, dtype):
+    _check(_case(2, 37, 50, H, G, 32, dtype, density=0.3, seed=H), dtype, what="%d/%d" % (H, G))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shared,soft", [(False, True), (True, False), (True, True)])
+def test_masks(shared, soft, dtype):
+    _check(_case(3, 90, 90, 4, 4, 16, dtype, density=0.1, shared_mask=shared, soft=soft), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("Nq,Nk,density", [(70, 70, None), (70, 70, 0.3), (5, 130, None), (130, 70, 0.5)])
+def test_padded_graphs(Nq, Nk, density, dtype):
+    _check(_case(5, Nq, Nk, 4, 2, 24, dtype, density=density, sizes=True, seed=Nk), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_behind_the_sizes_are_not_read(dtype):
+    c = _case(4, 70, 70, 2, 2, 16, dtype, sizes=True, seed=3)
+    want = _run(c)
+    for n in ("q", "k", "v", "dout"):
+        x = c[n].clone()
+        for b in range(4):
+            x[b, int(c["ks"][b]):] = float("nan")
+        c[n] = x
+    got = _run(c)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+        for b in range(4):
+            assert (got[n][b, int(c["ks"][b]):] == 0).all()
+
+
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float32).min, -1e9, float("nan")])
+def test_lowest_masks_and_empty_rows(low):
+    c = _case(2, 40, 40, 2, 2, 8, "f32", density=0.2, seed=5)
+    want = _run(c)
+    c["bias"] = torch.where(c["bias"] < -1e8, torch.full_like(c["bias"], low), c["bias"])
+    got = _run(c)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    assert (got["out"][:, 1] == 0).all() and (got["dq"][:, 1] == 0).all()
+
+
+def test_nothing_attended_at_all():
+    c = _case(2, 20, 30, 2, 1, 16, "f32", density=0.5)
+    c["bias"].fill_(-1e9)
+    for n, x in _run(c).items():
+        assert (x == 0).all(), n
+
+
+def test_nan_and_inf_in_an_attended_row_stay_visible():
+    c = _case(1, 20, 20, 1, 1, 8, "f32")
+    c["q"][0, 3] = float("nan")
+    out = _run(c, grad=False)["out"]
+    assert out[0, 3].isnan().all() and out[0, 4:].isfinite().all() and out[0, :3].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,Nq,Nk,H,G,D", [(1, 1, 512, 1, 1, 64), (1, 1, 5000, 8, 2, 64), (2, 3, 3001, 4, 1, 128), (1, 40, 2000, 2, 2, 8), (3, 1, 777, 6, 3, 100),
+                                           (1, 1, 70001, 4, 4, 16)])
+def test_few_rows_on_many_keys(B, Nq, Nk, H, G, D, dtype):
+    """Split over the keys; also with ranges that no key of a graph falls into, and gradients behind it."""
+    from gat_amd import _lib
+    assert _lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, G, (D + 7) // 8 * 8) > 0
+    c = _case(B, Nq, Nk, H, G, D, dtype, seed=Nk)
+    _check(c, dtype, grad=Nk <= 5000)
+    c["ks"] = torch.tensor([(Nk, 5, 0)[b % 3] for b in range(B)][::-1], dtype=torch.int32, device="cuda:0")
+    _check(c, dtype, grad=Nk <= 5000)
+
+
+@pytest.mark.parametrize("scale", [0.0, 3.0, -0.5])
+def test_scale(scale):
+    _check(_case(1, 50, 50, 2, 2, 16, "f32", density=0.5), "f32", scale=scale)
+
+
+def test_large_logits():
+    c = _case(1, 60, 60, 2, 2, 16, "f32")
+    c["q"] *= 30
+    _check(c, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_strided_rows_equal_contiguous_ones(dtype):
+    """Slices of one projection's output, a transposed layout, an offset that is not 16-byte aligned, an expanded gradient."""
+    from gat_amd import ops
+    dev = torch.device("cuda:0")
+    B, N, H, D = 2, 45, 4, 16
+    g = torch.Generator(device=dev).manual_seed(1)
+    rows = torch.randn((B, N, 3 * H, D), device=dev, generator=g).to(TYPES[dtype])
+    q, k, v = rows[:, :, :H], rows[:, :, H:2 * H], rows[:, :, 2 * H:]
+    want = ops.dot_attention(q.contiguous(), k.contiguous(), v.contiguous())
+    assert torch.equal(ops.dot_attention(q, k, v), want)
+    turned = lambda x: x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    assert torch.equal(ops.dot_attention(turned(q), k, turned(v)), want)
+    odd = torch.empty(B * N * H * D + 1, dtype=TYPES[dtype], device=dev)[1:].view(B, N, H, D)
+    odd.copy_(q)
+    assert odd.data_ptr() % 16 != 0
+    assert torch.equal(ops.dot_attention(odd, k, v), want)
+    leaf = q.contiguous().requires_grad_()
+    a = torch.autograd.grad(ops.dot_attention(leaf, k, v).sum(), leaf)[0]                  # gradient: one value expanded
+    b = torch.autograd.grad(ops.dot_attention(leaf, k, v), leaf, torch.ones_like(leaf))[0]
+    assert torch.equal(a, b)
+    wide = torch.full((B, N, 2 * N), -1e9, device=dev)
+    wide[:, :, :N] = torch.where(torch.rand((B, N, N), device=dev, generator=g) < 0.3, 0.0, -1e9)
+    assert torch.equal(ops.dot_attention(q, k, v, wide[:, :, :N]), ops.dot_attention(q, k, v, wide[:, :, :N].contiguous()))
+    mask_t = wide[:, :, :N].transpose(1, 2)
+    assert torch.equal(ops.dot_attention(q, k, v, mask_t), ops.dot_attention(q, k, v, mask_t.contiguous()))
+
+
+def test_empty_shapes():
+    from gat_amd import ops
+    dev = torch.device("cuda:0")
+    z = lambda *s: torch.zeros(s, device=dev, requires_grad=True)
+    for B, Nq, Nk in ((0, 4, 4), (2, 0, 4), (2, 4, 0), (2, 0, 0)):
+        q, k, v = z(B, Nq, 2, 8), z(B, Nk, 2, 8), z(B, Nk, 2, 8)
+        out = ops.dot_attention(q, k, v)
+        assert out.shape == q.shape and (out == 0).all()
+        for x, g in zip((q, k, v), torch.autograd.grad(out, (q, k, v), torch.ones_like(out))):
+            assert g.shape == x.shape and (g == 0).all()
+
+
+def test_twice_the_same_bits_and_on_another_stream():
+    c = _case(3, 100, 100, 6, 2, 64, "bf16", density=0.2)
+    want = _run(c)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(c)
+    torch.cuda.current_stream().wait_stream(side)
+    again = _run(c)
+    for n in want:
+        assert torch.equal(want[n], got[n]) and torch.equal(want[n], again[n]), n
+
+
+def test_captured_forward_and_backward():
+    """Replays with new inputs, eager work of the same sizes and synchronisations between them."""
+    from gat_amd import graphs, ops
+    c = _case(2, 90, 90, 4, 2, 32, "f32", density=0.2)
+    q, k, v = (c[n].clone().requires_grad_() for n in ("q", "k", "v"))
+
+    def step():
+        out = ops.dot_attention(q, k, v, c["bias"])
+        return (out, *torch.autograd.grad(out, (q, k, v), c["dout"]))
+
+    replay, res = graphs.capture(step, fresh_dropout=False)
+    one_query = _case(1, 1, 3000, 4, 2, 32, "f32", seed=9)                       # split over the keys: a workspace of its own
+    replay_one, res_one = graphs.capture(lambda: ops.dot_attention(one_query["q"], one_query["k"], one_query["v"]), fresh_dropout=False)
+    for seed in range(4):
+        n = _case(2, 90, 90, 4, 2, 32, "f32", density=0.2, seed=seed)
+        with torch.no_grad():
+            for a, b in ((q, n["q"]), (k, n["k"]), (v, n["v"])):
+                a.copy_(b)
+            c["bias"].copy_(n["bias"])
+            c["dout"].copy_(n["dout"])
+            one_query["q"].copy_(_case(1, 1, 3000, 4, 2, 32, "f32", seed=20 + seed)["q"])
+        replay()
+        replay_one()
+        torch.cuda.synchronize()
+        want = _run(n)
+        for got, name in zip(res, ("out", "dq", "dk", "dv")):
+            assert torch.equal(got, want[name]), (seed, name)
+        assert torch.equal(res_one, ops.dot_attention(one_query["q"], one_query["k"], one_query["v"]))
+
+
+def test_gradient_against_differences():
+    """d/dt of <out(x + t d), dout> from outputs at t = +-h: truncation is h^2 times a third derivative of order 1, rounding 1e-6 / h."""
+    from gat_amd import ops
+    c = _case(2, 30, 30, 4, 2, 16, "f32", density=0.4, soft=True, seed=11)
+    got = _run(c)
+    rng = np.random.default_rng(1)
+    h = 1e-2
+    for n, g in (("q", "dq"), ("k", "dk"), ("v", "dv")):
+        d = torch.tensor(rng.normal(0, 1, c[n].shape), dtype=torch.float32, device="cuda:0")
+        d /= d.norm()
+
+        def f(t):
+            x = {m: c[m] + t * d if m == n else c[m] for m in ("q", "k", "v")}
+            return (ops.dot_attention(x["q"], x["k"], x["v"], c["bias"]).double() * c["dout"].double()).sum().item()
+
+        slope = (f(h) - f(-h)) / (2 * h)
+        assert abs(slope - (got[g].double() * d.double()).sum().item()) < 1e-3 * got[g].norm().item() + 1e-3
+
+
+def test_wide_batch_and_long_rows():
+    """More graphs than a grid dimension of 65535 holds; offsets that pass 2^31 elements."""
+    from gat_amd import ops
+    dev = torch.device("cuda:0")
+    q = torch.randn((70000, 2, 1, 8), device=dev)
+    out = ops.dot_attention(q, q, q)
+    for b in (0, 1, 65535, 65536, 69999):
+        value, bound = attn_ref.attention(*(_np(q[b:b + 1]),) * 3)["out"]
+        within(_np(out[b:b + 1]), value, bound, "graph %d" % b)
+    k = torch.zeros((1, 17_000_000, 1, 128), dtype=torch.bfloat16, device=dev)              # 2.2e9 elements
+    k[0, -1] = 1.0
+    v = torch.zeros_like(k)
+    v[0, -1] = 2.0
+    one = torch.full((1, 1, 1, 128), 30.0, dtype=torch.bfloat16, device=dev)                # the last key's score is 339, all others are 0
+    assert (ops.dot_attention(one, k, v) == 2.0).all()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_shapes(seed):
+    rng = np.random.default_rng(1000 + seed)
+    G = int(rng.choice([1, 2, 3, 4]))
+    H = G * int(rng.choice([1, 1, 2, 3]))
+    same = rng.random() < 0.5
+    Nq = int(rng.integers(1, 300))
+    Nk = Nq if same else int(rng.integers(1, 400))
+    dtype = str(rng.choice(["f32", "bf16"]))
+    c = _case(int(rng.integers(1, 5)), Nq, Nk, H, G, int(rng.integers(1, 129)), dtype, density=float(rng.choice([0.05, 0.5, 1.0])) if rng.random() < 0.7 else None,
+              sizes=bool(rng.random() < 0.5), soft=bool(rng.random() < 0.3), seed=seed)
+    _check(c, dtype, what="seed %d: %s" % (seed, [tuple(c[n].shape) for n in ("q", "k")]))
