@@ -36,19 +36,28 @@ struct __attribute__((packed, aligned(4))) f32x4_u { float v[4]; };       // a 1
 constexpr float kAttended = -1e8f;
 constexpr int kSplitsMax = 256;
 
-// ---- operand fragments -------------------------------------------------------------------------------------------------
-// DP: head width padded to what is staged.  A fragment is what a lane holds of 16 rows x KD elements: lane (r = l & 15,
-// q = l >> 4) the PIECE bytes at q * PIECE of the fragment's part of row r.
-template <typename T, int DP> struct Shape;
-template <int DP> struct Shape<float, DP> {
-    static constexpr int PIECE = DP == 8 ? 8 : 16, KD = PIECE, FRAGS = DP / KD;           // PIECE bytes = PIECE / 4 elements, 4 lane groups: KD = PIECE elements
-    static constexpr int ROW = DP * 4, PAD = ROW + 16;                                    // bytes of a staged row, and its stride in LDS
-    static constexpr int CHUNK = 16;                                                      // rows that one fragment of the second product covers
-};
-template <int DP> struct Shape<uint16_t, DP> {
-    static constexpr int PIECE = 16, KD = 32, FRAGS = DP < 32 ? 1 : DP / 32;
-    static constexpr int ROW = (DP < 32 ? 32 : DP) * 2, PAD = ROW + 16;
-    static constexpr int CHUNK = 32;
+// ---- rows in LDS and operand fragments -----------------------------------------------------------------------------------
+// Staged rows are DP elements wide and lie in LDS without padding, because the loads go straight from memory to LDS (64 lanes
+// write 1 KB in lane order).  Instead the 16-byte pieces of row r are permuted by an exclusive or with a number made of r, so that the lanes of
+// one LDS read, which want the same piece of many rows, find them in different banks.
+// A fragment is what a lane holds of 16 rows x KD elements: lane (n = l & 15, q = l >> 4) the PIECE bytes at q * PIECE of the
+// fragment's part of row n.
+template <typename T, int DP> struct Shape {
+    static constexpr int SIZE = (int)sizeof(T), ROW = DP * SIZE, CPR = ROW / 16;         // bytes and 16-byte pieces of a row
+    static constexpr bool NARROW = ROW == 32;                                              // one fragment of 8 bytes a lane
+    static constexpr int PIECE = NARROW ? 8 : 16, FRAGS = ROW / (4 * PIECE), ELEMS = PIECE / SIZE, KD = 4 * ELEMS;
+    static constexpr int CHUNK = SIZE == 4 ? 16 : 32;                                      // rows that one fragment of the second product covers
+    static constexpr int KT = (SIZE == 4 && DP == 128) ? 32 : 64;                         // rows of a staged tile
+    static constexpr int DT = (DP + 15) / 16;                                            // 16-wide tiles of a result row
+    static constexpr int KTW = ROW >= 512 ? 16 : (ROW >= 128 ? 32 : 64);               // where each wave stages tiles of its own
+    static constexpr int TILE = KT * ROW;
+    // 16-row tiles of a wave: two where the accumulators and operands of two fit the 256 registers that leave two waves on a SIMD
+    static constexpr int NQ = SIZE == 4 && DP >= 64 ? 1 : 2, NK = ROW >= 256 ? 1 : 2;
+    __device__ static __forceinline__ int swizzle(int r) {      // the same for r and r + 16
+        if constexpr (CPR >= 16) return r & 15;
+        else return (r / (16 / CPR)) & (CPR - 1);
+    }
+    __device__ static __forceinline__ int at(int r, int byte) { return r * ROW + (((byte >> 4) ^ swizzle(r)) << 4) + (byte & 15); }
 };
 
 struct FragF { float v[4]; };
@@ -59,15 +68,9 @@ template <> struct FragOf<uint16_t> { using type = FragH; };
 template <typename T> using Frag = typename FragOf<T>::type;
 
 template <typename T, int DP>
-__device__ __forceinline__ Frag<T> frag_zero() {
-    if constexpr (sizeof(T) == 4) return FragF{{0.f, 0.f, 0.f, 0.f}};
-    else return FragH{make_uint4(0, 0, 0, 0)};
-}
-// from 16-byte aligned memory (8 for DP = 8)
-template <typename T, int DP>
 __device__ __forceinline__ Frag<T> frag_load(const char *p) {
     if constexpr (sizeof(T) == 4) {
-        if constexpr (DP == 8) {
+        if constexpr (Shape<T, DP>::NARROW) {
             const float2 u = *reinterpret_cast<const float2 *>(p);
             return FragF{{u.x, u.y, 0.f, 0.f}};
         } else {
@@ -75,8 +78,30 @@ __device__ __forceinline__ Frag<T> frag_load(const char *p) {
             return FragF{{u.x, u.y, u.z, u.w}};
         }
     } else {
-        return FragH{*reinterpret_cast<const uint4 *>(p)};
+        if constexpr (Shape<T, DP>::NARROW) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p);
+            return FragH{make_uint4(u.x, u.y, 0, 0)};
+        } else {
+            return FragH{*reinterpret_cast<const uint4 *>(p)};
+        }
     }
+}
+// the fragments of one row in memory: zeros behind its D elements and where there is no row
+template <typename T, int DP>
+__device__ __forceinline__ void row_frags(const T *row, int D, bool ok, Frag<T> (&f)[Shape<T, DP>::FRAGS]) {
+    using S = Shape<T, DP>;
+    const int q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int c = 0; c < S::FRAGS; ++c) {
+        const int e = c * S::KD + q * S::ELEMS;
+        if (ok && e < D) f[c] = frag_load<T, DP>(reinterpret_cast<const char *>(row + e));
+        else f[c] = Frag<T>{};
+    }
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_negated(Frag<T> f) {
+    if constexpr (sizeof(T) == 4) return FragF{{-f.v[0], -f.v[1], -f.v[2], -f.v[3]}};
+    else return FragH{make_uint4(f.v.x ^ 0x80008000u, f.v.y ^ 0x80008000u, f.v.z ^ 0x80008000u, f.v.w ^ 0x80008000u)};
 }
 
 // acc += A B over the KD elements of one fragment
@@ -84,11 +109,16 @@ template <typename T, int DP>
 __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int t = 0; t < (DP == 8 ? 2 : 4); ++t) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[t], b.v[t], acc, 0, 0, 0);
+        for (int t = 0; t < Shape<T, DP>::ELEMS; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[t], b.v[t], acc, 0, 0, 0);
+    } else if constexpr (Shape<T, DP>::NARROW) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, make_uint2(a.v.x, a.v.y)), __builtin_bit_cast(i16x4, make_uint2(b.v.x, b.v.y)), acc, 0, 0, 0);
     } else {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), acc, 0, 0, 0);
     }
 }
+// acc += A B over the CHUNK rows of one fragment of the second product
+template <typename T>
+__device__ __forceinline__ void mma_rows(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) { mma<T, 64>(a, b, acc); }
 
 // The second product sums over CHUNK staged rows.  Its B operand is made of score tiles (C layout: row 4 q + r of a
 // tile in register r), its A operand reads the staged rows column-wise in the same order of rows.
@@ -97,27 +127,32 @@ __device__ __forceinline__ Frag<T> frag_scores(const f32x4 *tile) {
     if constexpr (sizeof(T) == 4) return FragF{{tile[0][0], tile[0][1], tile[0][2], tile[0][3]}};
     else return FragH{make_uint4(pack_bf16x2(tile[0][0], tile[0][1]), pack_bf16x2(tile[0][2], tile[0][3]), pack_bf16x2(tile[1][0], tile[1][1]), pack_bf16x2(tile[1][2], tile[1][3]))};
 }
+// row0 a multiple of CHUNK, d0 of 16
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> frag_turned(const char *tile, int row0, int d0) {
+    using S = Shape<T, DP>;
     const int lane = threadIdx.x & 63;
     if constexpr (sizeof(T) == 4) {
-        const char *p = tile + (row0 + 4 * (lane >> 4)) * Shape<T, DP>::PAD + (d0 + (lane & 15)) * 4;
+        const int n = DP == 8 ? lane & 7 : lane & 15;                  // DP = 8: the upper eight columns are not used
         FragF f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const float *>(p + r * Shape<T, DP>::PAD);
+        for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const float *>(tile + S::at(row0 + 4 * (lane >> 4) + r, (d0 + n) * 4));
         return f;
     } else {
         // ds_read_b64_tr_b16: 16 lanes give the addresses of a 4 x 16 block (lane i: row i / 4, columns 4 (i % 4) ..), each gets a column of it
-        const char *p = tile + (row0 + 4 * (lane >> 4) + ((lane & 15) >> 2)) * Shape<T, DP>::PAD + (d0 + (lane & 3) * 4) * 2;
+        const char *p = tile + S::at(row0 + 4 * (lane >> 4) + ((lane & 15) >> 2), (d0 + (lane & 3) * 4) * 2);
         using lds4 = __attribute__((address_space(3))) i16x4;
         const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 16 * Shape<T, DP>::PAD));
+        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 16 * S::ROW));
         return FragH{__builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7))};
     }
 }
-// acc += A B over the rows of one such fragment (fp32: always four steps)
-template <typename T>
-__device__ __forceinline__ void mma_rows(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) { mma<T, 16>(a, b, acc); }
+template <typename T, int DP>
+__device__ __forceinline__ Frag<T> frag_row(const char *tile, int row0, int c) {
+    using S = Shape<T, DP>;
+    const int lane = threadIdx.x & 63;
+    return frag_load<T, DP>(tile + S::at(row0 + (lane & 15), c * 4 * S::PIECE + (lane >> 4) * S::PIECE));
+}
 
 // ---- arguments ---------------------------------------------------------------------------------------------------------
 struct DotRows {              // [B, N, heads, D] rows: element strides, D contiguous
@@ -133,81 +168,98 @@ struct DotArgs {
     int64_t bias_batch, bias_row;
     const int32_t *key_sizes, *query_sizes;
     int64_t b0;                         // first graph of this launch
-    int B, Nq, Nk, H, Hkv, group, D;
+    int B, Nq, Nk, H, Hkv, group, D;    // B: graphs of this launch
     int tiles, splits;                  // row (or key) tiles, key ranges
-    int split_keys;                     // keys of a range
-    float scale;
-    float *part_o, *part_ml;            // split forward: [rows of the launch][splits][DP], [..][2]
+    float scale, scale2;                // scale2 = |scale| log2 e; the sign is carried by q
+    float *part_o, *part_ml;            // split forward: [rows of the launch][splits][D], [..][2]
 };
 
 __device__ __forceinline__ int graph_size(const int32_t *sizes, int64_t b, int n) { return sizes ? max(0, min(sizes[b], n)) : n; }
 
-// one 16-byte (8-byte) piece of a row, zeros outside it
-template <typename T, int DP>
-__device__ __forceinline__ Frag<T> row_piece(const T *row, int elem, int D, bool ok) {
-    return ok && elem < D ? frag_load<T, DP>(reinterpret_cast<const char *>(row + elem)) : frag_zero<T, DP>();
+// Which (graph, key/value head, tile, split) a block of the 1-d grid works on.  Blocks go to the eight dies in turn and each die has an
+// L2 of its own.  What shares data forms a group whose blocks go to one die, next to each other: without a mask the tiles of one
+// (graph, head), which read the same keys and values; with a mask the heads of one (graph, tile, split), which read the same part of it.
+// Groups are dealt to the dies in turn (so that graphs of unequal sizes spread), the last groups that do not fill a round are cut into eight equal pieces.
+struct DotBlock { int64_t b; int hk, tile, split; bool ok; };
+template <bool BIAS>
+__device__ __forceinline__ DotBlock dot_block(const DotArgs &a) {
+    const uint32_t inner = BIAS ? a.Hkv : a.tiles * a.splits, groups = BIAS ? (uint32_t)a.B * a.tiles * a.splits : (uint32_t)a.B * a.Hkv;
+    const uint32_t die = blockIdx.x & 7, at = blockIdx.x >> 3, whole = groups / 8 * inner;       // blocks of a die that belong to whole rounds
+    uint32_t group = at / inner * 8 + die, i = at % inner;
+    DotBlock r;
+    r.ok = true;
+    if (at >= whole) {
+        const uint32_t rest = groups % 8 * inner, per = (rest + 7) / 8, item = die * per + (at - whole);
+        r.ok = at - whole < per && item < rest;
+        group = groups / 8 * 8 + item / inner;
+        i = item % inner;
+    }
+    if constexpr (BIAS) {
+        r.hk = i;
+        r.split = group % a.splits; group /= a.splits;
+        r.tile = group % a.tiles;
+        r.b = a.b0 + group / a.tiles;
+    } else {
+        r.split = i % a.splits;
+        r.tile = i / a.splits;
+        r.hk = group % a.Hkv;
+        r.b = a.b0 + group / a.Hkv;
+    }
+    return r;
 }
 
-// ---- staging of KT rows of two tensors -----------------------------------------------------------------------------------
-template <typename T, int DP, int KT, int THREADS>
-struct Stage {
+// ---- staging: KT rows of two tensors, straight from memory to LDS by WAVES waves --------------------------------------------
+// Rows behind the last one and pieces behind D are replaced by ones that exist: what is computed from them is masked, multiplied
+// by zeros of the other operand, or not stored.  row(x, r): element offset of row r (r < count).
+template <typename T, int DP, int KT, int WAVES, typename Row>
+__device__ __forceinline__ void stage(char *lds, const DotRows &x, const DotRows &y, int count, int D, int wave, Row &&row) {
     using S = Shape<T, DP>;
-    static constexpr int PIECES = S::ROW / S::PIECE, TOTAL = KT * PIECES, PER = (TOTAL + THREADS - 1) / THREADS, ELEMS = S::PIECE / (int)sizeof(T);
-    Frag<T> a[PER], b[PER];
-    // row r of the tile: rows.p + offset(r), valid while r < count
-    template <typename Off>
-    __device__ __forceinline__ void load(const DotRows &x, const DotRows &y, int count, int D, Off &&offset) {
+    constexpr int LOADS = KT * S::ROW / 1024, TOTAL = 2 * LOADS;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int e = threadIdx.x + u * THREADS, r = e / PIECES, c = (e % PIECES) * ELEMS;
-            const bool ok = (TOTAL % THREADS == 0 || e < TOTAL) && r < count && c < D;
-            if (ok) {
-                a[u] = frag_load<T, DP>(reinterpret_cast<const char *>(reinterpret_cast<const T *>(x.p) + offset(x, r) + c));
-                b[u] = frag_load<T, DP>(reinterpret_cast<const char *>(reinterpret_cast<const T *>(y.p) + offset(y, r) + c));
-            } else {
-                a[u] = frag_zero<T, DP>();
-                b[u] = frag_zero<T, DP>();
-            }
+    for (int u = 0; u < (TOTAL + WAVES - 1) / WAVES; ++u) {
+        const int load = u * WAVES + wave;                                  // the same for the whole wave
+        if (TOTAL % WAVES == 0 || load < TOTAL) {
+            const bool second = load >= LOADS;
+            const DotRows &z = second ? y : x;
+            const int piece = (load - (second ? LOADS : 0)) * 64 + lane, r = piece / S::CPR;
+            int c = (piece % S::CPR) ^ S::swizzle(r);
+            c = c * (16 / S::SIZE) < D ? c : 0;
+            const T *src = reinterpret_cast<const T *>(z.p) + row(z, min(r, count - 1)) + c * (16 / S::SIZE);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                             (__attribute__((address_space(3))) void *)(lds + load * 1024), 16, 0, 0);
         }
     }
-    __device__ __forceinline__ void put(char *p, const Frag<T> &f) const {
-        if constexpr (sizeof(T) == 4) {
-            if constexpr (DP == 8) *reinterpret_cast<float2 *>(p) = make_float2(f.v[0], f.v[1]);
-            else *reinterpret_cast<float4 *>(p) = make_float4(f.v[0], f.v[1], f.v[2], f.v[3]);
-        } else {
-            *reinterpret_cast<uint4 *>(p) = f.v;
-        }
-    }
-    __device__ __forceinline__ void store(char *x, char *y) const {
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int e = threadIdx.x + u * THREADS, r = e / PIECES, c = e % PIECES;
-            if (TOTAL % THREADS == 0 || e < TOTAL) {
-                put(x + r * S::PAD + c * S::PIECE, a[u]);
-                put(y + r * S::PAD + c * S::PIECE, b[u]);
-            }
-        }
-    }
-};
+}
+// what this wave (BLOCK: every wave) has asked for is in LDS; nobody reads the other buffer any more
+template <bool BLOCK>
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (BLOCK) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+}
 
-// z of four consecutive keys j .. j + 3 of one query, -inf where the key is not attended
-__device__ __forceinline__ void masked_logits(f32x4 &z, float scale, const float *bias_row, int j, int nk, int keys) {
-    if (bias_row) {
-        float bv[4];
-        if (j + 3 < nk) {
-            const f32x4_u u = *reinterpret_cast<const f32x4_u *>(bias_row + j);
+// biases of four consecutive keys of one query, -inf behind the row
+__device__ __forceinline__ f32x4 bias4(const float *row, int j, int nk) {
+    f32x4 v;
+    if (j + 3 < nk) {
+        const f32x4_u u = *reinterpret_cast<const f32x4_u *>(row + j);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) bv[r] = u.v[r];
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bv[r] = j + r < nk ? bias_row[j + r] : -INFINITY;
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = bv[r] > kAttended && j + r < keys ? fmaf(z[r], scale, bv[r]) : -INFINITY;
+        for (int r = 0; r < 4; ++r) v[r] = u.v[r];
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) z[r] = j + r < keys ? z[r] * scale : -INFINITY;
+        for (int r = 0; r < 4; ++r) v[r] = j + r < nk ? row[j + r] : -INFINITY;
     }
+    return v;
+}
+// scores of four keys in units of log2 from raw products, -inf where a key is not attended
+__device__ __forceinline__ f32x4 masked_scores(f32x4 z, float scale2, f32x4 bias, int j, int keys) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[r] = bias[r] > kAttended && j + r < keys ? fmaf(z[r], scale2, bias[r] * kLog2e) : -INFINITY;
+    return z;
+}
+__device__ __forceinline__ bool some_attended(f32x4 bias) {
+    return __ballot(fmaxf(fmaxf(bias[0], bias[1]), fmaxf(bias[2], bias[3])) > kAttended) != 0;
 }
 
 __device__ __forceinline__ float over_groups_max(float v) {
@@ -226,55 +278,45 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {
     else *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
-// which (graph, key/value head, tile, split) a block of the 1-d grid works on
-struct DotBlock { int64_t b; int hk, tile, split; };
-__device__ __forceinline__ DotBlock dot_block(const DotArgs &a) {
-    DotBlock r;
-    uint32_t id = blockIdx.x;
-    r.split = id % a.splits; id /= a.splits;
-    r.tile = id % a.tiles; id /= a.tiles;
-    r.hk = id % a.Hkv;
-    r.b = a.b0 + id / a.Hkv;
-    return r;
-}
-
-template <typename T, int DP> struct Tiles {
-    static constexpr int KT = (sizeof(T) == 4 && DP == 128) ? 32 : 64;      // staged rows: both tensors' tiles stay below 64 KB
-    static constexpr int DT = (DP + 15) / 16;                              // 16-wide tiles of a result row
-    static constexpr int LDS = 2 * KT * Shape<T, DP>::PAD;
-};
-
 // ---- forward -------------------------------------------------------------------------------------------------------------
-// WAVES x NQ x 16 rows per block.  SPLIT: the block covers one range of the keys and leaves its unnormalised row sums.
-template <typename T, int DP, int WAVES, int NQ, bool SPLIT>
-__global__ __launch_bounds__(64 * WAVES) void dot_fwd_kernel(DotArgs a) {
+// A wave owns NQ x 16 rows.  KEYW = false: four waves with rows of their own walk the staged tiles together.  KEYW = true: for 16 rows or
+// fewer, the four waves have the same rows and walk different tiles, each staging its own, and join at the end.
+// SPLIT: the block covers one range of the keys and leaves its unnormalised sums.
+template <typename T, int DP, bool KEYW, int NQ, bool SPLIT, bool BIAS>
+__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
     using S = Shape<T, DP>;
-    using TL = Tiles<T, DP>;
-    constexpr int KT = TL::KT, DT = TL::DT, ROWS = WAVES * NQ * 16;
-    __shared__ __attribute__((aligned(16))) char lds[TL::LDS];
-    char *ks = lds, *vs = lds + KT * S::PAD;
+    constexpr int KT = KEYW ? S::KTW : S::KT, TILE = KT * S::ROW, KS = KT / 16, DT = S::DT, ROWS = KEYW ? 16 : 64 * NQ, OWNERS = KEYW ? 4 : 1, STEP = OWNERS * KT;
+    constexpr bool ONES = DP == 8 && S::SIZE == 4;              // eight columns of the last product are free: one of them sums the probabilities
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const DotBlock blk = dot_block<BIAS>(a);
+    if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
-    const DotBlock blk = dot_block(a);
     const int64_t b = blk.b;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
-    const int j0 = SPLIT ? blk.split * a.split_keys : 0, j1 = SPLIT ? min(keys, j0 + a.split_keys) : keys;
+    const int share = SPLIT ? ((keys + a.splits - 1) / a.splits + 63) / 64 * 64 : keys;           // of this graph's own keys
+    const int j0 = SPLIT ? blk.split * share : 0, j1 = min(keys, j0 + share);
+    char *const mine = lds + (KEYW ? wave * 4 * TILE : 0);
+    auto buf = [&](int at) { return mine + at * 2 * TILE; };
     int row[NQ], qi[NQ], head[NQ];
     bool live[NQ];
     Frag<T> qf[NQ][S::FRAGS];
     const float *bias_row[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
-        row[u] = blk.tile * ROWS + (wave * NQ + u) * 16 + n;
+        row[u] = blk.tile * ROWS + ((KEYW ? 0 : wave) * NQ + u) * 16 + n;
         qi[u] = row[u] / a.group;
-        head[u] = blk.hk * a.group + row[u] % a.group;
+        head[u] = blk.hk * a.group + row[u] - qi[u] * a.group;
         live[u] = qi[u] < queries;
-        const T *qrow = reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + (live[u] ? qi[u] : 0) * a.q.node + head[u] * a.q.head;
+        const int64_t i = live[u] ? qi[u] : 0;
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + i * a.q.node + head[u] * a.q.head, a.D, live[u], qf[u]);
+        if (a.scale < 0.f) {
 #pragma unroll
-        for (int c = 0; c < S::FRAGS; ++c) qf[u][c] = row_piece<T, DP>(qrow, c * S::KD + q4 * (S::PIECE / (int)sizeof(T)), a.D, live[u]);
-        bias_row[u] = a.bias ? a.bias + b * a.bias_batch + (int64_t)(live[u] ? qi[u] : 0) * a.bias_row : nullptr;
+            for (int c = 0; c < S::FRAGS; ++c) qf[u][c] = frag_negated<T>(qf[u][c]);
+        }
+        bias_row[u] = BIAS ? a.bias + b * a.bias_batch + i * a.bias_row : nullptr;
     }
     f32x4 o[NQ][DT];
-    float m[NQ], l[NQ];
+    float m[NQ], l[NQ];                 // every term of a row is formed against the same m, which follows the maximum only when that has grown by 8 (in log2): see below
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
         m[u] = -INFINITY;
@@ -282,83 +324,171 @@ __global__ __launch_bounds__(64 * WAVES) void dot_fwd_kernel(DotArgs a) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    Stage<T, DP, KT, 64 * WAVES> st;
     const int64_t kb = b * a.k.batch + blk.hk * a.k.head, vb = b * a.v.batch + blk.hk * a.v.head;
-    auto fetch = [&](int j) {
-        st.load(a.k, a.v, j1 - j, a.D, [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
+    auto fetch = [&](char *to, int j) {
+        stage<T, DP, KT, KEYW ? 1 : 4>(to, a.k, a.v, j1 - j, a.D, KEYW ? 0 : wave,
+                                   [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
     };
-    if (j0 < j1) fetch(j0);
-    for (int j = j0; j < j1; j += KT) {
-        __syncthreads();
-        st.store(ks, vs);
-        __syncthreads();
-        if (j + KT < j1) fetch(j + KT);
-        f32x4 z[NQ][KT / 16];
+    f32x4 bias[NQ][KS];
+    auto fetch_bias = [&](int j) {
+        if constexpr (BIAS) {
 #pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
+            for (int u = 0; u < NQ; ++u)
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < KS; ++t) bias[u][t] = bias4(bias_row[u], j + 16 * t + 4 * q4, a.Nk);
+        }
+    };
+    int j = j0 + (KEYW ? wave * KT : 0), at = 0;
+    if (j < j1) {
+        fetch(buf(0), j);
+        fetch_bias(j);
+    }
+    for (; j < j1; j += STEP, at ^= 1) {
+        arrived<!KEYW>();
+        const char *ks = buf(at), *vs = ks + TILE;
+        if (j + STEP < j1) fetch(buf(at ^ 1), j + STEP);
+        f32x4 z[NQ][KS];
+        bool some[NQ][KS];               // the same for the whole wave
+        float top[NQ];
 #pragma unroll
-            for (int c = 0; c < S::FRAGS; ++c) {
-                const Frag<T> kf = frag_load<T, DP>(ks + (16 * t + n) * S::PAD + c * 4 * S::PIECE + q4 * S::PIECE);
+        for (int u = 0; u < NQ; ++u) top[u] = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) mma<T, DP>(kf, qf[u][c], z[u][t]);
+        for (int t = 0; t < KS; ++t) {
+            bool any = !BIAS;
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                some[u][t] = !BIAS || some_attended(bias[u][t]);
+                any |= some[u][t];
+                z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            }
+            if (any) {
+#pragma unroll
+                for (int c = 0; c < S::FRAGS; ++c) {
+                    const Frag<T> kf = frag_row<T, DP>(ks, 16 * t, c);
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u)
+                        if (some[u][t]) mma<T, DP>(kf, qf[u][c], z[u][t]);
+                }
             }
         }
+        const bool plain = !BIAS && j + KT <= j1;                     // no entry of this tile is masked
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
-            float top = -INFINITY;
+            if (plain) {
 #pragma unroll
-            for (int t = 0; t < KT / 16; ++t) {
-                masked_logits(z[u][t], a.scale, bias_row[u], j + 16 * t + 4 * q4, a.Nk, j1);
-                top = fmaxf(top, fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
+                for (int t = 0; t < KS; ++t) top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
+                top[u] *= a.scale2;
+            } else {
+#pragma unroll
+                for (int t = 0; t < KS; ++t)
+                    if (some[u][t]) {
+                        z[u][t] = masked_scores(z[u][t], a.scale2, BIAS ? bias[u][t] : (f32x4){0.f, 0.f, 0.f, 0.f}, j + 16 * t + 4 * q4, j1);
+                        top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
+                    }
             }
-            top = over_groups_max(top) * kLog2e;                     // the maximum in units of log2: every term of the row uses the same rounded value
-            const float now = fmaxf(m[u], top), base = now == -INFINITY ? 0.f : now;
-            const float shrink = __builtin_amdgcn_exp2f(m[u] - base);
-            m[u] = now;
-            float sum = 0.f;
+            // The running maximum only has to keep the exponentials in range.  It is raised, and the sums shrunk, when some row's
+            // maximum has passed it by 8: after the first tiles hardly ever.  Terms up to 2^8 lose nothing in fp32 or bf16.
+            if (__ballot(top[u] > m[u] + 8.f)) {
+                top[u] = over_groups_max(top[u]);
+                const float now = fmaxf(m[u], top[u]), shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - now);
+                m[u] = now;
+                l[u] *= shrink;
 #pragma unroll
-            for (int t = 0; t < KT / 16; ++t)
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], kLog2e, -base));
-                    sum += z[u][t][r];
+                    for (int r = 0; r < 4; ++r) o[u][t][r] *= shrink;
+            }
+            const float base = m[u] == -INFINITY ? 0.f : m[u];
+#pragma unroll
+            for (int t = 0; t < KS; ++t) {
+                if (some[u][t]) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        z[u][t][r] = __builtin_amdgcn_exp2f(plain ? fmaf(z[u][t][r], a.scale2, -base) : z[u][t][r] - base);
+                        if constexpr (!ONES) l[u] += z[u][t][r];
+                    }
                 }
-            l[u] = l[u] * shrink + sum;
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[u][t][r] *= shrink;
+            }
         }
+        if (j + STEP < j1) fetch_bias(j + STEP);
 #pragma unroll
         for (int c = 0; c < KT / S::CHUNK; ++c) {
+            constexpr int PER = S::CHUNK / 16;
+            bool any = false;
+            bool use[NQ];
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                use[u] = some[u][c * PER] || some[u][c * PER + PER - 1];
+                any |= use[u];
+            }
+            if (!any) continue;
             Frag<T> pf[NQ];
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) pf[u] = frag_scores<T>(&z[u][c * (S::CHUNK / 16)]);
+            for (int u = 0; u < NQ; ++u) pf[u] = frag_scores<T>(&z[u][c * PER]);       // a tile without attended keys holds zeros
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
-                const Frag<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, 16 * t);
+                Frag<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, 16 * t);
+                if constexpr (ONES) {
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) mma_rows<T>(vf, pf[u], o[u][t]);
+                    for (int r = 0; r < 4; ++r) vf.v[r] = n == 8 ? 1.f : vf.v[r];
+                }
+#pragma unroll
+                for (int u = 0; u < NQ; ++u)
+                    if (use[u]) mma_rows<T>(vf, pf[u], o[u][t]);
             }
         }
     }
+    float sum[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
-        const float sum = over_groups_sum(l[u]);
+        if constexpr (ONES) sum[u] = __shfl(o[u][0][0], 32 + n, 64);                   // row 8 of the transposed result
+        else sum[u] = over_groups_sum(l[u]);
+    }
+    if constexpr (KEYW) {                                                            // NQ = 1: join the four waves
+        __syncthreads();
+        float *ml = reinterpret_cast<float *>(lds), *po = ml + 128;
+        if (q4 == 0) {
+            ml[wave * 16 + n] = m[0];
+            ml[64 + wave * 16 + n] = sum[0];
+        }
+        __syncthreads();
+        const float now = fmaxf(fmaxf(ml[n], ml[16 + n]), fmaxf(ml[32 + n], ml[48 + n]));
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) total += now == -INFINITY ? 0.f : ml[64 + w * 16 + n] * __builtin_amdgcn_exp2f(ml[w * 16 + n] - now);
+        const float part = now == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[0] - now);
+        m[0] = now;
+        sum[0] = total;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) po[(wave * DT + t) * 256 + r * 64 + lane] = o[0][t][r] * part;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v += po[(w * DT + t) * 256 + r * 64 + lane];
+                o[0][t][r] = v;
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < NQ; ++u) {
         if (qi[u] >= a.Nq) continue;
         if constexpr (SPLIT) {
-            const int64_t at = ((((b - a.b0) * a.Hkv + blk.hk) * (int64_t)a.Nq * a.group + row[u]) * a.splits + blk.split);
+            const int64_t slot = ((((b - a.b0) * a.Hkv + blk.hk) * (int64_t)a.Nq * a.group + row[u]) * a.splits + blk.split);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
-                if (16 * t + 4 * q4 < a.D) store4<float>(a.part_o + at * a.D + 16 * t + 4 * q4, o[u][t]);
+                if (16 * t + 4 * q4 < a.D) store4<float>(a.part_o + slot * a.D + 16 * t + 4 * q4, o[u][t]);
             if (q4 == 0) {
-                a.part_ml[2 * at] = m[u];
-                a.part_ml[2 * at + 1] = sum;
+                a.part_ml[2 * slot] = m[u];
+                a.part_ml[2 * slot + 1] = sum[u];
             }
         } else {
-            const float inv = !live[u] || sum == 0.f ? 0.f : 1.0f / sum;
+            const float inv = !live[u] || sum[u] == 0.f ? 0.f : 1.0f / sum[u];
             T *orow = reinterpret_cast<T *>(a.out) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
@@ -368,51 +498,100 @@ __global__ __launch_bounds__(64 * WAVES) void dot_fwd_kernel(DotArgs a) {
                     for (int r = 0; r < 4; ++r) v[r] = inv == 0.f ? 0.f : v[r] * inv;
                     store4<T>(orow + 16 * t + 4 * q4, v);
                 }
-            if (a.lse && q4 == 0) a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] = inv == 0.f ? INFINITY : m[u] + log2f(sum);
+            if (a.lse && q4 == 0) a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] = inv == 0.f ? INFINITY : m[u] + log2f(sum[u]);
         }
     }
 }
 
-// joins the key ranges of a row: one thread per element of the result
 template <typename T>
-__global__ __launch_bounds__(256) void dot_join_kernel(DotArgs a, int64_t total) {
-    for (int64_t e = blockIdx.x * 256ll + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int d = (int)(e % a.D);
-        const int64_t rr = e / a.D, rows = (int64_t)a.Nq * a.group;
-        const int r = (int)(rr % rows), hk = (int)(rr / rows % a.Hkv), qi = r / a.group, head = hk * a.group + r % a.group;
-        const int64_t b = a.b0 + rr / rows / a.Hkv;
-        const float *ml = a.part_ml + 2 * rr * a.splits, *po = a.part_o + rr * a.splits * a.D + d;
-        float top = -INFINITY;
-        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, o = 0.f;
-        for (int s = 0; s < a.splits; ++s) {
-            const float w = __builtin_amdgcn_exp2f(ml[2 * s] - base);
-            sum = fmaf(ml[2 * s + 1], w, sum);
-            o = fmaf(po[(int64_t)s * a.D], w, o);
+__device__ __forceinline__ void store_joined(const DotArgs &a, int64_t b, int qi, int head, int d, float top, float sum, float4 acc) {
+    const bool live = qi < graph_size(a.query_sizes, b, a.Nq);
+    const float inv = !live || sum == 0.f ? 0.f : 1.0f / sum;
+    f32x4 v = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = inv == 0.f ? 0.f : v[k] * inv;
+    store4<T>(reinterpret_cast<T *>(a.out) + ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d, v);
+    if (a.lse && d == 0) a.lse[(b * a.H + head) * a.Nq + qi] = inv == 0.f ? INFINITY : top + log2f(sum);
+}
+
+// Joins the key ranges of a row where there are few of them: D / 4 lanes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void dot_join_few_kernel(DotArgs a, int64_t rows) {
+    const int lanes = a.D / 4, groups = 256 / lanes, g = threadIdx.x / lanes, d = (threadIdx.x - g * lanes) * 4;
+    const int64_t rr = blockIdx.x * (int64_t)groups + g, per = (int64_t)a.Nq * a.group;
+    if (g >= groups || rr >= rows) return;
+    const int r = (int)(rr % per), hk = (int)(rr / per % a.Hkv), qi = r / a.group, head = hk * a.group + r % a.group;
+    const int64_t b = a.b0 + rr / per / a.Hkv;
+    const float *ml = a.part_ml + 2 * rr * a.splits, *po = a.part_o + rr * a.splits * a.D + d;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
+        sum = fmaf(ml[2 * s + 1], w, sum);
+        acc = f4_fma(w, *reinterpret_cast<const float4 *>(po + (int64_t)s * a.D), acc);
+    }
+    store_joined<T>(a, b, qi, head, d, top, sum, acc);
+}
+
+// Joins the key ranges of a row where there are many (one block a row): the weights of the ranges first, then groups of lanes add up every so many ranges, four elements
+// a lane, and their sums are added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void dot_join_kernel(DotArgs a, int64_t rows) {
+    __shared__ float weight[kSplitsMax], red[8];
+    __shared__ __attribute__((aligned(16))) float part[256 * 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t rr = blockIdx.x; rr < rows; rr += gridDim.x) {
+        const int64_t per = (int64_t)a.Nq * a.group;
+        const int r = (int)(rr % per), hk = (int)(rr / per % a.Hkv), qi = r / a.group, head = hk * a.group + r % a.group;
+        const int64_t b = a.b0 + rr / per / a.Hkv;
+        const bool has = (int)threadIdx.x < a.splits;
+        const float *ml = a.part_ml + 2 * (rr * a.splits + (has ? threadIdx.x : 0));
+        const float ms = has ? ml[0] : -INFINITY, ls = has ? ml[1] : 0.f;
+        const float wtop = wave_max(ms);
+        if (lane == 0) red[wave] = wtop;
+        __syncthreads();
+        const float top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float w = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - top);
+        if (has) weight[threadIdx.x] = w;
+        const float ws = group_sum<64>(ls * w);
+        if (lane == 0) red[4 + wave] = ws;
+        __syncthreads();
+        const float sum = (red[4] + red[5]) + (red[6] + red[7]);
+        const int lanes = a.D / 4, groups = 256 / lanes, g = threadIdx.x / lanes, d = (threadIdx.x - g * lanes) * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (g < groups) {
+            const float *po = a.part_o + rr * a.splits * a.D + d;
+#pragma unroll 4
+            for (int s = g; s < a.splits; s += groups) acc = f4_fma(weight[s], *reinterpret_cast<const float4 *>(po + (int64_t)s * a.D), acc);
+            *reinterpret_cast<float4 *>(&part[4 * threadIdx.x]) = acc;
         }
-        const bool live = qi < graph_size(a.query_sizes, b, a.Nq);
-        const float inv = !live || sum == 0.f ? 0.f : 1.0f / sum;
-        const float v = inv == 0.f ? 0.f : o * inv;
-        T *out = reinterpret_cast<T *>(a.out) + ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float *>(out) = v;
-        else *out = (T)pack_bf16x2(v, 0.f);
-        if (a.lse && d == 0) a.lse[(b * a.H + head) * a.Nq + qi] = inv == 0.f ? INFINITY : top + log2f(sum);
+        __syncthreads();
+        if (g == 0) {
+            for (int k = 1; k < groups; ++k) acc = f4_add(acc, *reinterpret_cast<const float4 *>(&part[4 * (threadIdx.x + k * lanes)]));
+            store_joined<T>(a, b, qi, head, d, top, sum, acc);
+        }
+        __syncthreads();
     }
 }
 
 // ---- backward: dq and delta ------------------------------------------------------------------------------------------------
-template <typename T, int DP, int WAVES, int NQ>
-__global__ __launch_bounds__(64 * WAVES) void dot_bwd_q_kernel(DotArgs a) {
+template <typename T, int DP, int NQ, bool BIAS>
+__global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
     using S = Shape<T, DP>;
-    using TL = Tiles<T, DP>;
-    constexpr int KT = TL::KT, DT = TL::DT, ROWS = WAVES * NQ * 16;
-    __shared__ __attribute__((aligned(16))) char lds[TL::LDS];
-    char *ks = lds, *vs = lds + KT * S::PAD;
+    constexpr int KT = S::KT, DT = S::DT, ROWS = 64 * NQ, PER = S::CHUNK / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const DotBlock blk = dot_block<BIAS>(a);
+    if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
-    const DotBlock blk = dot_block(a);
     const int64_t b = blk.b;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
+    auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
+    const int64_t kb = b * a.k.batch + blk.hk * a.k.head, vb = b * a.v.batch + blk.hk * a.v.head;
+    auto fetch = [&](char *to, int j) {
+        stage<T, DP, KT, 4>(to, a.k, a.v, keys - j, a.D, wave, [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
+    };
+    if (keys > 0) fetch(buf(0), 0);
     int qi[NQ], head[NQ];
     float lse[NQ], delta[NQ];
     Frag<T> qf[NQ][S::FRAGS], df[NQ][S::FRAGS];
@@ -421,81 +600,95 @@ __global__ __launch_bounds__(64 * WAVES) void dot_bwd_q_kernel(DotArgs a) {
     for (int u = 0; u < NQ; ++u) {
         const int row = blk.tile * ROWS + (wave * NQ + u) * 16 + n;
         qi[u] = row / a.group;
-        head[u] = blk.hk * a.group + row % a.group;
+        head[u] = blk.hk * a.group + row - qi[u] * a.group;
         const bool live = qi[u] < queries;
         const int64_t i = live ? qi[u] : 0;
-        const T *qrow = reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + i * a.q.node + head[u] * a.q.head;
-        const T *drow = reinterpret_cast<const T *>(a.d_o.p) + b * a.d_o.batch + i * a.d_o.node + head[u] * a.d_o.head;
-        const T *orow = reinterpret_cast<const T *>(a.o.p) + b * a.o.batch + i * a.o.node + head[u] * a.o.head;
+        Frag<T> of[S::FRAGS];
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + i * a.q.node + head[u] * a.q.head, a.D, live, qf[u]);
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.d_o.p) + b * a.d_o.batch + i * a.d_o.node + head[u] * a.d_o.head, a.D, live, df[u]);
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.o.p) + b * a.o.batch + i * a.o.node + head[u] * a.o.head, a.D, live, of);
         float dot = 0.f;
 #pragma unroll
         for (int c = 0; c < S::FRAGS; ++c) {
-            const int e = c * S::KD + q4 * (S::PIECE / (int)sizeof(T));
-            qf[u][c] = row_piece<T, DP>(qrow, e, a.D, live);
-            df[u][c] = row_piece<T, DP>(drow, e, a.D, live);
-            const Frag<T> of = row_piece<T, DP>(orow, e, a.D, live);
-            if constexpr (sizeof(T) == 4) {
+            if constexpr (S::SIZE == 4) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) dot = fmaf(df[u][c].v[t], of.v[t], dot);
+                for (int t = 0; t < S::ELEMS; ++t) dot = fmaf(df[u][c].v[t], of[c].v[t], dot);
             } else {
-                const uint32_t *x = reinterpret_cast<const uint32_t *>(&df[u][c].v), *y = reinterpret_cast<const uint32_t *>(&of.v);
+                const uint32_t x[4] = {df[u][c].v.x, df[u][c].v.y, df[u][c].v.z, df[u][c].v.w}, y[4] = {of[c].v.x, of[c].v.y, of[c].v.z, of[c].v.w};
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < S::ELEMS / 2; ++t) {
                     dot = fmaf(__uint_as_float(x[t] << 16), __uint_as_float(y[t] << 16), dot);
                     dot = fmaf(__uint_as_float(x[t] & 0xffff0000u), __uint_as_float(y[t] & 0xffff0000u), dot);
                 }
             }
+            if (a.scale < 0.f) qf[u][c] = frag_negated<T>(qf[u][c]);
         }
         delta[u] = over_groups_sum(dot);
         lse[u] = live ? a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] : INFINITY;
         if (q4 == 0 && qi[u] < a.Nq) a.delta[(b * a.H + head[u]) * a.Nq + qi[u]] = delta[u];
-        bias_row[u] = a.bias ? a.bias + b * a.bias_batch + i * a.bias_row : nullptr;
+        bias_row[u] = BIAS ? a.bias + b * a.bias_batch + i * a.bias_row : nullptr;
     }
     f32x4 acc[NQ][DT];
 #pragma unroll
     for (int u = 0; u < NQ; ++u)
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    Stage<T, DP, KT, 64 * WAVES> st;
-    const int64_t kb = b * a.k.batch + blk.hk * a.k.head, vb = b * a.v.batch + blk.hk * a.v.head;
-    auto fetch = [&](int j) {
-        st.load(a.k, a.v, keys - j, a.D, [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
-    };
-    if (keys > 0) fetch(0);
-    for (int j = 0; j < keys; j += KT) {
-        __syncthreads();
-        st.store(ks, vs);
-        __syncthreads();
-        if (j + KT < keys) fetch(j + KT);
+    for (int j = 0, at = 0; j < keys; j += KT, at ^= 1) {
+        f32x4 bias[NQ][KT / 16];
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int u = 0; u < NQ; ++u)
+#pragma unroll
+                for (int t = 0; t < KT / 16; ++t) bias[u][t] = bias4(bias_row[u], j + 16 * t + 4 * q4, a.Nk);
+        }
+        arrived<true>();
+        const char *ks = buf(at), *vs = ks + S::TILE;
+        if (j + KT < keys) fetch(buf(at ^ 1), j + KT);
+        const bool plain = !BIAS && j + KT <= keys;
 #pragma unroll
         for (int c = 0; c < KT / S::CHUNK; ++c) {
-            f32x4 z[NQ][S::CHUNK / 16];
+            f32x4 z[NQ][PER];
+            bool use[NQ], any = false;
 #pragma unroll
-            for (int t = 0; t < S::CHUNK / 16; ++t) {
+            for (int u = 0; u < NQ; ++u) use[u] = false;
+#pragma unroll
+            for (int t = 0; t < PER; ++t) {
                 const int r0 = c * S::CHUNK + 16 * t;
                 f32x4 dp[NQ];
-#pragma unroll
-                for (int u = 0; u < NQ; ++u) z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int f = 0; f < S::FRAGS; ++f) {
-                    const int at = (r0 + n) * S::PAD + f * 4 * S::PIECE + q4 * S::PIECE;
-                    const Frag<T> kf = frag_load<T, DP>(ks + at), vf = frag_load<T, DP>(vs + at);
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u) {
-                        mma<T, DP>(kf, qf[u][f], z[u][t]);
-                        mma<T, DP>(vf, df[u][f], dp[u]);
-                    }
-                }
+                bool some[NQ], here = false;
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
-                    masked_logits(z[u][t], a.scale, bias_row[u], j + r0 + 4 * q4, a.Nk, keys);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], kLog2e, -lse[u]));
-                        z[u][t][r] = p * (dp[u][r] - delta[u]);
-                    }
+                    z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                    some[u] = !BIAS || some_attended(bias[u][r0 / 16]);
+                    use[u] |= some[u];
+                    here |= some[u];
                 }
+                any |= here;
+                if (!here) continue;
+#pragma unroll
+                for (int f = 0; f < S::FRAGS; ++f) {
+                    const Frag<T> kf = frag_row<T, DP>(ks, r0, f), vf = frag_row<T, DP>(vs, r0, f);
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u)
+                        if (some[u]) {
+                            mma<T, DP>(kf, qf[u][f], z[u][t]);
+                            mma<T, DP>(vf, df[u][f], dp[u]);
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < NQ; ++u)
+                    if (some[u]) {
+                        if (plain) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], a.scale2, -lse[u])) * (dp[u][r] - delta[u]);
+                        } else {
+                            const f32x4 s = masked_scores(z[u][t], a.scale2, BIAS ? bias[u][r0 / 16] : (f32x4){0.f, 0.f, 0.f, 0.f}, j + r0 + 4 * q4, keys);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(s[r] - lse[u]) * (dp[u][r] - delta[u]);
+                        }
+                    }
             }
+            if (!any) continue;
             Frag<T> zf[NQ];
 #pragma unroll
             for (int u = 0; u < NQ; ++u) zf[u] = frag_scores<T>(z[u]);
@@ -503,7 +696,8 @@ __global__ __launch_bounds__(64 * WAVES) void dot_bwd_q_kernel(DotArgs a) {
             for (int t = 0; t < DT; ++t) {
                 const Frag<T> kf = frag_turned<T, DP>(ks, c * S::CHUNK, 16 * t);
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) mma_rows<T>(kf, zf[u], acc[u][t]);
+                for (int u = 0; u < NQ; ++u)
+                    if (use[u]) mma_rows<T>(kf, zf[u], acc[u][t]);
             }
         }
     }
@@ -523,101 +717,105 @@ __global__ __launch_bounds__(64 * WAVES) void dot_bwd_q_kernel(DotArgs a) {
 }
 
 // ---- backward: dk and dv -----------------------------------------------------------------------------------------------------
-// A wave owns NK x 16 keys (one per lane of a row of 16) and walks all rows of the sharing heads.
-template <typename T, int DP, int WAVES, int NK>
-__global__ __launch_bounds__(64 * WAVES) void dot_bwd_kv_kernel(DotArgs a) {
+// A wave owns NK x 16 keys (one per lane of a row of 16) and walks all rows of the sharing heads.  Rows behind the last one come with
+// lse = inf: their probabilities are zero.
+template <typename T, int DP, int NK, bool BIAS>
+__global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_bwd_kv_kernel(DotArgs a) {
     using S = Shape<T, DP>;
-    using TL = Tiles<T, DP>;
-    constexpr int QT = TL::KT, DT = TL::DT, KEYS = WAVES * NK * 16;
-    __shared__ __attribute__((aligned(16))) char lds[TL::LDS];
-    __shared__ __attribute__((aligned(16))) float lses[QT], deltas[QT];
-    char *qs = lds, *ds = lds + QT * S::PAD;
+    constexpr int QT = S::KT, DT = S::DT, KEYS = 64 * NK, PER = S::CHUNK / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
+    __shared__ const float *bias_rows[2][BIAS ? QT : 1];
+    const DotBlock blk = dot_block<BIAS>(a);
+    if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
-    const DotBlock blk = dot_block(a);
     const int64_t b = blk.b;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
     const int rows = queries * a.group;
-    int key[NK];
+    auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
+    auto fetch = [&](int to, int r0) {
+        stage<T, DP, QT, 4>(buf(to), a.q, a.d_o, rows - r0, a.D, wave, [&](const DotRows &x, int r) {
+            const int row = r0 + r, i = row / a.group;
+            return b * x.batch + (int64_t)i * x.node + (blk.hk * a.group + row - i * a.group) * x.head;
+        });
+        if (threadIdx.x < QT) {
+            const int row = min(r0 + (int)threadIdx.x, rows - 1), i = row / a.group;
+            const int64_t at = (b * a.H + blk.hk * a.group + row - i * a.group) * a.Nq + i;
+            lses[to][threadIdx.x] = r0 + (int)threadIdx.x < rows ? a.lse[at] : INFINITY;
+            deltas[to][threadIdx.x] = a.delta[at];
+            if constexpr (BIAS) bias_rows[to][threadIdx.x] = a.bias + b * a.bias_batch + i * a.bias_row;
+        }
+    };
+    if (rows > 0) fetch(0, 0);
+    int key[NK], col[NK];
     Frag<T> kf[NK][S::FRAGS], vf[NK][S::FRAGS];
     f32x4 dk[NK][DT], dv[NK][DT];
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
         key[u] = blk.tile * KEYS + (wave * NK + u) * 16 + n;
         const bool live = key[u] < keys;
-        const int64_t j = live ? key[u] : 0;
-        const T *krow = reinterpret_cast<const T *>(a.k.p) + b * a.k.batch + j * a.k.node + blk.hk * a.k.head;
-        const T *vrow = reinterpret_cast<const T *>(a.v.p) + b * a.v.batch + j * a.v.node + blk.hk * a.v.head;
+        col[u] = live ? key[u] : 0;
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.k.p) + b * a.k.batch + (int64_t)col[u] * a.k.node + blk.hk * a.k.head, a.D, live, kf[u]);
+        row_frags<T, DP>(reinterpret_cast<const T *>(a.v.p) + b * a.v.batch + (int64_t)col[u] * a.v.node + blk.hk * a.v.head, a.D, live, vf[u]);
+        if (a.scale < 0.f) {
 #pragma unroll
-        for (int c = 0; c < S::FRAGS; ++c) {
-            const int e = c * S::KD + q4 * (S::PIECE / (int)sizeof(T));
-            kf[u][c] = row_piece<T, DP>(krow, e, a.D, live);
-            vf[u][c] = row_piece<T, DP>(vrow, e, a.D, live);
+            for (int c = 0; c < S::FRAGS; ++c) kf[u][c] = frag_negated<T>(kf[u][c]);
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[u][t] = dv[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    Stage<T, DP, QT, 64 * WAVES> st;
-    float next_lse = 0.f, next_delta = 0.f;
-    auto fetch = [&](int r0) {
-        st.load(a.q, a.d_o, rows - r0, a.D, [&](const DotRows &x, int r) {
-            const int row = r0 + r, i = row / a.group;
-            return b * x.batch + (int64_t)i * x.node + (blk.hk * a.group + row - i * a.group) * x.head;
-        });
-        if (threadIdx.x < QT) {
-            const int row = r0 + threadIdx.x, i = row / a.group;
-            const bool ok = row < rows;
-            const int64_t at = (b * a.H + blk.hk * a.group + row - i * a.group) * a.Nq + i;
-            next_lse = ok ? a.lse[at] : INFINITY;
-            next_delta = ok ? a.delta[at] : 0.f;
-        }
-    };
-    if (rows > 0) fetch(0);
-    for (int r0 = 0; r0 < rows; r0 += QT) {
-        __syncthreads();
-        st.store(qs, ds);
-        if (threadIdx.x < QT) {
-            lses[threadIdx.x] = next_lse;
-            deltas[threadIdx.x] = next_delta;
-        }
-        __syncthreads();
-        if (r0 + QT < rows) fetch(r0 + QT);
+    for (int r0 = 0, at = 0; r0 < rows; r0 += QT, at ^= 1) {
+        arrived<true>();
+        const char *qs = buf(at), *ds = qs + S::TILE;
+        if (r0 + QT < rows) fetch(at ^ 1, r0 + QT);
 #pragma unroll
         for (int c = 0; c < QT / S::CHUNK; ++c) {
-            f32x4 p[NK][S::CHUNK / 16], z[NK][S::CHUNK / 16];
+            f32x4 p[NK][PER], z[NK][PER];
+            bool use[NK], any = false;
 #pragma unroll
-            for (int t = 0; t < S::CHUNK / 16; ++t) {
+            for (int u = 0; u < NK; ++u) use[u] = false;
+#pragma unroll
+            for (int t = 0; t < PER; ++t) {
                 const int s0 = c * S::CHUNK + 16 * t;
-                f32x4 dp[NK];
+                f32x4 dp[NK], bias[NK];
+                bool some[NK], here = false;
 #pragma unroll
-                for (int u = 0; u < NK; ++u) z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                for (int u = 0; u < NK; ++u) {
+                    z[u][t] = dp[u] = p[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                    some[u] = true;
+                    if constexpr (BIAS) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
+                        some[u] = some_attended(bias[u]);
+                    }
+                    use[u] |= some[u];
+                    here |= some[u];
+                }
+                any |= here;
+                if (!here) continue;
 #pragma unroll
                 for (int f = 0; f < S::FRAGS; ++f) {
-                    const int at = (s0 + n) * S::PAD + f * 4 * S::PIECE + q4 * S::PIECE;
-                    const Frag<T> qf = frag_load<T, DP>(qs + at), df = frag_load<T, DP>(ds + at);
+                    const Frag<T> qf = frag_row<T, DP>(qs, s0, f), df = frag_row<T, DP>(ds, s0, f);
 #pragma unroll
-                    for (int u = 0; u < NK; ++u) {
-                        mma<T, DP>(qf, kf[u][f], z[u][t]);
-                        mma<T, DP>(df, vf[u][f], dp[u]);
-                    }
+                    for (int u = 0; u < NK; ++u)
+                        if (some[u]) {
+                            mma<T, DP>(qf, kf[u][f], z[u][t]);
+                            mma<T, DP>(df, vf[u][f], dp[u]);
+                        }
                 }
-                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[s0 + 4 * q4]);
+                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[at][s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[at][s0 + 4 * q4]);
 #pragma unroll
                 for (int u = 0; u < NK; ++u)
+                    if (some[u]) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = r0 + s0 + 4 * q4 + r;
-                        bool seen = key[u] < keys && row < rows;
-                        float zz = z[u][t][r] * a.scale;
-                        if (a.bias && seen) {
-                            const float bv = a.bias[b * a.bias_batch + (int64_t)(row / a.group) * a.bias_row + key[u]];
-                            seen = bv > kAttended;
-                            zz = fmaf(z[u][t][r], a.scale, bv);
+                        for (int r = 0; r < 4; ++r) {
+                            const float s = BIAS ? (bias[u][r] > kAttended ? fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e) - lse[r] : -INFINITY) : fmaf(z[u][t][r], a.scale2, -lse[r]);
+                            p[u][t][r] = __builtin_amdgcn_exp2f(s);
+                            z[u][t][r] = p[u][t][r] * (dp[u][r] - delta[r]);
                         }
-                        const float pv = seen ? __builtin_amdgcn_exp2f(fmaf(zz, kLog2e, -lse[r])) : 0.f;
-                        p[u][t][r] = pv;
-                        z[u][t][r] = pv * (dp[u][r] - delta[r]);
                     }
             }
+            if (!any) continue;
             Frag<T> pf[NK], zf[NK];
 #pragma unroll
             for (int u = 0; u < NK; ++u) {
@@ -628,25 +826,30 @@ __global__ __launch_bounds__(64 * WAVES) void dot_bwd_kv_kernel(DotArgs a) {
             for (int t = 0; t < DT; ++t) {
                 const Frag<T> df = frag_turned<T, DP>(ds, c * S::CHUNK, 16 * t), qf = frag_turned<T, DP>(qs, c * S::CHUNK, 16 * t);
 #pragma unroll
-                for (int u = 0; u < NK; ++u) {
-                    mma_rows<T>(df, pf[u], dv[u][t]);
-                    mma_rows<T>(qf, zf[u], dk[u][t]);
-                }
+                for (int u = 0; u < NK; ++u)
+                    if (use[u]) {
+                        mma_rows<T>(df, pf[u], dv[u][t]);
+                        mma_rows<T>(qf, zf[u], dk[u][t]);
+                    }
             }
         }
     }
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
         if (key[u] >= a.Nk) continue;
+        const float keep = key[u] < keys ? 1.f : 0.f;                  // a key behind the graph's own has been walked as a row of zeros
         const int64_t at = ((b * a.Nk + key[u]) * a.Hkv + blk.hk) * (int64_t)a.D;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             if (16 * t + 4 * q4 < a.D) {
-                f32x4 v = dk[u][t];
+                f32x4 x = dk[u][t], y = dv[u][t];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] *= a.scale;
-                store4<T>(reinterpret_cast<T *>(a.dk) + at + 16 * t + 4 * q4, v);
-                store4<T>(reinterpret_cast<T *>(a.dv) + at + 16 * t + 4 * q4, dv[u][t]);
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = keep == 0.f ? 0.f : x[r] * a.scale;
+                    y[r] = keep == 0.f ? 0.f : y[r];
+                }
+                store4<T>(reinterpret_cast<T *>(a.dk) + at + 16 * t + 4 * q4, x);
+                store4<T>(reinterpret_cast<T *>(a.dv) + at + 16 * t + 4 * q4, y);
             }
     }
 }
@@ -673,15 +876,34 @@ static int dot_rows(const char *what, const char *name, DotRows *r, const void *
 
 constexpr int64_t kDotBlocks = 1 << 22;      // blocks of one launch
 
-// Rows per block: four waves of 32 rows, of 16 where that leaves most of a block idle, one wave of 16 for the rows of single queries.
-static int dot_rows_per_block(int64_t rows) { return rows <= 16 ? 16 : (rows <= 64 ? 64 : 128); }
+// Rows per block: the four waves share 16 rows and walk different keys, or have 16 or 32 rows each.
+static int dot_rows_per_block(int64_t rows, int nq) { return rows <= 16 ? 16 : (rows <= 64 ? 64 : 64 * nq); }
 
-// Key ranges of a forward launch: enough blocks for every compute unit twice, ranges of 256 keys or more.
+// Key ranges of a forward launch: as many blocks as are resident at once (two to a compute unit), ranges of 512 keys or more.
 static int dot_splits(int64_t B, int64_t rows, int32_t Hkv, int32_t Nk) {
-    const int per = dot_rows_per_block(rows);
+    const int per = dot_rows_per_block(rows, 2);
     const int64_t blocks = B * Hkv * ((rows + per - 1) / per);
-    if (blocks >= 512 || Nk < 512) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kSplitsMax, Nk / 256), (1024 + blocks - 1) / std::max<int64_t>(1, blocks)));
+    if (blocks >= 384 || Nk < 1024) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kSplitsMax, Nk / 512), (512 + blocks / 2) / blocks));
+}
+
+// graphs that one launch takes
+static int64_t dot_graphs(const DotArgs &a) {
+    const int64_t per = (int64_t)a.tiles * a.splits * a.Hkv;
+    return std::max<int64_t>(1, kDotBlocks / per);
+}
+
+template <typename K>
+static int dot_launch(const char *what, K kernel, const DotArgs &a, size_t lds, hipStream_t st) {
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return fail(GATMI_EHIP, "%s: %s", what, hipGetErrorString(e));
+    }
+    const int64_t inner = a.bias ? a.Hkv : (int64_t)a.tiles * a.splits, groups = (int64_t)a.B * a.Hkv * a.tiles * a.splits / inner;
+    const int64_t blocks = 8 * (groups / 8 * inner + (groups % 8 * inner + 7) / 8);
+    GATMI_REQUIRE(blocks <= 2 * kDotBlocks, GATMI_ERANGE, "%s: %lld blocks for one graph", what, (long long)blocks);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), lds, st, a);
+    return GATMI_OK;
 }
 
 }  // namespace gatmi
@@ -697,30 +919,30 @@ extern "C" size_t gatmi_dot_attn_fwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk
 
 template <typename T, int DP>
 static int dot_fwd_run(DotArgs a, int64_t B, hipStream_t st) {
+    using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
-    const int per = dot_rows_per_block(rows);
+    const int per = dot_rows_per_block(rows, S::NQ);
     a.tiles = (int)((rows + per - 1) / per);
-    const int64_t per_graph = (int64_t)a.tiles * a.Hkv * a.splits;
-    GATMI_REQUIRE(per_graph <= kDotBlocks, GATMI_ERANGE, "dot_attn_fwd: %lld blocks for one graph", (long long)per_graph);
-    const int64_t step = a.splits > 1 ? B : kDotBlocks / per_graph;              // split launches are small by construction
+    const int64_t step = a.splits > 1 ? B : dot_graphs(a);              // split launches are small by construction
+    const size_t lds = 4 * S::TILE, lds_keyw = std::max<size_t>(16 * S::KTW * S::ROW, 512 + 4 * S::DT * 1024);
     for (int64_t b0 = 0; b0 < B; b0 += step) {
-        const int64_t now = std::min(step, B - b0);
         a.b0 = b0;
-        const dim3 grid((unsigned)(per_graph * now));
-#define RUN(w, nq)                                                                                                                 \
-    do {                                                                                                                           \
-        if (a.splits > 1) hipLaunchKernelGGL((dot_fwd_kernel<T, DP, w, nq, true>), grid, dim3(64 * w), 0, st, a);                  \
-        else hipLaunchKernelGGL((dot_fwd_kernel<T, DP, w, nq, false>), grid, dim3(64 * w), 0, st, a);                              \
-    } while (0)
-        if (per == 16) RUN(1, 1);
-        else if (per == 64) RUN(4, 1);
-        else RUN(4, 2);
+        a.B = (int)std::min(step, B - b0);
+        int rc;
+#define RUN(keyw, nq, split, bytes)                                                                                          \
+    (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, true>, a, bytes, st)                        \
+            : dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, false>, a, bytes, st))
+        if (per == 16) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
+        else if (per == 64) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);
+        else rc = a.splits > 1 ? RUN(false, S::NQ, true, lds) : RUN(false, S::NQ, false, lds);
 #undef RUN
+        if (rc) return rc;
     }
     if (a.splits > 1) {
-        a.b0 = 0;
-        const int64_t total = B * a.Hkv * rows * a.D;
-        hipLaunchKernelGGL((dot_join_kernel<T>), dim3((unsigned)std::min<int64_t>(4096, (total + 255) / 256)), dim3(256), 0, st, a, total);
+        const int64_t total = B * a.Hkv * rows;
+        const int64_t per_block = 256 / (a.D / 4);
+        if (a.splits <= 16) hipLaunchKernelGGL((dot_join_few_kernel<T>), dim3((unsigned)((total + per_block - 1) / per_block)), dim3(256), 0, st, a, total);
+        else hipLaunchKernelGGL((dot_join_kernel<T>), dim3((unsigned)std::min<int64_t>(1 << 16, total)), dim3(256), 0, st, a, total);
     }
     GATMI_LAUNCH_CHECK("dot_attn_fwd");
     return GATMI_OK;
@@ -755,11 +977,10 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     GATMI_REQUIRE_ALIGNED(out);
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq == 1, GATMI_EINVAL, "dot_attn_fwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
     a.out = out; a.lse = lse; a.bias = Nk > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
-    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale;
+    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::fabs(scale) * kLog2e;
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     const int64_t rows = (int64_t)Nq * a.group;
     a.splits = dot_splits(B, rows, Hkv, Nk);
-    a.split_keys = a.splits > 1 ? ((Nk + a.splits - 1) / a.splits + 63) / 64 * 64 : Nk;
     if (a.splits > 1) {
         GATMI_REQUIRE(ws, GATMI_EINVAL, "dot_attn_fwd: workspace is null");
         GATMI_REQUIRE_ALIGNED(ws);
@@ -774,28 +995,25 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
 
 template <typename T, int DP>
 static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
+    using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
-    constexpr int NQ = (sizeof(T) == 4 && DP == 128) ? 1 : 2, NK = DP == 128 ? 1 : 2;      // registers: two row tiles per wave where the accumulators leave room
+    a.splits = 1;
     for (int pass = 0; pass < 2; ++pass) {
-        const bool wide = pass == 0 ? rows > 64 : a.Nk > 64;
-        const int per = pass == 0 ? (wide ? 64 * NQ : 64) : (wide ? 64 * NK : 64);
         const int64_t count = pass == 0 ? rows : a.Nk;
         if (count == 0) continue;
+        const bool wide = count > 64;
+        const int per = 64 * (wide ? (pass == 0 ? S::NQ : S::NK) : 1);
         a.tiles = (int)((count + per - 1) / per);
-        a.splits = 1;
-        const int64_t per_graph = (int64_t)a.tiles * a.Hkv;
-        GATMI_REQUIRE(per_graph <= kDotBlocks, GATMI_ERANGE, "dot_attn_bwd: %lld blocks for one graph", (long long)per_graph);
-        const int64_t step = kDotBlocks / per_graph;
+        const int64_t step = dot_graphs(a);
         for (int64_t b0 = 0; b0 < B; b0 += step) {
             a.b0 = b0;
-            const dim3 grid((unsigned)(per_graph * std::min(step, B - b0)));
-            if (pass == 0) {
-                if (wide) hipLaunchKernelGGL((dot_bwd_q_kernel<T, DP, 4, NQ>), grid, dim3(256), 0, st, a);
-                else hipLaunchKernelGGL((dot_bwd_q_kernel<T, DP, 4, 1>), grid, dim3(256), 0, st, a);
-            } else {
-                if (wide) hipLaunchKernelGGL((dot_bwd_kv_kernel<T, DP, 4, NK>), grid, dim3(256), 0, st, a);
-                else hipLaunchKernelGGL((dot_bwd_kv_kernel<T, DP, 4, 1>), grid, dim3(256), 0, st, a);
-            }
+            a.B = (int)std::min(step, B - b0);
+            int rc;
+#define RUN(kernel, n) (a.bias ? dot_launch("dot_attn_bwd", kernel<T, DP, n, true>, a, 4 * S::TILE, st) : dot_launch("dot_attn_bwd", kernel<T, DP, n, false>, a, 4 * S::TILE, st))
+            if (pass == 0) rc = wide ? RUN(dot_bwd_q_kernel, S::NQ) : RUN(dot_bwd_q_kernel, 1);
+            else rc = wide ? RUN(dot_bwd_kv_kernel, S::NK) : RUN(dot_bwd_kv_kernel, 1);
+#undef RUN
+            if (rc) return rc;
         }
     }
     GATMI_LAUNCH_CHECK("dot_attn_bwd");
@@ -828,7 +1046,7 @@ extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq <= 1, GATMI_EINVAL, "dot_attn_bwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
     a.dq = dq; a.dk = dk; a.dv = dv; a.lse = const_cast<float *>(lse); a.delta = delta;
     a.bias = Nk > 0 && Nq > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
-    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale;
+    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::fabs(scale) * kLog2e;
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
 #define RUN(T, dp) dot_bwd_run<T, dp>(a, B, st)

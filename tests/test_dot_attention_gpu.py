@@ -141,7 +141,7 @@ def test_nan_and_inf_in_an_attended_row_stay_visible():
 def test_few_rows_on_many_keys(B, Nq, Nk, H, G, D, dtype):
     """Split over the keys; also with ranges that no key of a graph falls into, and gradients behind it."""
     from gat_amd import _lib
-    assert _lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, G, (D + 7) // 8 * 8) > 0
+    assert Nk < 2000 or _lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, G, (D + 7) // 8 * 8) > 0
     c = _case(B, Nq, Nk, H, G, D, dtype, seed=Nk)
     _check(c, dtype, grad=Nk <= 5000)
     c["ks"] = torch.tensor([(Nk, 5, 0)[b % 3] for b in range(B)][::-1], dtype=torch.int32, device="cuda:0")
