@@ -181,12 +181,14 @@ __global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
         const int row = e / NP, col = e % NP;
         const int up = row / 16 <= col / 16 ? e : col * NP + row;          // tiles below the diagonal are not formed
         double s = 0;
+#pragma unroll 8
         for (int p = 0; p < a.parts; ++p) s += g[(size_t)p * (NP * NP) + up];
         A[row * LD + col] = s;
     }
     __syncthreads();
     double trace = 0;
-    for (int d = 0; d < a.n; ++d) trace += A[d * LD + d];
+#pragma unroll 16
+    for (int d = 0; d < NP; ++d) trace += A[d * LD + d];              // zeros behind n
     const double inv = 1.0 / (sqrt(trace) + a.eps);
     __syncthreads();
     for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) A[e / NP * LD + e % NP] *= inv * inv;
@@ -262,11 +264,17 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(NarrowArgs a) {
 }
 
 // ---- wide --------------------------------------------------------------------------------------------------------------
-constexpr int kWT = 128;          // rows and columns of a tile
+constexpr int kWT = 128;          // sides are padded to this: rows and columns of the larger tile
 constexpr int kWK = 32;           // depth of a step
-constexpr int kNormBlocks = 64;   // partial sums of squares per matrix
+constexpr int kNormBlocks = 256;  // partial sums of squares per matrix
 
-struct Planes { _Float16 *hi, *lo; };     // value = (hi + lo) / kPlaneScale
+// A matrix [rows][K] of values (hi + lo) / kPlaneScale: every 32 entries of a row are 32 hi and then their 32 lo, so that a step of depth 32
+// reads whole 128-byte lines.
+struct Planes {
+    _Float16 *p;
+    __device__ static __forceinline__ int64_t at(int64_t row, int64_t k, int64_t K) { return row * 2 * K + (k >> 5) * 64 + (k & 31); }
+    __device__ __forceinline__ void put(int64_t at, _Float16 hi, _Float16 lo) const { p[at] = hi; p[at + 32] = lo; }
+};
 
 struct WideArgs {
     NsMatrix a;
@@ -274,7 +282,7 @@ struct WideArgs {
     int64_t np, lp;               // padded to whole tiles (zeros)
     Planes x, xt, g, p;           // X [np][lp], X^T [lp][np], X X^T and the polynomial [np][np]; per matrix
     Planes xt_new;                // a step's X^T: other blocks still read the old one
-    int64_t x_plane, g_plane;     // elements of one matrix
+    int64_t x_plane, g_plane;     // fp16 numbers of one matrix
     double *norm;                 // [batch][kNormBlocks]
     int32_t *shift;               // [batch]: e of the first step
     float ca, cb, cc;
@@ -298,16 +306,45 @@ __device__ __forceinline__ void split16(float v, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)(s - (float)hi);
 }
 
-template <typename T>
+// Partial sums of squares: pieces of kNormPiece entries of a row, dealt to the blocks in turn.  VEC: rows start 4 elements aligned.
+constexpr int kNormPiece = 4096;
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void ns_norm_kernel(WideArgs a) {
     __shared__ double part[4];
     const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.y * a.a.x_batch;
+    const int64_t per_row = (a.a.n + kNormPiece - 1) / kNormPiece;
     double s = 0;
-    for (int64_t i = blockIdx.x; i < a.a.m; i += gridDim.x)
-        for (int64_t j = threadIdx.x; j < a.a.n; j += 256) {
-            const double v = ns_load<T>(x + i * a.a.x_row + j);
-            s += v * v;
+    for (int64_t item = blockIdx.x; item < a.a.m * per_row; item += gridDim.x) {
+        const int64_t i = item / per_row, j0 = (item - i * per_row) * kNormPiece, j1 = min(a.a.n, j0 + kNormPiece);
+        const T *row = x + i * a.a.x_row;
+        if constexpr (VEC) {
+            const int64_t j4 = j0 + (j1 - j0) / 4 * 4;
+#pragma unroll 4
+            for (int64_t j = j0 + 4 * (int)threadIdx.x; j < j4; j += 4 * 256) {
+                float v[4];
+                if constexpr (sizeof(T) == 4) {
+                    const float4 u = *reinterpret_cast<const float4 *>(row + j);
+                    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+                } else {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(row + j);
+                    v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
+                    v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += (double)v[k] * (double)v[k];
+            }
+            for (int64_t j = j4 + threadIdx.x; j < j1; j += 256) {
+                const double v = ns_load<T>(row + j);
+                s += v * v;
+            }
+        } else {
+#pragma unroll 4
+            for (int64_t j = j0 + threadIdx.x; j < j1; j += 256) {
+                const double v = ns_load<T>(row + j);
+                s += v * v;
+            }
         }
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -315,15 +352,29 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(WideArgs a) {
     if (threadIdx.x == 0) a.norm[blockIdx.y * kNormBlocks + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+// sum over the 256 threads of a block, the same in all of them
+__device__ __forceinline__ double block_sum_f64(double s, double *part, int waves) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    double total = 0;
+    for (int w = 0; w < waves; ++w) total += part[w];
+    return total;
+}
+
+// e of the first step from |X|_F = unit
+__device__ __forceinline__ int ns_first_shift(double unit) { return unit > 0.0 && unit < 0.5 ? min(120, -ilogb(unit) - 1) : 0; }
+
 // X and X^T as planes, zero in the padding: 32 x 32 tiles through LDS
 template <typename T, bool TALL>
 __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
     __shared__ float tile[32][33];
-    double s = 0;
-    for (int k = 0; k < kNormBlocks; ++k) s += a.norm[blockIdx.z * kNormBlocks + k];
+    __shared__ double part[4];
+    const double s = block_sum_f64(a.norm[blockIdx.z * kNormBlocks + threadIdx.x], part, 4);
     double inv = 1.0 / (sqrt(s) + a.eps);
     const double unit = sqrt(s) * inv;                                     // |X|_F
-    const int e0 = unit > 0.0 && unit < 0.5 ? min(120, -ilogb(unit) - 1) : 0;
+    const int e0 = ns_first_shift(unit);
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.shift[blockIdx.z] = e0;
     inv = ldexp(inv, e0);
     const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.z * a.a.x_batch;
@@ -331,8 +382,8 @@ __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t rows = TALL ? a.lp : a.np, cols = TALL ? a.np : a.lp;
     Planes straight = TALL ? a.xt : a.x, turned = TALL ? a.x : a.xt;
-    straight.hi += blockIdx.z * a.x_plane; straight.lo += blockIdx.z * a.x_plane;
-    turned.hi += blockIdx.z * a.x_plane; turned.lo += blockIdx.z * a.x_plane;
+    straight.p += blockIdx.z * a.x_plane;
+    turned.p += blockIdx.z * a.x_plane;
 #pragma unroll
     for (int r = 0; r < 32; r += 8) {
         const int64_t i = i0 + ty + r, j = j0 + tx;
@@ -340,8 +391,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
         tile[ty + r][tx] = v;
         _Float16 hi, lo;
         split16(v, hi, lo);
-        straight.hi[i * cols + j] = hi;
-        straight.lo[i * cols + j] = lo;
+        straight.put(Planes::at(i, j, cols), hi, lo);
     }
     __syncthreads();
 #pragma unroll
@@ -349,88 +399,103 @@ __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
         const int64_t j = j0 + ty + r, i = i0 + tx;
         _Float16 hi, lo;
         split16(tile[tx][ty + r], hi, lo);
-        turned.hi[j * rows + i] = hi;
-        turned.lo[j * rows + i] = lo;
+        turned.put(Planes::at(j, i, rows), hi, lo);
     }
 }
 
-// C = U V^T over depth K for planes U [.][K] and V [.][K], a 128 x 128 tile per block, 64 x 64 per wave.
+// C = U V^T over depth K for planes U [.][K] and V [.][K], a WT x WT tile per block, a quarter per wave.
 // MODE: what becomes of C.
 constexpr int kNsGram = 0, kNsPoly = 1, kNsStep = 2, kNsLast = 3;
-template <int MODE, typename T, bool TALL>
+template <int MODE, int WT, typename T, bool TALL>
 __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
-    __shared__ __attribute__((aligned(16))) _Float16 buf[2][4][kWT * kWK];        // two stages of U.hi U.lo V.hi V.lo
+    constexpr int WV = WT / 2, F = WV / 16;                                       // a wave's part of the tile, in fragments
+    // Stages of U and V, rows of 128 bytes.  The symmetric products have about one block to a compute unit: three stages, two of them on their way.
+    constexpr int STAGES = MODE == kNsGram || MODE == kNsPoly ? 3 : 2;
+    extern __shared__ __attribute__((aligned(16))) char ns_lds[];
+    _Float16 (*buf)[2][WT * 2 * kWK] = reinterpret_cast<_Float16 (*)[2][WT * 2 * kWK]>(ns_lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t b = blockIdx.z;
-    int ti, tj;
-    if constexpr (MODE == kNsGram || MODE == kNsPoly) {
-        int t = blockIdx.x, tiles = (int)(a.np / kWT);                             // upper tiles, row by row
-        ti = 0;
-        while (t >= tiles - ti) { t -= tiles - ti; ++ti; }
-        tj = ti + t;
-    } else {
-        ti = blockIdx.x;
-        tj = blockIdx.y;
-    }
+    // Blocks go to the eight dies in turn; each die gets an eighth of the tiles in one piece, ordered by squares of 4 x 4 tiles: the blocks
+    // that run together on a die then share rows of U and V in its L2.
+    constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
+    const uint32_t ty = (uint32_t)(a.np / WT), tx = SYM ? ty : (uint32_t)(a.lp / WT), sx = (tx + 3) / 4, per = (((ty + 3) / 4) * sx * 16 + 7) / 8;
+    const uint32_t slot = (blockIdx.x & 7) * per + (blockIdx.x >> 3), sq = slot >> 4;
+    const int ti = (int)(sq / sx * 4 + ((slot >> 2) & 3)), tj = (int)(sq % sx * 4 + (slot & 3));
+    if ((uint32_t)ti >= ty || (uint32_t)tj >= tx || (SYM && tj < ti)) return;        // of a symmetric result only the upper tiles
     const int64_t K = MODE == kNsGram ? a.lp : a.np;
-    const int64_t uoff = MODE == kNsGram ? b * a.x_plane : b * a.g_plane;
-    const int64_t voff = MODE == kNsPoly ? b * a.g_plane : b * a.x_plane;
-    const Planes U = MODE == kNsGram ? a.x : (MODE == kNsPoly ? a.g : a.p);
-    const Planes V = MODE == kNsGram ? a.x : (MODE == kNsPoly ? a.g : a.xt);
-    const _Float16 *src[4] = {U.hi + uoff + ti * (int64_t)kWT * K, U.lo + uoff + ti * (int64_t)kWT * K,
-                              V.hi + voff + tj * (int64_t)kWT * K, V.lo + voff + tj * (int64_t)kWT * K};
-    // a wave stages one operand's tile: 128 rows of 64 bytes, eight loads of 64 lanes x 16 bytes straight into LDS
-    const _Float16 *mine = src[wave] + (lane >> 2) * K + (lane & 3) * 8;
+    const _Float16 *U = (MODE == kNsGram ? a.x.p + b * a.x_plane : (MODE == kNsPoly ? a.g.p : a.p.p) + b * a.g_plane) + ti * (int64_t)WT * 2 * K;
+    const _Float16 *V = (MODE == kNsPoly ? a.g.p + b * a.g_plane : (MODE == kNsGram ? a.x.p : a.xt.p) + b * a.x_plane) + tj * (int64_t)WT * 2 * K;
+    // Rows go straight to LDS, eight a load of 64 lanes x 16 bytes; piece c of row r lies at place c ^ (r / 2 % 8), so that the lanes of a
+    // fragment read, which want one piece of 16 rows, find them in different banks.
+    const _Float16 *mine = (wave < 2 ? U : V) + (lane >> 3) * 2 * K + ((lane & 7) ^ ((lane >> 4) & 3)) * 8;
+    constexpr int LOADS = WT / 16;                                                // of a wave: half of the rows of one operand
     auto stage = [&](int s, int64_t k) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(mine + c * 16 * K + k),
-                                             (__attribute__((address_space(3))) void *)(&buf[s][wave][c * 16 * kWK]), 16, 0, 0);
+        for (int c = 0; c < LOADS; ++c) {
+            const int r0 = ((wave & 1) * LOADS + c) * 8;
+            // (r / 2) % 8 of row r0 + lane / 8 is lane / 16 with 4 added for odd r0 / 8
+            const _Float16 *src = mine + (int64_t)r0 * 2 * K + 2 * k;
+            const int flip = (r0 >> 3) & 1 ? 32 : 0;                              // piece index ^ 4: 32 numbers up or down
+            src += flip ? (((lane & 7) ^ ((lane >> 4) & 3)) & 4 ? -32 : 32) : 0;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                             (__attribute__((address_space(3))) void *)(&buf[s][wave >> 1][r0 * 64]), 16, 0, 0);
+        }
     };
-    f32x4 acc[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-    const int frag = (lane & 15) * kWK + (lane >> 4) * 8;
-    // the loads of the other waves have to be in LDS too: each waits for its own before the barrier
-    auto arrived = [] {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // the loads of the other waves have to be in LDS too: each waits for its own (all but those of the newest stage) before the barrier
+    auto arrived = [&](bool all) {
+        if (all) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
         __syncthreads();
     };
-    stage(0, 0);
-    arrived();
-    int s = 0;
-    for (int64_t k = 0; k < K; k += kWK, s ^= 1) {
-        if (k + kWK < K) stage(s ^ 1, k + kWK);
-        f16x8 uh[4], ul[4], vh[4], vl[4];
+    f32x4 acc[F][F];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uh[i] = *reinterpret_cast<const f16x8 *>(&buf[s][0][(wi + 16 * i) * kWK + frag]);
-            ul[i] = *reinterpret_cast<const f16x8 *>(&buf[s][1][(wi + 16 * i) * kWK + frag]);
-            vh[i] = *reinterpret_cast<const f16x8 *>(&buf[s][2][(wj + 16 * i) * kWK + frag]);
-            vl[i] = *reinterpret_cast<const f16x8 *>(&buf[s][3][(wj + 16 * i) * kWK + frag]);
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const int wi = (wave >> 1) * WV, wj = (wave & 1) * WV;
+    const int turn = ((lane & 15) >> 1) & 7, row0 = (lane & 15) * 64;
+    const int at_hi = row0 + ((lane >> 4) ^ turn) * 8, at_lo = row0 + (((lane >> 4) + 4) ^ turn) * 8;
+    constexpr int64_t AHEAD = (STAGES - 1) * kWK;
+#pragma unroll
+    for (int g = 0; g < STAGES - 1; ++g) stage(g, g * kWK);                       // K is a multiple of 128: there are that many
+    arrived(STAGES == 2);
+    int s = 0;
+    for (int64_t k = 0; k < K; k += kWK, s = s + 1 == STAGES ? 0 : s + 1) {
+        const bool more = k + AHEAD < K;
+        if (more) stage(s == 0 ? STAGES - 1 : s - 1, k + AHEAD);
+        f16x8 uh[F], ul[F], vh[F], vl[F];
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            const _Float16 *u = &buf[s][0][(wi + 16 * i) * 64], *v = &buf[s][1][(wj + 16 * i) * 64];
+            uh[i] = *reinterpret_cast<const f16x8 *>(u + at_hi);
+            ul[i] = *reinterpret_cast<const f16x8 *>(u + at_lo);
+            vh[i] = *reinterpret_cast<const f16x8 *>(v + at_hi);
+            vl[i] = *reinterpret_cast<const f16x8 *>(v + at_lo);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < F; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < F; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul[i], vh[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
-            }
-        arrived();
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
+        arrived(STAGES == 2 || !more);
     }
     constexpr float kInv = 1.0f / (kPlaneScale * kPlaneScale);
     const NsShift sh = ns_shift(a, b);
     const float unscale = MODE == kNsGram ? kInv / sh.now / sh.now : (MODE == kNsStep ? kInv * (sh.next / sh.now) : (MODE == kNsLast ? kInv / sh.now : kInv));
     const int n0 = lane & 15, m0 = (lane >> 4) * 4;                               // C: row m0 + r, column n0
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t row = ti * (int64_t)kWT + wi + 16 * i + m0, col = tj * (int64_t)kWT + wj + 16 * j + n0;
+        for (int j = 0; j < F; ++j) {
+            const int64_t row = ti * (int64_t)WT + wi + 16 * i + m0, col = tj * (int64_t)WT + wj + 16 * j + n0;
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * unscale;
@@ -440,13 +505,12 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
                 for (int r = 0; r < 4; ++r)
                     if (row + r < a.n && col < a.len) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, row + r, col), v[r]);
             } else {
-                const bool sym = MODE != kNsStep;
                 const Planes C = MODE == kNsGram ? a.g : (MODE == kNsPoly ? a.p : a.x);
                 const Planes Ct = MODE == kNsStep ? a.xt_new : C;
-                const int64_t off = sym ? b * a.g_plane : b * a.x_plane, ld = sym ? a.np : a.lp;
-                if constexpr (MODE == kNsPoly) {                                  // a I + b G + c G^2
-                    const int64_t at = off + col * a.np + row;                    // G is symmetric: four consecutive entries of its row `col`
-                    const f16x4 gh = *reinterpret_cast<const f16x4 *>(a.g.hi + at), gl = *reinterpret_cast<const f16x4 *>(a.g.lo + at);
+                const int64_t off = SYM ? b * a.g_plane : b * a.x_plane, ld = SYM ? a.np : a.lp;
+                const int64_t turned = off + Planes::at(col, row, a.np);               // four consecutive numbers of row `col`
+                if constexpr (MODE == kNsPoly) {                                       // a I + b G + c G^2, G symmetric
+                    const f16x4 gh = *reinterpret_cast<const f16x4 *>(a.g.p + turned), gl = *reinterpret_cast<const f16x4 *>(a.g.p + turned + 32);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         v[r] = a.cc * v[r] + a.cb * (((float)gh[r] + (float)gl[r]) * (1.0f / kPlaneScale)) + (row + r == col ? a.ca : 0.f);
@@ -458,18 +522,16 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
                     split16(v[r], h, l);
                     hi[r] = h;
                     lo[r] = l;
-                    C.hi[off + (row + r) * ld + col] = h;
-                    C.lo[off + (row + r) * ld + col] = l;
+                    C.put(off + Planes::at(row + r, col, ld), h, l);
                 }
-                if (!sym || ti != tj) {
-                    *reinterpret_cast<f16x4 *>(Ct.hi + off + col * a.np + row) = hi;
-                    *reinterpret_cast<f16x4 *>(Ct.lo + off + col * a.np + row) = lo;
+                if (!SYM || ti != tj) {
+                    *reinterpret_cast<f16x4 *>(Ct.p + turned) = hi;
+                    *reinterpret_cast<f16x4 *>(Ct.p + turned + 32) = lo;
                 }
             }
         }
 }
 
-// ---- entry points ------------------------------------------------------------------------------------------------------
 }  // namespace gatmi
 
 using namespace gatmi;
@@ -551,6 +613,27 @@ static int run_narrow(const NsMatrix &mat, int64_t batch, int steps, double ca, 
     return GATMI_OK;
 }
 
+// One product.  Tiles of 128, of 64 where those are fewer than kTileBlocks.
+constexpr int64_t kTileBlocks = 128;
+template <int MODE, typename T, bool TALL>
+static int ns_gemm(const WideArgs &a, int64_t batch, hipStream_t st) {
+    constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
+    const int64_t ty = a.np / 128, tx = SYM ? ty : a.lp / 128;
+    auto blocks = [&](int64_t w) {
+        const int64_t y = a.np / w, x = SYM ? y : a.lp / w;
+        return dim3((unsigned)((((y + 3) / 4) * ((x + 3) / 4) * 16 + 7) / 8 * 8), 1, (unsigned)batch);
+    };
+    const bool wide = (SYM ? ty * (ty + 1) / 2 : ty * tx) * batch >= kTileBlocks;
+    const size_t lds = (SYM ? 3 : 2) * (wide ? 128 : 64) * 256;
+    auto kernel = wide ? ns_gemm_kernel<MODE, 128, T, TALL> : ns_gemm_kernel<MODE, 64, T, TALL>;
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return fail(GATMI_EHIP, "newton_schulz: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, blocks(wide ? 128 : 64), dim3(256), lds, st, a);
+    return GATMI_OK;
+}
+
 template <typename T, bool TALL>
 static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, double cb, double cc, double eps, float *ws, hipStream_t st) {
     WideArgs a;
@@ -559,33 +642,30 @@ static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, do
     a.len = std::max(mat.m, mat.n);
     a.np = round_up(a.n, kWT);
     a.lp = round_up(a.len, kWT);
-    a.x_plane = a.np * a.lp;
-    a.g_plane = a.np * a.np;
+    a.x_plane = 2 * a.np * a.lp;
+    a.g_plane = 2 * a.np * a.np;
     a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.eps = eps;
     a.growth = std::max(1, (int)std::ceil(std::log2(ns_bound(steps, ca, cb, cc))));
     a.norm = reinterpret_cast<double *>(ws);
     a.shift = reinterpret_cast<int32_t *>(ws + 2 * (size_t)batch * kNormBlocks);
     _Float16 *p = reinterpret_cast<_Float16 *>(ws + wide_head(batch));
     const size_t xs = (size_t)batch * a.x_plane, gs = (size_t)batch * a.g_plane;
-    a.x = {p, p + xs};
-    a.xt = {p + 2 * xs, p + 3 * xs};
-    a.xt_new = {p + 4 * xs, p + 5 * xs};
-    a.g = {p + 6 * xs, p + 6 * xs + gs};
-    a.p = {p + 6 * xs + 2 * gs, p + 6 * xs + 3 * gs};
-    hipLaunchKernelGGL((ns_norm_kernel<T>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);
+    a.x.p = p;
+    a.xt.p = p + xs;
+    a.xt_new.p = p + 2 * xs;
+    a.g.p = p + 3 * xs;
+    a.p.p = p + 3 * xs + gs;
+    const bool vec = mat.x_row % 4 == 0 && mat.x_batch % 4 == 0 && reinterpret_cast<uintptr_t>(mat.x) % (4 * sizeof(T)) == 0;
+    if (vec) hipLaunchKernelGGL((ns_norm_kernel<T, true>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);
     const int64_t rows = TALL ? a.lp : a.np, cols = TALL ? a.np : a.lp;
     hipLaunchKernelGGL((ns_split_kernel<T, TALL>), dim3((unsigned)(cols / 32), (unsigned)(rows / 32), (unsigned)batch), dim3(256), 0, st, a);
-    const unsigned tn = (unsigned)(a.np / kWT), tl = (unsigned)(a.lp / kWT), sym = tn * (tn + 1) / 2;
     for (int k = 0; k < steps; ++k) {
         a.step = k;
-        hipLaunchKernelGGL((ns_gemm_kernel<kNsGram, T, TALL>), dim3(sym, 1, (unsigned)batch), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((ns_gemm_kernel<kNsPoly, T, TALL>), dim3(sym, 1, (unsigned)batch), dim3(256), 0, st, a);
-        if (k + 1 < steps) {
-            hipLaunchKernelGGL((ns_gemm_kernel<kNsStep, T, TALL>), dim3(tn, tl, (unsigned)batch), dim3(256), 0, st, a);
-            std::swap(a.xt, a.xt_new);
-        } else {
-            hipLaunchKernelGGL((ns_gemm_kernel<kNsLast, T, TALL>), dim3(tn, tl, (unsigned)batch), dim3(256), 0, st, a);
-        }
+        if (int rc = ns_gemm<kNsGram, T, TALL>(a, batch, st)) return rc;
+        if (int rc = ns_gemm<kNsPoly, T, TALL>(a, batch, st)) return rc;
+        if (int rc = k + 1 < steps ? ns_gemm<kNsStep, T, TALL>(a, batch, st) : ns_gemm<kNsLast, T, TALL>(a, batch, st)) return rc;
+        std::swap(a.xt, a.xt_new);
     }
     GATMI_LAUNCH_CHECK("newton_schulz");
     return GATMI_OK;

@@ -862,34 +862,73 @@ def inner_product_decoder(z, activation="sigmoid", dropout=0.0, seed=None):
 _FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
-def _float_type(what, *ts):
+def _float_type(what, t, *others):
     """Code of the one dtype (fp32 or bf16) that all tensors share."""
-    if ts[0].dtype not in _FLOATS or any(t.dtype != ts[0].dtype for t in ts):
-        raise TypeError("%s: fp32 or bf16 tensors of one type expected, got %s" % (what, ", ".join(str(t.dtype) for t in ts)))
-    return _FLOATS[ts[0].dtype]
+    code = _FLOATS.get(t.dtype)
+    if code is None or any(o.dtype != t.dtype for o in others):
+        raise TypeError("%s: fp32 or bf16 tensors of one type expected, got %s" % (what, ", ".join(str(o.dtype) for o in (t, *others))))
+    return code
 
 
-def _same_device(what, *ts):
-    _require_cuda(*ts)
-    devs = {t.device for t in ts if t is not None}
-    if len(devs) > 1:
-        raise ValueError("%s: tensors on different devices: %s" % (what, ", ".join(sorted(map(str, devs)))))
-    return ts[0].device
+def _same_device(what, t, *others):
+    _require_cuda(t, *others)
+    dev = t.device
+    for o in others:
+        if o is not None and o.device != dev:
+            raise ValueError("%s: tensors on different devices: %s and %s" % (what, dev, o.device))
+    return dev
+
+
+def _launch(device, name, *args):
+    """One library call on `device`, on the stream torch currently records on there."""
+    if device.index == torch.cuda.current_device():
+        rc = getattr(_lib.lib, name)(*args, _lib.current_stream())
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(_lib.lib, name)(*args, _lib.current_stream())
+    if rc:
+        _lib.check(rc, name)
+
+
+def _scratch(floats, device):
+    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+
+
+_Int64x3 = ctypes.c_int64 * 3
 
 
 def _strides(t):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+    s = t.stride()
+    return _Int64x3(s[0], s[1], s[2])
 
 
 def _attn_rows(t, width):
     """t [B, N, heads, D] as rows the kernels take: D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
-    if t.shape[-1] != width:
-        return torch.nn.functional.pad(t, (0, width - t.shape[-1]))
-    unit = 16 // t.element_size()
-    if t.stride(3) == 1 and all(s % unit == 0 for s in t.stride()[:3]) and t.data_ptr() % 16 == 0:
+    if t.shape[3] != width:
+        return torch.nn.functional.pad(t, (0, width - t.shape[3]))
+    s, low = t.stride(), 15 // t.element_size()                    # strides are multiples of 4 (fp32) or 8 (bf16) elements
+    if s[3] == 1 and not ((s[0] | s[1] | s[2]) & low) and not (t.data_ptr() & 15):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
+    """(rows of q, k, v as the kernels read them, out with padded width, lse or None, bias strides)"""
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    dtype = _FLOATS[q.dtype]
+    unit = 4 if dtype == _lib.DTYPE_F32 else 8
+    width = (D + unit - 1) // unit * unit
+    dev = q.device
+    qr, kr, vr = _attn_rows(q, width), _attn_rows(k, width), _attn_rows(v, width)
+    out = torch.empty((B, Nq, H, width), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=dev) if need else None
+    ws = _scratch(_lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, Hkv, width), dev)
+    strides = (0, Nk) if bias is None else (bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1))
+    _launch(dev, "gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr), vr.data_ptr(), _strides(vr),
+            ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(lse), ptr(ws))
+    return qr, kr, vr, out, lse, strides
 
 
 class DotAttentionFn(torch.autograd.Function):
@@ -897,25 +936,11 @@ class DotAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, bias, key_sizes, query_sizes, scale):
-        B, Nq, H, D = q.shape
-        Nk, Hkv = k.shape[1], k.shape[2]
-        dtype = _FLOATS[q.dtype]
-        unit = 4 if dtype == _lib.DTYPE_F32 else 8
-        width = (D + unit - 1) // unit * unit
-        qr, kr, vr = (_attn_rows(t, width) for t in (q, k, v))
-        out = torch.empty((B, Nq, H, width), dtype=q.dtype, device=q.device)
-        need = any(ctx.needs_input_grad[:3])
-        lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if need else None
-        floats = _lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, Hkv, width)
-        ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        bb, br = (0, Nk) if bias is None else (bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1))
-        with torch.cuda.device(q.device):
-            _lib.call("gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, ptr(qr), _strides(qr), ptr(kr), _strides(kr), ptr(vr), _strides(vr),
-                      ptr(bias), bb, br, ptr(key_sizes), ptr(query_sizes), scale, ptr(out), ptr(lse), ptr(ws), _lib.current_stream())
-        if need:
-            ctx.save_for_backward(qr, kr, vr, out, lse, bias, key_sizes, query_sizes)
-            ctx.scale, ctx.D, ctx.bias_strides = scale, D, (bb, br)
-        return out[..., :D] if width != D else out
+        D = q.shape[3]
+        qr, kr, vr, out, lse, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
+        ctx.save_for_backward(qr, kr, vr, out, lse, bias, key_sizes, query_sizes)
+        ctx.scale, ctx.D, ctx.bias_strides = scale, D, strides
+        return out[..., :D] if out.shape[3] != D else out
 
     @staticmethod
     def backward(ctx, dout):
@@ -925,11 +950,10 @@ class DotAttentionFn(torch.autograd.Function):
         D = ctx.D
         dr = _attn_rows(dout, width)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (qr, kr, vr))
-        delta = torch.empty_like(lse)
-        with torch.cuda.device(qr.device):
-            _lib.call("gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], ptr(qr), _strides(qr), ptr(kr), _strides(kr), ptr(vr), _strides(vr),
-                      ptr(out), ptr(dr), _strides(dr), ptr(lse), ptr(bias), *ctx.bias_strides, ptr(key_sizes), ptr(query_sizes), ctx.scale,
-                      ptr(dq), ptr(dk), ptr(dv), ptr(delta), _lib.current_stream())
+        delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
+        _launch(qr.device, "gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr),
+                vr.data_ptr(), _strides(vr), out.data_ptr(), dr.data_ptr(), _strides(dr), lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
+                ptr(query_sizes), ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr())
         if width != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
         return dq, dk, dv, None, None, None, None
@@ -976,7 +1000,24 @@ def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, s
         if bias_mat.stride(2) != 1 or bias_mat.stride(1) < Nk:
             bias_mat = bias_mat.contiguous()
     scale = float(D) ** -0.5 if scale is None else float(scale)
-    return DotAttentionFn.apply(q, k, v, bias_mat, _sizes("key_sizes", key_sizes, B, dev), _sizes("query_sizes", query_sizes, B, dev), scale)
+    key_sizes, query_sizes = _sizes("key_sizes", key_sizes, B, dev), _sizes("query_sizes", query_sizes, B, dev)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return DotAttentionFn.apply(q, k, v, bias_mat, key_sizes, query_sizes, scale)
+    out = _dot_forward(q, k, v, bias_mat, key_sizes, query_sizes, scale, False)[3]
+    return out[..., :D] if out.shape[3] != D else out
+
+
+def _embed_forward(ids, table, scale):
+    """(ids flat, scale * table[ids])"""
+    rows, width = table.shape
+    flat = ids.reshape(-1)
+    flat = flat if flat.is_contiguous() else flat.contiguous()
+    n = flat.numel()
+    tb = table if table.stride(1) == 1 and table.stride(0) >= width else table.contiguous()
+    out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
+    _launch(table.device, "gatmi_embed_fwd", flat.data_ptr(), 8 * flat.element_size(), n, tb.data_ptr(), tb.stride(0), rows, width, _FLOATS[table.dtype], scale,
+            out.data_ptr())
+    return flat, out
 
 
 class EmbeddingFn(torch.autograd.Function):
@@ -984,18 +1025,10 @@ class EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ids, table, scale):
-        rows, width = table.shape
-        dtype = _FLOATS[table.dtype]
-        flat = ids.reshape(-1)
-        flat = flat if flat.is_contiguous() else flat.contiguous()
-        tb = table if table.stride(1) == 1 and table.stride(0) >= width else table.contiguous()
-        out = torch.empty((flat.numel(), width), dtype=table.dtype, device=table.device)
-        with torch.cuda.device(table.device):
-            _lib.call("gatmi_embed_fwd", ptr(flat), 8 * flat.element_size(), flat.numel(), ptr(tb), tb.stride(0), rows, width, dtype, scale, ptr(out),
-                      _lib.current_stream())
+        flat, out = _embed_forward(ids, table, scale)
         ctx.save_for_backward(flat)
-        ctx.scale, ctx.rows = scale, rows
-        return out.reshape(*ids.shape, width)
+        ctx.scale, ctx.rows = scale, table.shape[0]
+        return out
 
     @staticmethod
     def backward(ctx, dout):
@@ -1003,11 +1036,11 @@ class EmbeddingFn(torch.autograd.Function):
         n, rows, width = flat.numel(), ctx.rows, dout.shape[-1]
         d = dout.reshape(n, width)
         d = d if d.stride(1) == 1 and d.stride(0) >= width else d.contiguous()
-        grad = torch.empty((rows, width), dtype=dout.dtype, device=dout.device)
-        ws = torch.empty(_lib.lib.gatmi_embed_bwd_ws_floats(n, rows, width), dtype=torch.float32, device=dout.device)
-        with torch.cuda.device(dout.device):
-            _lib.call("gatmi_embed_bwd", ptr(flat), 8 * flat.element_size(), n, ptr(d), d.stride(0), rows, width, _FLOATS[dout.dtype], ctx.scale,
-                      ptr(grad), ptr(ws), _lib.current_stream())
+        dev = dout.device
+        grad = torch.empty((rows, width), dtype=dout.dtype, device=dev)
+        ws = _scratch(_lib.lib.gatmi_embed_bwd_ws_floats(n, rows, width), dev)
+        _launch(dev, "gatmi_embed_bwd", flat.data_ptr(), 8 * flat.element_size(), n, d.data_ptr(), d.stride(0), rows, width, _FLOATS[dout.dtype], ctx.scale,
+                grad.data_ptr(), ptr(ws))
         return None, grad, None
 
 
@@ -1021,13 +1054,14 @@ def embedding(ids, table, scale=1.0):
         raise ValueError("embedding: table is [rows, width], got %s" % (tuple(table.shape) if torch.is_tensor(table) else type(table),))
     _float_type("embedding", table)
     _same_device("embedding", table, ids)
-    return EmbeddingFn.apply(ids, table, float(scale))
+    if table.requires_grad and torch.is_grad_enabled():
+        return EmbeddingFn.apply(ids, table, float(scale))
+    return _embed_forward(ids, table, float(scale))[1]
 
 
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # a, b, c of the quintic usual for orthogonalised updates: steep at 0, and [0.7, 1.2] maps into itself
 
 
-@torch.no_grad()
 def newton_schulz(x, steps=5, eps=1e-7, coefficients=NEWTON_SCHULZ):
     """Every m x n matrix of x [..., m, n] (fp32 or bf16) with its singular values driven towards 1: from X = x / (|x|_F + eps), `steps`
     times X <- a X + b (X X^T) X + c (X X^T)^2 X, at fp32 accuracy whatever the type (gatmi_newton_schulz).  Outside autograd."""
@@ -1035,15 +1069,17 @@ def newton_schulz(x, steps=5, eps=1e-7, coefficients=NEWTON_SCHULZ):
         raise ValueError("newton_schulz: x is [..., m, n], got %s" % (tuple(x.shape) if torch.is_tensor(x) else type(x),))
     dtype = _float_type("newton_schulz", x)
     _require_cuda(x)
-    m, n = x.shape[-2:]
-    x3 = x.reshape(math.prod(x.shape[:-2]), m, n)
+    shape = x.shape
+    m, n = shape[-2:]
+    x3 = x.detach()
+    if x3.dim() != 3:
+        x3 = x3.reshape(math.prod(shape[:-2]), m, n)
     if x3.stride(2) != 1 or x3.stride(1) < n:
         x3 = x3.contiguous()
-    out = torch.empty(x3.shape, dtype=x.dtype, device=x.device)
-    a, b, c = (float(v) for v in coefficients)
-    batch = x3.shape[0]
-    ws = torch.empty(_lib.lib.gatmi_newton_schulz_ws_floats(batch, m, n), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.call("gatmi_newton_schulz", batch, m, n, ptr(x3), x3.stride(0), x3.stride(1), dtype, int(steps), a, b, c, float(eps),
-                  ptr(out), m * n, n, ptr(ws), _lib.current_stream())
-    return out.reshape(x.shape)
+    dev = x.device
+    out = torch.empty(shape, dtype=x.dtype, device=dev)
+    a, b, c = coefficients
+    ws = _scratch(_lib.lib.gatmi_newton_schulz_ws_floats(x3.shape[0], m, n), dev)
+    _launch(dev, "gatmi_newton_schulz", x3.shape[0], m, n, x3.data_ptr(), x3.stride(0), x3.stride(1), dtype, int(steps), float(a), float(b), float(c), float(eps),
+            out.data_ptr(), m * n, n, ptr(ws))
+    return out
