@@ -120,6 +120,28 @@ __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &a
 template <typename T>
 __device__ __forceinline__ void mma_rows(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) { mma<T, 64>(a, b, acc); }
 
+// Results of matrix instructions that a branch stands between them and their first other reader: hipcc (ROCm 7.2) counts the wait states such a
+// reader needs (10 at most here) along straight code and can miss them behind a branch, and the hardware does not wait by itself.  The
+// wait is therefore taken here, next to the matrix instructions, and the values pass through it.
+__device__ __forceinline__ void settle(f32x4 &a) { asm volatile("s_nop 10" : "+v"(a)); }
+__device__ __forceinline__ void settle(f32x4 &a, f32x4 &b) { asm volatile("s_nop 10" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void settle(f32x4 &a, f32x4 &b, f32x4 &c, f32x4 &d) { asm volatile("s_nop 10" : "+v"(a), "+v"(b), "+v"(c), "+v"(d)); }
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&z)[N]) {
+    static_assert(N == 1 || N == 2 || N == 4, "tiles of a lane");
+    if constexpr (N == 1) settle(z[0]);
+    else if constexpr (N == 2) settle(z[0], z[1]);
+    else settle(z[0], z[1], z[2], z[3]);
+}
+template <int M, int N>
+__device__ __forceinline__ void settle(f32x4 (&z)[M][N]) {
+    static_assert(M == 1 || M == 2, "tiles of a lane");
+    if constexpr (M == 1) settle(z[0]);
+    else if constexpr (N == 1) settle(z[0][0], z[1][0]);
+    else if constexpr (N == 2) settle(z[0][0], z[0][1], z[1][0], z[1][1]);
+    else asm volatile("s_nop 10" : "+v"(z[0][0]), "+v"(z[0][1]), "+v"(z[0][2]), "+v"(z[0][3]), "+v"(z[1][0]), "+v"(z[1][1]), "+v"(z[1][2]), "+v"(z[1][3]));
+}
+
 // The second product sums over CHUNK staged rows.  Its B operand is made of score tiles (C layout: row 4 q + r of a
 // tile in register r), its A operand reads the staged rows column-wise in the same order of rows.
 template <typename T>
@@ -154,6 +176,9 @@ __device__ __forceinline__ Frag<T> frag_row(const char *tile, int row0, int c) {
     return frag_load<T, DP>(tile + S::at(row0 + (lane & 15), c * 4 * S::PIECE + (lane >> 4) * S::PIECE));
 }
 
+// how a kernel gets the mask: there is none; as floats (single rows, and columns that shared heads walk); as bits
+constexpr int kNoMask = 0, kFloats = 1, kBits = 2;
+
 // ---- arguments ---------------------------------------------------------------------------------------------------------
 struct DotRows {              // [B, N, heads, D] rows: element strides, D contiguous
     const void *p;
@@ -166,6 +191,8 @@ struct DotArgs {
     float *lse, *delta;                 // [B, H, Nq]: log2 of the row's sum of exponentials; <do, out>
     const float *bias;
     int64_t bias_batch, bias_row;
+    const ulonglong2 *row_words, *col_words;      // the mask as bits (dot_mask_kernel), or null
+    int64_t row_words_batch, col_words_batch;     // of one graph; 0: one mask for all
     const int32_t *key_sizes, *query_sizes;
     int64_t b0;                         // first graph of this launch
     int B, Nq, Nk, H, Hkv, group, D;    // B: graphs of this launch
@@ -181,9 +208,9 @@ __device__ __forceinline__ int graph_size(const int32_t *sizes, int64_t b, int n
 // (graph, head), which read the same keys and values; with a mask the heads of one (graph, tile, split), which read the same part of it.
 // Groups are dealt to the dies in turn (so that graphs of unequal sizes spread), the last groups that do not fill a round are cut into eight equal pieces.
 struct DotBlock { int64_t b; int hk, tile, split; bool ok; };
-template <bool BIAS>
+template <int MASK>
 __device__ __forceinline__ DotBlock dot_block(const DotArgs &a) {
-    const uint32_t inner = BIAS ? a.Hkv : a.tiles * a.splits, groups = BIAS ? (uint32_t)a.B * a.tiles * a.splits : (uint32_t)a.B * a.Hkv;
+    const uint32_t inner = MASK ? a.Hkv : a.tiles * a.splits, groups = MASK ? (uint32_t)a.B * a.tiles * a.splits : (uint32_t)a.B * a.Hkv;
     const uint32_t die = blockIdx.x & 7, at = blockIdx.x >> 3, whole = groups / 8 * inner;       // blocks of a die that belong to whole rounds
     uint32_t group = at / inner * 8 + die, i = at % inner;
     DotBlock r;
@@ -194,7 +221,7 @@ __device__ __forceinline__ DotBlock dot_block(const DotArgs &a) {
         group = groups / 8 * 8 + item / inner;
         i = item % inner;
     }
-    if constexpr (BIAS) {
+    if constexpr (MASK != kNoMask) {
         r.hk = i;
         r.split = group % a.splits; group /= a.splits;
         r.tile = group % a.tiles;
@@ -239,6 +266,52 @@ __device__ __forceinline__ void arrived() {
     else __builtin_amdgcn_wave_barrier();
 }
 
+// ---- the mask as bits --------------------------------------------------------------------------------------------------------
+// Every head of every pass reads the mask of a row; as floats that was most of the bytes of small heads.  Read once, it becomes 64 entries
+// a word, along the rows and along the columns: {attended, attended with a bias other than 0}.  Hard masks need the first only; where a tile has a
+// bit in the second, the kernels read the floats too.
+__global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_t bias_batch, int64_t bias_row, int Nq, int Nk, ulonglong2 *row_words, ulonglong2 *col_words) {
+    __shared__ uint16_t part[2][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rw = (Nk + 63) / 64, cw = (Nq + 63) / 64;
+    const uint32_t tj = blockIdx.x % rw, ti = blockIdx.x / rw % cw;
+    const int64_t b = blockIdx.x / rw / cw;
+    const int j = tj * 64 + lane;
+    const float *p = bias + b * bias_batch + j;
+    uint32_t seen = 0, soft = 0;
+    float v[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = ti * 64 + wave * 16 + r;
+        v[r] = i < Nq && j < Nk ? p[i * bias_row] : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = ti * 64 + wave * 16 + r;
+        const bool a = v[r] > kAttended, s = a && v[r] != 0.f;
+        const uint64_t wa = __ballot(a), ws = __ballot(s);
+        if (lane == 0 && i < Nq) row_words[(b * Nq + i) * rw + tj] = make_ulonglong2(wa, ws);
+        seen |= (uint32_t)a << r;
+        soft |= (uint32_t)s << r;
+    }
+    part[0][wave][lane] = (uint16_t)seen;
+    part[1][wave][lane] = (uint16_t)soft;
+    __syncthreads();
+    if (wave == 0 && j < Nk) {
+        uint64_t w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) w[k] = (uint64_t)part[k][0][lane] | (uint64_t)part[k][1][lane] << 16 | (uint64_t)part[k][2][lane] << 32 | (uint64_t)part[k][3][lane] << 48;
+        col_words[(b * Nk + j) * cw + ti] = make_ulonglong2(w[0], w[1]);
+    }
+}
+// the first `n` of 64 entries
+__device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0 : (1ull << n) - 1); }
+// z where bit `pos` of w is set, -inf elsewhere
+__device__ __forceinline__ float where_bit(uint32_t w, int pos, float z) {
+    const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)w, pos, 1);
+    return __uint_as_float((__float_as_uint(z) & m) | (0xff800000u & ~m));
+}
+
 // biases of four consecutive keys of one query, -inf behind the row
 __device__ __forceinline__ f32x4 bias4(const float *row, int j, int nk) {
     f32x4 v;
@@ -252,15 +325,65 @@ __device__ __forceinline__ f32x4 bias4(const float *row, int j, int nk) {
     }
     return v;
 }
-// scores of four keys in units of log2 from raw products, -inf where a key is not attended
-__device__ __forceinline__ f32x4 masked_scores(f32x4 z, float scale2, f32x4 bias, int j, int keys) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) z[r] = bias[r] > kAttended && j + r < keys ? fmaf(z[r], scale2, bias[r] * kLog2e) : -INFINITY;
-    return z;
-}
 __device__ __forceinline__ bool some_attended(f32x4 bias) {
     return __ballot(fmaxf(fmaxf(bias[0], bias[1]), fmaxf(bias[2], bias[3])) > kAttended) != 0;
 }
+
+// The mask of one lane's row over a tile of KT keys.  In a lane only the bits of its own keys (16 t + 4 q .. + 3) count.
+template <int MASK, int KT>
+struct RowMask {
+    const float *bias;                  // the row's floats and words
+    const ulonglong2 *words;
+    ulonglong2 next;                    // of the tile to come
+    f32x4 floats[MASK == kFloats ? KT / 16 : 1];
+    uint32_t lo, hi;                    // attended keys of the present tile, shifted by 4 q
+    bool soft;                          // some attended entry of the wave's tile has a bias other than 0
+    __device__ __forceinline__ void init(const DotArgs &a, int64_t b, int64_t i) {
+        if constexpr (MASK != kNoMask) bias = a.bias + b * a.bias_batch + i * a.bias_row;
+        if constexpr (MASK == kBits) words = a.row_words + b * a.row_words_batch + i * ((a.Nk + 63) / 64);
+    }
+    __device__ __forceinline__ void fetch(int j, int nk) {
+        const int q = (threadIdx.x & 63) >> 4;
+        if constexpr (MASK == kBits) next = words[j >> 6];
+        if constexpr (MASK == kFloats) {
+#pragma unroll
+            for (int t = 0; t < KT / 16; ++t) floats[t] = bias4(bias, j + 16 * t + 4 * q, nk);
+        }
+    }
+    // takes what was fetched for the tile at j; keys from `end` on are not attended
+    __device__ __forceinline__ void take(int j, int end) {
+        const int q = (threadIdx.x & 63) >> 4;
+        uint64_t w = first_bits(end - j);
+        soft = false;
+        if constexpr (MASK == kBits) {
+            w &= next.x >> (j & 63);
+            soft = __ballot((next.y >> (j & 63) & w) != 0) != 0;
+        }
+        w >>= 4 * q;
+        lo = (uint32_t)w;
+        hi = (uint32_t)(w >> 32);
+        if constexpr (MASK == kFloats) {
+            soft = true;
+#pragma unroll
+            for (int t = 0; t < KT / 16; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!(floats[t][r] > kAttended)) (t < 2 ? lo : hi) &= ~(1u << (16 * (t & 1) + r));
+        }
+    }
+    __device__ __forceinline__ bool some(int t) const { return __ballot(((t < 2 ? lo : hi) >> (16 * (t & 1)) & 15u) != 0) != 0; }
+    // raw products of tile t -> what exp2(fma(z, factor(), -base)) takes
+    __device__ __forceinline__ void apply(f32x4 &z, int t, int j, int nk, float scale2) const {
+        if (MASK != kNoMask && soft) {
+            const f32x4 f = MASK == kFloats ? floats[t] : bias4(bias, j + 16 * t + 4 * ((threadIdx.x & 63) >> 4), nk);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] = fmaf(z[r], scale2, f[r] * kLog2e);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[r] = where_bit(t < 2 ? lo : hi, 16 * (t & 1) + r, z[r]);
+    }
+    __device__ __forceinline__ float factor(float scale2) const { return MASK != kNoMask && soft ? 1.f : scale2; }
+};
 
 __device__ __forceinline__ float over_groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, 64));
@@ -282,13 +405,13 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {
 // A wave owns NQ x 16 rows.  KEYW = false: four waves with rows of their own walk the staged tiles together.  KEYW = true: for 16 rows or
 // fewer, the four waves have the same rows and walk different tiles, each staging its own, and join at the end.
 // SPLIT: the block covers one range of the keys and leaves its unnormalised sums.
-template <typename T, int DP, bool KEYW, int NQ, bool SPLIT, bool BIAS>
+template <typename T, int DP, bool KEYW, int NQ, bool SPLIT, int MASK>
 __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int KT = KEYW ? S::KTW : S::KT, TILE = KT * S::ROW, KS = KT / 16, DT = S::DT, ROWS = KEYW ? 16 : 64 * NQ, OWNERS = KEYW ? 4 : 1, STEP = OWNERS * KT;
     constexpr bool ONES = DP == 8 && S::SIZE == 4;              // eight columns of the last product are free: one of them sums the probabilities
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const DotBlock blk = dot_block<BIAS>(a);
+    const DotBlock blk = dot_block<MASK>(a);
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
@@ -300,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
     int row[NQ], qi[NQ], head[NQ];
     bool live[NQ];
     Frag<T> qf[NQ][S::FRAGS];
-    const float *bias_row[NQ];
+    RowMask<MASK, KT> mask[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
         row[u] = blk.tile * ROWS + ((KEYW ? 0 : wave) * NQ + u) * 16 + n;
@@ -313,7 +436,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
 #pragma unroll
             for (int c = 0; c < S::FRAGS; ++c) qf[u][c] = frag_negated<T>(qf[u][c]);
         }
-        bias_row[u] = BIAS ? a.bias + b * a.bias_batch + i * a.bias_row : nullptr;
+        mask[u].init(a, b, i);
     }
     f32x4 o[NQ][DT];
     float m[NQ], l[NQ];                 // every term of a row is formed against the same m, which follows the maximum only when that has grown by 8 (in log2): see below
@@ -329,35 +452,30 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
         stage<T, DP, KT, KEYW ? 1 : 4>(to, a.k, a.v, j1 - j, a.D, KEYW ? 0 : wave,
                                    [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
     };
-    f32x4 bias[NQ][KS];
-    auto fetch_bias = [&](int j) {
-        if constexpr (BIAS) {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u)
-#pragma unroll
-                for (int t = 0; t < KS; ++t) bias[u][t] = bias4(bias_row[u], j + 16 * t + 4 * q4, a.Nk);
-        }
-    };
     int j = j0 + (KEYW ? wave * KT : 0), at = 0;
     if (j < j1) {
         fetch(buf(0), j);
-        fetch_bias(j);
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) mask[u].fetch(j, a.Nk);
     }
     for (; j < j1; j += STEP, at ^= 1) {
         arrived<!KEYW>();
         const char *ks = buf(at), *vs = ks + TILE;
         if (j + STEP < j1) fetch(buf(at ^ 1), j + STEP);
+        const bool plain = MASK == kNoMask && j + KT <= j1;           // no entry of this tile is masked
         f32x4 z[NQ][KS];
         bool some[NQ][KS];               // the same for the whole wave
         float top[NQ];
+        if (!plain) {
 #pragma unroll
-        for (int u = 0; u < NQ; ++u) top[u] = -INFINITY;
+            for (int u = 0; u < NQ; ++u) mask[u].take(j, j1);
+        }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
-            bool any = !BIAS;
+            bool any = MASK == kNoMask;
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
-                some[u][t] = !BIAS || some_attended(bias[u][t]);
+                some[u][t] = MASK == kNoMask || mask[u].some(t);
                 any |= some[u][t];
                 z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
             }
@@ -369,23 +487,27 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
                     for (int u = 0; u < NQ; ++u)
                         if (some[u][t]) mma<T, DP>(kf, qf[u][c], z[u][t]);
                 }
+                if constexpr (MASK != kNoMask) {
+                    if constexpr (NQ == 1) settle(z[0][t]);
+                    else settle(z[0][t], z[1][t]);
+                }
             }
         }
-        const bool plain = !BIAS && j + KT <= j1;                     // no entry of this tile is masked
+        if constexpr (MASK == kNoMask) settle(z);
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
-            if (plain) {
-#pragma unroll
-                for (int t = 0; t < KS; ++t) top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
-                top[u] *= a.scale2;
-            } else {
+            float factor = a.scale2;
+            if (!plain) {
+                factor = mask[u].factor(a.scale2);
 #pragma unroll
                 for (int t = 0; t < KS; ++t)
-                    if (some[u][t]) {
-                        z[u][t] = masked_scores(z[u][t], a.scale2, BIAS ? bias[u][t] : (f32x4){0.f, 0.f, 0.f, 0.f}, j + 16 * t + 4 * q4, j1);
-                        top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
-                    }
+                    if (some[u][t]) mask[u].apply(z[u][t], t, j, a.Nk, a.scale2);
             }
+            top[u] = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < KS; ++t)
+                if (some[u][t]) top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
+            top[u] *= factor;
             // The running maximum only has to keep the exponentials in range.  It is raised, and the sums shrunk, when some row's
             // maximum has passed it by 8: after the first tiles hardly ever.  Terms up to 2^8 lose nothing in fp32 or bf16.
             if (__ballot(top[u] > m[u] + 8.f)) {
@@ -404,13 +526,16 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
                 if (some[u][t]) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        z[u][t][r] = __builtin_amdgcn_exp2f(plain ? fmaf(z[u][t][r], a.scale2, -base) : z[u][t][r] - base);
+                        z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -base));
                         if constexpr (!ONES) l[u] += z[u][t][r];
                     }
                 }
             }
         }
-        if (j + STEP < j1) fetch_bias(j + STEP);
+        if (j + STEP < j1) {
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) mask[u].fetch(j + STEP, a.Nk);
+        }
 #pragma unroll
         for (int c = 0; c < KT / S::CHUNK; ++c) {
             constexpr int PER = S::CHUNK / 16;
@@ -576,12 +701,12 @@ __global__ __launch_bounds__(256) void dot_join_kernel(DotArgs a, int64_t rows) 
 }
 
 // ---- backward: dq and delta ------------------------------------------------------------------------------------------------
-template <typename T, int DP, int NQ, bool BIAS>
+template <typename T, int DP, int NQ, int MASK>
 __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int KT = S::KT, DT = S::DT, ROWS = 64 * NQ, PER = S::CHUNK / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const DotBlock blk = dot_block<BIAS>(a);
+    const DotBlock blk = dot_block<MASK>(a);
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
@@ -595,7 +720,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
     int qi[NQ], head[NQ];
     float lse[NQ], delta[NQ];
     Frag<T> qf[NQ][S::FRAGS], df[NQ][S::FRAGS];
-    const float *bias_row[NQ];
+    RowMask<MASK, KT> mask[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
         const int row = blk.tile * ROWS + (wave * NQ + u) * 16 + n;
@@ -626,7 +751,11 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
         delta[u] = over_groups_sum(dot);
         lse[u] = live ? a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] : INFINITY;
         if (q4 == 0 && qi[u] < a.Nq) a.delta[(b * a.H + head[u]) * a.Nq + qi[u]] = delta[u];
-        bias_row[u] = BIAS ? a.bias + b * a.bias_batch + i * a.bias_row : nullptr;
+        mask[u].init(a, b, i);
+    }
+    if (keys > 0) {
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) mask[u].fetch(0, a.Nk);
     }
     f32x4 acc[NQ][DT];
 #pragma unroll
@@ -634,17 +763,20 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     for (int j = 0, at = 0; j < keys; j += KT, at ^= 1) {
-        f32x4 bias[NQ][KT / 16];
-        if constexpr (BIAS) {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u)
-#pragma unroll
-                for (int t = 0; t < KT / 16; ++t) bias[u][t] = bias4(bias_row[u], j + 16 * t + 4 * q4, a.Nk);
-        }
         arrived<true>();
         const char *ks = buf(at), *vs = ks + S::TILE;
         if (j + KT < keys) fetch(buf(at ^ 1), j + KT);
-        const bool plain = !BIAS && j + KT <= keys;
+        const bool plain = MASK == kNoMask && j + KT <= keys;
+        float factor[NQ];
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+            factor[u] = a.scale2;
+            if (!plain) {
+                mask[u].take(j, keys);
+                factor[u] = mask[u].factor(a.scale2);
+            }
+            if (j + KT < keys) mask[u].fetch(j + KT, a.Nk);
+        }
 #pragma unroll
         for (int c = 0; c < KT / S::CHUNK; ++c) {
             f32x4 z[NQ][PER];
@@ -659,7 +791,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 #pragma unroll
                 for (int u = 0; u < NQ; ++u) {
                     z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-                    some[u] = !BIAS || some_attended(bias[u][r0 / 16]);
+                    some[u] = MASK == kNoMask || mask[u].some(r0 / 16);
                     use[u] |= some[u];
                     here |= some[u];
                 }
@@ -675,17 +807,14 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
                             mma<T, DP>(vf, df[u][f], dp[u]);
                         }
                 }
+                if constexpr (NQ == 1) settle(z[0][t], dp[0]);
+                else settle(z[0][t], dp[0], z[1][t], dp[1]);
 #pragma unroll
                 for (int u = 0; u < NQ; ++u)
                     if (some[u]) {
-                        if (plain) {
+                        if (!plain) mask[u].apply(z[u][t], r0 / 16, j, a.Nk, a.scale2);
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], a.scale2, -lse[u])) * (dp[u][r] - delta[u]);
-                        } else {
-                            const f32x4 s = masked_scores(z[u][t], a.scale2, BIAS ? bias[u][r0 / 16] : (f32x4){0.f, 0.f, 0.f, 0.f}, j + r0 + 4 * q4, keys);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(s[r] - lse[u]) * (dp[u][r] - delta[u]);
-                        }
+                        for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor[u], -lse[u])) * (dp[u][r] - delta[u]);
                     }
             }
             if (!any) continue;
@@ -719,14 +848,14 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 // ---- backward: dk and dv -----------------------------------------------------------------------------------------------------
 // A wave owns NK x 16 keys (one per lane of a row of 16) and walks all rows of the sharing heads.  Rows behind the last one come with
 // lse = inf: their probabilities are zero.
-template <typename T, int DP, int NK, bool BIAS>
+template <typename T, int DP, int NK, int MASK>
 __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_bwd_kv_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int QT = S::KT, DT = S::DT, KEYS = 64 * NK, PER = S::CHUNK / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
-    __shared__ const float *bias_rows[2][BIAS ? QT : 1];
-    const DotBlock blk = dot_block<BIAS>(a);
+    __shared__ const float *bias_rows[2][MASK ? QT : 1];
+    const DotBlock blk = dot_block<MASK>(a);
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
@@ -743,11 +872,13 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
             const int64_t at = (b * a.H + blk.hk * a.group + row - i * a.group) * a.Nq + i;
             lses[to][threadIdx.x] = r0 + (int)threadIdx.x < rows ? a.lse[at] : INFINITY;
             deltas[to][threadIdx.x] = a.delta[at];
-            if constexpr (BIAS) bias_rows[to][threadIdx.x] = a.bias + b * a.bias_batch + i * a.bias_row;
+            if constexpr (MASK != kNoMask) bias_rows[to][threadIdx.x] = a.bias + b * a.bias_batch + i * a.bias_row;
         }
     };
     if (rows > 0) fetch(0, 0);
     int key[NK], col[NK];
+    const ulonglong2 *words[NK];          // the mask of this lane's key over the queries (kBits: rows are queries, the heads are not shared)
+    ulonglong2 next[NK];
     Frag<T> kf[NK][S::FRAGS], vf[NK][S::FRAGS];
     f32x4 dk[NK][DT], dv[NK][DT];
 #pragma unroll
@@ -761,6 +892,10 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
 #pragma unroll
             for (int c = 0; c < S::FRAGS; ++c) kf[u][c] = frag_negated<T>(kf[u][c]);
         }
+        if constexpr (MASK == kBits) {
+            words[u] = a.col_words + b * a.col_words_batch + (int64_t)col[u] * ((a.Nq + 63) / 64);
+            if (rows > 0) next[u] = words[u][0];
+        }
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[u][t] = dv[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -768,6 +903,19 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
         arrived<true>();
         const char *qs = buf(at), *ds = qs + S::TILE;
         if (r0 + QT < rows) fetch(at ^ 1, r0 + QT);
+        uint32_t lo[NK], hi[NK];
+        bool soft[NK];
+#pragma unroll
+        for (int u = 0; u < NK; ++u) {
+            soft[u] = MASK == kFloats;
+            if constexpr (MASK == kBits) {
+                const uint64_t w = next[u].x >> (r0 & 63);
+                soft[u] = __ballot(next[u].y >> (r0 & 63) != 0) != 0;
+                lo[u] = (uint32_t)(w >> (4 * q4));
+                hi[u] = (uint32_t)(w >> (4 * q4) >> 32);
+                if (r0 + QT < rows) next[u] = words[u][(r0 + QT) >> 6];
+            }
+        }
 #pragma unroll
         for (int c = 0; c < QT / S::CHUNK; ++c) {
             f32x4 p[NK][PER], z[NK][PER];
@@ -783,11 +931,14 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                 for (int u = 0; u < NK; ++u) {
                     z[u][t] = dp[u] = p[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
                     some[u] = true;
-                    if constexpr (BIAS) {
+                    if constexpr (MASK == kBits) some[u] = __ballot(((s0 < 32 ? lo[u] : hi[u]) >> (s0 & 31) & 15u) != 0) != 0;
+                    if constexpr (MASK != kNoMask) {
+                        if (soft[u]) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
-                        some[u] = some_attended(bias[u]);
+                            for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
+                        }
                     }
+                    if constexpr (MASK == kFloats) some[u] = some_attended(bias[u]);
                     use[u] |= some[u];
                     here |= some[u];
                 }
@@ -803,14 +954,28 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                             mma<T, DP>(df, vf[u][f], dp[u]);
                         }
                 }
+                if constexpr (NK == 1) settle(z[0][t], dp[0]);
+                else settle(z[0][t], dp[0], z[1][t], dp[1]);
                 const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[at][s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[at][s0 + 4 * q4]);
 #pragma unroll
                 for (int u = 0; u < NK; ++u)
                     if (some[u]) {
+                        float factor = a.scale2;
+                        if constexpr (MASK != kNoMask) {
+                            if (soft[u]) {
+                                factor = 1.f;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) z[u][t][r] = fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e);
+                            }
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                if constexpr (MASK == kBits) z[u][t][r] = where_bit(s0 < 32 ? lo[u] : hi[u], (s0 & 31) + r, z[u][t][r]);
+                                else z[u][t][r] = bias[u][r] > kAttended ? z[u][t][r] : -INFINITY;
+                            }
+                        }
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float s = BIAS ? (bias[u][r] > kAttended ? fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e) - lse[r] : -INFINITY) : fmaf(z[u][t][r], a.scale2, -lse[r]);
-                            p[u][t][r] = __builtin_amdgcn_exp2f(s);
+                            p[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -lse[r]));
                             z[u][t][r] = p[u][t][r] * (dp[u][r] - delta[r]);
                         }
                     }
@@ -910,6 +1075,41 @@ static int dot_launch(const char *what, K kernel, const DotArgs &a, size_t lds, 
 
 using namespace gatmi;
 
+// floats that hold the words of `graphs` masks: rows, then columns
+static size_t dot_mask_floats(int64_t graphs, int64_t Nq, int64_t Nk) {
+    return 4 * (size_t)graphs * ((size_t)Nq * ((Nk + 63) / 64) + (size_t)Nk * ((Nq + 63) / 64));
+}
+
+// builds the words of the mask of one call (graphs: B, or 1 where all share it) and points `a` at them
+static int dot_mask_words(const char *what, DotArgs *a, int64_t graphs, float *words, bool build, hipStream_t st) {
+    GATMI_REQUIRE(words, GATMI_EINVAL, "%s: mask words are null", what);
+    GATMI_REQUIRE_ALIGNED(words);
+    const int64_t rw = (a->Nk + 63) / 64, cw = (a->Nq + 63) / 64, per = rw * cw;
+    ulonglong2 *rows = reinterpret_cast<ulonglong2 *>(words), *cols = rows + graphs * a->Nq * rw;
+    a->row_words = rows;
+    a->col_words = cols;
+    a->row_words_batch = graphs > 1 ? a->Nq * rw : 0;
+    a->col_words_batch = graphs > 1 ? a->Nk * cw : 0;
+    if (!build) return GATMI_OK;
+    GATMI_REQUIRE(per <= kDotBlocks, GATMI_ERANGE, "%s: a mask of %d x %d", what, a->Nq, a->Nk);
+    const int64_t step = std::max<int64_t>(1, kDotBlocks / per);
+    for (int64_t b0 = 0; b0 < graphs; b0 += step) {
+        const int64_t now = std::min(step, graphs - b0);
+        hipLaunchKernelGGL(dot_mask_kernel, dim3((unsigned)(now * per)), dim3(256), 0, st, a->bias + b0 * a->bias_batch, a->bias_batch, a->bias_row, a->Nq, a->Nk,
+                           rows + b0 * a->Nq * rw, cols + b0 * a->Nk * cw);
+    }
+    GATMI_LAUNCH_CHECK("dot_attn (mask)");
+    return GATMI_OK;
+}
+
+// whether the passes read the mask as words: more than one wave of rows walks it
+static bool dot_wants_words(int64_t rows) { return rows > 16; }
+
+extern "C" size_t gatmi_dot_attn_mask_floats(int64_t B, int32_t Nq, int32_t Nk, int64_t bias_batch) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0) return 0;
+    return dot_mask_floats(bias_batch ? B : 1, Nq, Nk);
+}
+
 extern "C" size_t gatmi_dot_attn_fwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0) return 0;
     const int64_t rows = (int64_t)Nq * (H / Hkv);
@@ -929,9 +1129,9 @@ static int dot_fwd_run(DotArgs a, int64_t B, hipStream_t st) {
         a.b0 = b0;
         a.B = (int)std::min(step, B - b0);
         int rc;
-#define RUN(keyw, nq, split, bytes)                                                                                          \
-    (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, true>, a, bytes, st)                        \
-            : dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, false>, a, bytes, st))
+#define RUN(keyw, nq, split, bytes)                                                                                                      \
+    (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, keyw ? kFloats : kBits>, a, bytes, st)                   \
+            : dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, kNoMask>, a, bytes, st))
         if (per == 16) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
         else if (per == 64) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);
         else rc = a.splits > 1 ? RUN(false, S::NQ, true, lds) : RUN(false, S::NQ, false, lds);
@@ -963,7 +1163,7 @@ static int dot_fwd_run(DotArgs a, int64_t B, hipStream_t st) {
 
 extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
                                   const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const float *bias, int64_t bias_batch,
-                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse, float *ws, void *stream) {
+                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse, float *mask_words, float *ws, void *stream) {
     if (int rc = dot_check("dot_attn_fwd", B, Nq, Nk, H, Hkv, D, dtype)) return rc;
     GATMI_REQUIRE(std::isfinite(scale), GATMI_EINVAL, "dot_attn_fwd: scale %g", (double)scale);
     if (B == 0 || Nq == 0) return GATMI_OK;
@@ -977,7 +1177,7 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     GATMI_REQUIRE_ALIGNED(out);
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq == 1, GATMI_EINVAL, "dot_attn_fwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
     a.out = out; a.lse = lse; a.bias = Nk > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
-    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::fabs(scale) * kLog2e;
+    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);      // above 0: -inf stays -inf
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     const int64_t rows = (int64_t)Nq * a.group;
     a.splits = dot_splits(B, rows, Hkv, Nk);
@@ -988,6 +1188,8 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
         a.part_ml = ws + (size_t)B * Hkv * rows * a.splits * D;
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (a.bias && (mask_words || dot_wants_words(rows)))
+        if (int rc = dot_mask_words("dot_attn_fwd", &a, bias_batch ? B : 1, mask_words, true, st)) return rc;
 #define RUN(T, dp) dot_fwd_run<T, dp>(a, B, st)
     GATMI_DOT_DISPATCH(RUN)
 #undef RUN
@@ -1009,9 +1211,13 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
             a.b0 = b0;
             a.B = (int)std::min(step, B - b0);
             int rc;
-#define RUN(kernel, n) (a.bias ? dot_launch("dot_attn_bwd", kernel<T, DP, n, true>, a, 4 * S::TILE, st) : dot_launch("dot_attn_bwd", kernel<T, DP, n, false>, a, 4 * S::TILE, st))
-            if (pass == 0) rc = wide ? RUN(dot_bwd_q_kernel, S::NQ) : RUN(dot_bwd_q_kernel, 1);
-            else rc = wide ? RUN(dot_bwd_kv_kernel, S::NK) : RUN(dot_bwd_kv_kernel, 1);
+#define RUN(kernel, n, mask) dot_launch("dot_attn_bwd", kernel<T, DP, n, mask>, a, 4 * S::TILE, st)
+#define RUN_Q(n) (a.bias ? RUN(dot_bwd_q_kernel, n, kBits) : RUN(dot_bwd_q_kernel, n, kNoMask))
+#define RUN_KV(n) (a.bias ? (a.group == 1 ? RUN(dot_bwd_kv_kernel, n, kBits) : RUN(dot_bwd_kv_kernel, n, kFloats)) : RUN(dot_bwd_kv_kernel, n, kNoMask))
+            if (pass == 0) rc = wide ? RUN_Q(S::NQ) : RUN_Q(1);
+            else rc = wide ? RUN_KV(S::NK) : RUN_KV(1);
+#undef RUN_KV
+#undef RUN_Q
 #undef RUN
             if (rc) return rc;
         }
@@ -1023,7 +1229,8 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
 extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
                                   const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const void *out, const void *dout,
                                   const int64_t *dout_stride, const float *lse, const float *bias, int64_t bias_batch, int64_t bias_row,
-                                  const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *dq, void *dk, void *dv, float *delta, void *stream) {
+                                  const int32_t *key_sizes, const int32_t *query_sizes, float scale, float *mask_words, void *dq, void *dk, void *dv,
+                                  float *delta, void *stream) {
     if (int rc = dot_check("dot_attn_bwd", B, Nq, Nk, H, Hkv, D, dtype)) return rc;
     GATMI_REQUIRE(std::isfinite(scale), GATMI_EINVAL, "dot_attn_bwd: scale %g", (double)scale);
     if (B == 0 || (Nq == 0 && Nk == 0)) return GATMI_OK;
@@ -1046,9 +1253,11 @@ extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq <= 1, GATMI_EINVAL, "dot_attn_bwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
     a.dq = dq; a.dk = dk; a.dv = dv; a.lse = const_cast<float *>(lse); a.delta = delta;
     a.bias = Nk > 0 && Nq > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
-    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::fabs(scale) * kLog2e;
+    a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);      // above 0: -inf stays -inf
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    if (a.bias)
+        if (int rc = dot_mask_words("dot_attn_bwd", &a, bias_batch ? B : 1, mask_words, false, st)) return rc;
 #define RUN(T, dp) dot_bwd_run<T, dp>(a, B, st)
     GATMI_DOT_DISPATCH(RUN)
 #undef RUN

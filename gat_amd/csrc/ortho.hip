@@ -140,6 +140,8 @@ struct NsProduct {
                 const double *ar = A + (16 * p + i) * LD + kq, *br = B + (16 * q + i) * LD + kq;        // B symmetric: its column is its row
 #pragma unroll
                 for (int k = 0; k < NP; k += 4) acc[u] = __builtin_amdgcn_mfma_f64_16x16x4f64(ar[k], br[k], acc[u], 0, 0, 0);
+                // the wait states before the first other reader, which comes behind a branch, taken here (see settle in dot_attn.hip)
+                asm volatile("s_nop 15\n\ts_nop 3" : "+v"(acc[u]));
             }
         }
     }
