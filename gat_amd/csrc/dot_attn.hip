@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 #include "device_common.h"
@@ -126,6 +127,12 @@ __device__ __forceinline__ void mma_rows(const Frag<T> &a, const Frag<T> &b, f32
 __device__ __forceinline__ void settle(f32x4 &a) { asm volatile("s_nop 10" : "+v"(a)); }
 __device__ __forceinline__ void settle(f32x4 &a, f32x4 &b) { asm volatile("s_nop 10" : "+v"(a), "+v"(b)); }
 __device__ __forceinline__ void settle(f32x4 &a, f32x4 &b, f32x4 &c, f32x4 &d) { asm volatile("s_nop 10" : "+v"(a), "+v"(b), "+v"(c), "+v"(d)); }
+// the same for sums that stay where they are (the end of a loop's body)
+__device__ __forceinline__ void settle_sums() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 10" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 template <int N>
 __device__ __forceinline__ void settle(f32x4 (&z)[N]) {
     static_assert(N == 1 || N == 2 || N == 4, "tiles of a lane");
@@ -463,104 +470,114 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
         const char *ks = buf(at), *vs = ks + TILE;
         if (j + STEP < j1) fetch(buf(at ^ 1), j + STEP);
         const bool plain = MASK == kNoMask && j + KT <= j1;           // no entry of this tile is masked
-        f32x4 z[NQ][KS];
-        bool some[NQ][KS];               // the same for the whole wave
-        float top[NQ];
-        if (!plain) {
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) mask[u].take(j, j1);
-        }
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-            bool any = MASK == kNoMask;
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                some[u][t] = MASK == kNoMask || mask[u].some(t);
-                any |= some[u][t];
-                z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            }
-            if (any) {
-#pragma unroll
-                for (int c = 0; c < S::FRAGS; ++c) {
-                    const Frag<T> kf = frag_row<T, DP>(ks, 16 * t, c);
-#pragma unroll
-                    for (int u = 0; u < NQ; ++u)
-                        if (some[u][t]) mma<T, DP>(kf, qf[u][c], z[u][t]);
-                }
-                if constexpr (MASK != kNoMask) {
-                    if constexpr (NQ == 1) settle(z[0][t]);
-                    else settle(z[0][t], z[1][t]);
-                }
-            }
-        }
-        if constexpr (MASK == kNoMask) settle(z);
+        bool has[NQ][KS], full = true;   // tiles with an attended key, the same for the whole wave
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
-            float factor = a.scale2;
-            if (!plain) {
-                factor = mask[u].factor(a.scale2);
-#pragma unroll
-                for (int t = 0; t < KS; ++t)
-                    if (some[u][t]) mask[u].apply(z[u][t], t, j, a.Nk, a.scale2);
-            }
-            top[u] = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < KS; ++t)
-                if (some[u][t]) top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
-            top[u] *= factor;
-            // The running maximum only has to keep the exponentials in range.  It is raised, and the sums shrunk, when some row's
-            // maximum has passed it by 8: after the first tiles hardly ever.  Terms up to 2^8 lose nothing in fp32 or bf16.
-            if (__ballot(top[u] > m[u] + 8.f)) {
-                top[u] = over_groups_max(top[u]);
-                const float now = fmaxf(m[u], top[u]), shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - now);
-                m[u] = now;
-                l[u] *= shrink;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[u][t][r] *= shrink;
-            }
-            const float base = m[u] == -INFINITY ? 0.f : m[u];
+            if (!plain) mask[u].take(j, j1);
 #pragma unroll
             for (int t = 0; t < KS; ++t) {
-                if (some[u][t]) {
+                has[u][t] = MASK == kNoMask || mask[u].some(t);
+                full &= has[u][t];
+            }
+        }
+        // Straight code where no tile is empty: its reads and matrix instructions run ahead of each other.
+        auto walk = [&](auto skip) __attribute__((always_inline)) {
+            constexpr bool SKIP = decltype(skip)::value;
+            f32x4 z[NQ][KS];
+            float top[NQ];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -base));
-                        if constexpr (!ONES) l[u] += z[u][t][r];
+            for (int t = 0; t < KS; ++t) {
+                bool any = !SKIP;
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) {
+                    any |= has[u][t];
+                    z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                }
+                if (any) {
+#pragma unroll
+                    for (int c = 0; c < S::FRAGS; ++c) {
+                        const Frag<T> kf = frag_row<T, DP>(ks, 16 * t, c);
+#pragma unroll
+                        for (int u = 0; u < NQ; ++u)
+                            if (!SKIP || has[u][t]) mma<T, DP>(kf, qf[u][c], z[u][t]);
+                    }
+                    if constexpr (SKIP) {
+                        if constexpr (NQ == 1) settle(z[0][t]);
+                        else settle(z[0][t], z[1][t]);
                     }
                 }
             }
-        }
+            if constexpr (!SKIP) settle(z);
+#pragma unroll
+            for (int u = 0; u < NQ; ++u) {
+                float factor = a.scale2;
+                if (!plain) {
+                    factor = mask[u].factor(a.scale2);
+#pragma unroll
+                    for (int t = 0; t < KS; ++t)
+                        if (!SKIP || has[u][t]) mask[u].apply(z[u][t], t, j, a.Nk, a.scale2);
+                }
+                top[u] = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < KS; ++t)
+                    if (!SKIP || has[u][t]) top[u] = fmaxf(top[u], fmaxf(fmaxf(z[u][t][0], z[u][t][1]), fmaxf(z[u][t][2], z[u][t][3])));
+                top[u] *= factor;
+                // The running maximum only has to keep the exponentials in range.  It is raised, and the sums shrunk, when some row's
+                // maximum has passed it by 8: after the first tiles hardly ever.  Terms up to 2^8 lose nothing in fp32 or bf16.
+                if (__ballot(top[u] > m[u] + 8.f)) {
+                    top[u] = over_groups_max(top[u]);
+                    const float now = fmaxf(m[u], top[u]), shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[u] - now);
+                    m[u] = now;
+                    l[u] *= shrink;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[u][t][r] *= shrink;
+                }
+                const float base = m[u] == -INFINITY ? 0.f : m[u];
+#pragma unroll
+                for (int t = 0; t < KS; ++t) {
+                    if (!SKIP || has[u][t]) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -base));
+                            if constexpr (!ONES) l[u] += z[u][t][r];
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < KT / S::CHUNK; ++c) {
+                constexpr int PER = S::CHUNK / 16;
+                bool any = !SKIP, use[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) {
+                    use[u] = has[u][c * PER] || has[u][c * PER + PER - 1];
+                    any |= use[u];
+                }
+                if (!any) continue;
+                Frag<T> pf[NQ];
+#pragma unroll
+                for (int u = 0; u < NQ; ++u) pf[u] = frag_scores<T>(&z[u][c * PER]);       // a tile without attended keys holds zeros
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    Frag<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, 16 * t);
+                    if constexpr (ONES) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) vf.v[r] = n == 8 ? 1.f : vf.v[r];
+                    }
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u)
+                        if (!SKIP || use[u]) mma_rows<T>(vf, pf[u], o[u][t]);
+                }
+            }
+            settle_sums();
+        };
+        if (MASK == kNoMask || full) walk(std::false_type{});
+        else walk(std::true_type{});
         if (j + STEP < j1) {
 #pragma unroll
             for (int u = 0; u < NQ; ++u) mask[u].fetch(j + STEP, a.Nk);
-        }
-#pragma unroll
-        for (int c = 0; c < KT / S::CHUNK; ++c) {
-            constexpr int PER = S::CHUNK / 16;
-            bool any = false;
-            bool use[NQ];
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) {
-                use[u] = some[u][c * PER] || some[u][c * PER + PER - 1];
-                any |= use[u];
-            }
-            if (!any) continue;
-            Frag<T> pf[NQ];
-#pragma unroll
-            for (int u = 0; u < NQ; ++u) pf[u] = frag_scores<T>(&z[u][c * PER]);       // a tile without attended keys holds zeros
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                Frag<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, 16 * t);
-                if constexpr (ONES) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) vf.v[r] = n == 8 ? 1.f : vf.v[r];
-                }
-#pragma unroll
-                for (int u = 0; u < NQ; ++u)
-                    if (use[u]) mma_rows<T>(vf, pf[u], o[u][t]);
-            }
         }
     }
     float sum[NQ];
@@ -775,59 +792,75 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
                 mask[u].take(j, keys);
                 factor[u] = mask[u].factor(a.scale2);
             }
-            if (j + KT < keys) mask[u].fetch(j + KT, a.Nk);
         }
+        bool has[NQ][KT / 16], full = true;
 #pragma unroll
-        for (int c = 0; c < KT / S::CHUNK; ++c) {
-            f32x4 z[NQ][PER];
-            bool use[NQ], any = false;
+        for (int u = 0; u < NQ; ++u)
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) use[u] = false;
+            for (int t = 0; t < KT / 16; ++t) {
+                has[u][t] = MASK == kNoMask || mask[u].some(t);
+                full &= has[u][t];
+            }
+        auto walk = [&](auto skip) __attribute__((always_inline)) {
+            constexpr bool SKIP = decltype(skip)::value;
 #pragma unroll
-            for (int t = 0; t < PER; ++t) {
-                const int r0 = c * S::CHUNK + 16 * t;
-                f32x4 dp[NQ];
-                bool some[NQ], here = false;
+            for (int c = 0; c < KT / S::CHUNK; ++c) {
+                f32x4 z[NQ][PER];
+                bool use[NQ], any = !SKIP;
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) {
-                    z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-                    some[u] = MASK == kNoMask || mask[u].some(r0 / 16);
-                    use[u] |= some[u];
-                    here |= some[u];
-                }
-                any |= here;
-                if (!here) continue;
+                for (int u = 0; u < NQ; ++u) use[u] = false;
 #pragma unroll
-                for (int f = 0; f < S::FRAGS; ++f) {
-                    const Frag<T> kf = frag_row<T, DP>(ks, r0, f), vf = frag_row<T, DP>(vs, r0, f);
+                for (int t = 0; t < PER; ++t) {
+                    const int r0 = c * S::CHUNK + 16 * t;
+                    f32x4 dp[NQ];
+                    bool here = !SKIP;
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u) {
+                        z[u][t] = dp[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                        use[u] |= has[u][r0 / 16];
+                        here |= has[u][r0 / 16];
+                    }
+                    any |= here;
+                    if (!here) continue;
+#pragma unroll
+                    for (int f = 0; f < S::FRAGS; ++f) {
+                        const Frag<T> kf = frag_row<T, DP>(ks, r0, f), vf = frag_row<T, DP>(vs, r0, f);
+#pragma unroll
+                        for (int u = 0; u < NQ; ++u)
+                            if (!SKIP || has[u][r0 / 16]) {
+                                mma<T, DP>(kf, qf[u][f], z[u][t]);
+                                mma<T, DP>(vf, df[u][f], dp[u]);
+                            }
+                    }
+                    if constexpr (NQ == 1) settle(z[0][t], dp[0]);
+                    else settle(z[0][t], dp[0], z[1][t], dp[1]);
 #pragma unroll
                     for (int u = 0; u < NQ; ++u)
-                        if (some[u]) {
-                            mma<T, DP>(kf, qf[u][f], z[u][t]);
-                            mma<T, DP>(vf, df[u][f], dp[u]);
+                        if (!SKIP || has[u][r0 / 16]) {
+                            if (!plain) mask[u].apply(z[u][t], r0 / 16, j, a.Nk, a.scale2);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor[u], -lse[u])) * (dp[u][r] - delta[u]);
                         }
                 }
-                if constexpr (NQ == 1) settle(z[0][t], dp[0]);
-                else settle(z[0][t], dp[0], z[1][t], dp[1]);
+                if (!any) continue;
+                Frag<T> zf[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u)
-                    if (some[u]) {
-                        if (!plain) mask[u].apply(z[u][t], r0 / 16, j, a.Nk, a.scale2);
+                for (int u = 0; u < NQ; ++u) zf[u] = frag_scores<T>(z[u]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) z[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor[u], -lse[u])) * (dp[u][r] - delta[u]);
-                    }
+                for (int t = 0; t < DT; ++t) {
+                    const Frag<T> kf = frag_turned<T, DP>(ks, c * S::CHUNK, 16 * t);
+#pragma unroll
+                    for (int u = 0; u < NQ; ++u)
+                        if (!SKIP || use[u]) mma_rows<T>(kf, zf[u], acc[u][t]);
+                }
             }
-            if (!any) continue;
-            Frag<T> zf[NQ];
+            settle_sums();
+        };
+        if (MASK == kNoMask || full) walk(std::false_type{});
+        else walk(std::true_type{});
+        if (j + KT < keys) {
 #pragma unroll
-            for (int u = 0; u < NQ; ++u) zf[u] = frag_scores<T>(z[u]);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const Frag<T> kf = frag_turned<T, DP>(ks, c * S::CHUNK, 16 * t);
-#pragma unroll
-                for (int u = 0; u < NQ; ++u)
-                    if (use[u]) mma_rows<T>(kf, zf[u], acc[u][t]);
-            }
+            for (int u = 0; u < NQ; ++u) mask[u].fetch(j + KT, a.Nk);
         }
     }
 #pragma unroll
@@ -916,88 +949,101 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                 if (r0 + QT < rows) next[u] = words[u][(r0 + QT) >> 6];
             }
         }
+        bool has[NK][QT / 16], full = MASK != kFloats;
 #pragma unroll
-        for (int c = 0; c < QT / S::CHUNK; ++c) {
-            f32x4 p[NK][PER], z[NK][PER];
-            bool use[NK], any = false;
+        for (int u = 0; u < NK; ++u)
 #pragma unroll
-            for (int u = 0; u < NK; ++u) use[u] = false;
+            for (int t = 0; t < QT / 16; ++t) {
+                has[u][t] = MASK != kBits || __ballot(((t < 2 ? lo[u] : hi[u]) >> (16 * (t & 1)) & 15u) != 0) != 0;
+                full &= has[u][t];
+            }
+        auto walk = [&](auto skip) __attribute__((always_inline)) {
+            constexpr bool SKIP = decltype(skip)::value;
 #pragma unroll
-            for (int t = 0; t < PER; ++t) {
-                const int s0 = c * S::CHUNK + 16 * t;
-                f32x4 dp[NK], bias[NK];
-                bool some[NK], here = false;
+            for (int c = 0; c < QT / S::CHUNK; ++c) {
+                f32x4 p[NK][PER], z[NK][PER];
+                bool use[NK], any = !SKIP;
 #pragma unroll
-                for (int u = 0; u < NK; ++u) {
-                    z[u][t] = dp[u] = p[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-                    some[u] = true;
-                    if constexpr (MASK == kBits) some[u] = __ballot(((s0 < 32 ? lo[u] : hi[u]) >> (s0 & 31) & 15u) != 0) != 0;
-                    if constexpr (MASK != kNoMask) {
-                        if (soft[u]) {
+                for (int u = 0; u < NK; ++u) use[u] = false;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
-                        }
-                    }
-                    if constexpr (MASK == kFloats) some[u] = some_attended(bias[u]);
-                    use[u] |= some[u];
-                    here |= some[u];
-                }
-                any |= here;
-                if (!here) continue;
+                for (int t = 0; t < PER; ++t) {
+                    const int s0 = c * S::CHUNK + 16 * t;
+                    f32x4 dp[NK], bias[NK];
+                    bool some[NK], here = !SKIP;
 #pragma unroll
-                for (int f = 0; f < S::FRAGS; ++f) {
-                    const Frag<T> qf = frag_row<T, DP>(qs, s0, f), df = frag_row<T, DP>(ds, s0, f);
-#pragma unroll
-                    for (int u = 0; u < NK; ++u)
-                        if (some[u]) {
-                            mma<T, DP>(qf, kf[u][f], z[u][t]);
-                            mma<T, DP>(df, vf[u][f], dp[u]);
-                        }
-                }
-                if constexpr (NK == 1) settle(z[0][t], dp[0]);
-                else settle(z[0][t], dp[0], z[1][t], dp[1]);
-                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[at][s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[at][s0 + 4 * q4]);
-#pragma unroll
-                for (int u = 0; u < NK; ++u)
-                    if (some[u]) {
-                        float factor = a.scale2;
+                    for (int u = 0; u < NK; ++u) {
+                        z[u][t] = dp[u] = p[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                        some[u] = has[u][s0 / 16];
                         if constexpr (MASK != kNoMask) {
                             if (soft[u]) {
-                                factor = 1.f;
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) z[u][t][r] = fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e);
+                                for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
+                            }
+                        }
+                        if constexpr (MASK == kFloats) some[u] = some_attended(bias[u]);
+                        use[u] |= some[u];
+                        here |= some[u];
+                    }
+                    any |= here;
+                    if (!here) continue;
+#pragma unroll
+                    for (int f = 0; f < S::FRAGS; ++f) {
+                        const Frag<T> qf = frag_row<T, DP>(qs, s0, f), df = frag_row<T, DP>(ds, s0, f);
+#pragma unroll
+                        for (int u = 0; u < NK; ++u)
+                            if (!SKIP || some[u]) {
+                                mma<T, DP>(qf, kf[u][f], z[u][t]);
+                                mma<T, DP>(df, vf[u][f], dp[u]);
+                            }
+                    }
+                    if constexpr (NK == 1) settle(z[0][t], dp[0]);
+                    else settle(z[0][t], dp[0], z[1][t], dp[1]);
+                    const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[at][s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[at][s0 + 4 * q4]);
+#pragma unroll
+                    for (int u = 0; u < NK; ++u)
+                        if (!SKIP || some[u]) {
+                            float factor = a.scale2;
+                            if constexpr (MASK != kNoMask) {
+                                if (soft[u]) {
+                                    factor = 1.f;
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) z[u][t][r] = fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e);
+                                }
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    if constexpr (MASK == kBits) z[u][t][r] = where_bit(s0 < 32 ? lo[u] : hi[u], (s0 & 31) + r, z[u][t][r]);
+                                    else z[u][t][r] = bias[u][r] > kAttended ? z[u][t][r] : -INFINITY;
+                                }
                             }
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                if constexpr (MASK == kBits) z[u][t][r] = where_bit(s0 < 32 ? lo[u] : hi[u], (s0 & 31) + r, z[u][t][r]);
-                                else z[u][t][r] = bias[u][r] > kAttended ? z[u][t][r] : -INFINITY;
+                                p[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -lse[r]));
+                                z[u][t][r] = p[u][t][r] * (dp[u][r] - delta[r]);
                             }
                         }
+                }
+                if (!any) continue;
+                Frag<T> pf[NK], zf[NK];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            p[u][t][r] = __builtin_amdgcn_exp2f(fmaf(z[u][t][r], factor, -lse[r]));
-                            z[u][t][r] = p[u][t][r] * (dp[u][r] - delta[r]);
+                for (int u = 0; u < NK; ++u) {
+                    pf[u] = frag_scores<T>(p[u]);
+                    zf[u] = frag_scores<T>(z[u]);
+                }
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const Frag<T> df = frag_turned<T, DP>(ds, c * S::CHUNK, 16 * t), qf = frag_turned<T, DP>(qs, c * S::CHUNK, 16 * t);
+#pragma unroll
+                    for (int u = 0; u < NK; ++u)
+                        if (!SKIP || use[u]) {
+                            mma_rows<T>(df, pf[u], dv[u][t]);
+                            mma_rows<T>(qf, zf[u], dk[u][t]);
                         }
-                    }
+                }
             }
-            if (!any) continue;
-            Frag<T> pf[NK], zf[NK];
-#pragma unroll
-            for (int u = 0; u < NK; ++u) {
-                pf[u] = frag_scores<T>(p[u]);
-                zf[u] = frag_scores<T>(z[u]);
-            }
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const Frag<T> df = frag_turned<T, DP>(ds, c * S::CHUNK, 16 * t), qf = frag_turned<T, DP>(qs, c * S::CHUNK, 16 * t);
-#pragma unroll
-                for (int u = 0; u < NK; ++u)
-                    if (use[u]) {
-                        mma_rows<T>(df, pf[u], dv[u][t]);
-                        mma_rows<T>(qf, zf[u], dk[u][t]);
-                    }
-            }
-        }
+            settle_sums();
+        };
+        if (MASK == kNoMask || full) walk(std::false_type{});
+        else walk(std::true_type{});
     }
 #pragma unroll
     for (int u = 0; u < NK; ++u) {
