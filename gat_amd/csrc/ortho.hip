@@ -5,18 +5,19 @@
 // a in every step that follows (3.44^5 = 485 for the usual coefficients): with 16-bit operands five steps leave errors
 // of 2 to 10 %.  Two ways keep fp32's accuracy, by the length n of the shorter side:
 //
-// n <= 64 (`narrow`): with G = X^T X (n x n; the longer side is summed over), all factors are polynomials in G and
+// n <= 64 and more than 128 long (`narrow`): with G = X^T X (n x n; the longer side is summed over), all factors are polynomials in G and
 //   commute: the result is X Q(G) with an n x n matrix Q.  Three launches: G, Q, X Q, whatever the longer side.  Squaring the
 //   singular values doubles the digits that small ones need, so G, Q and the last product are formed in fp64 on
 //   v_mfma_f64_16x16x4_f64 (128 flop / clock / CU): for n <= 64 they are small.  |x|_F is the root of G's trace.
 //
-// n > 64 (`wide`): the steps themselves, three products each, on the 16-bit matrix instructions at fp32 accuracy: an
+// Otherwise the steps themselves, three products each, on the 16-bit matrix instructions at fp32 accuracy: an
 //   operand v is kept as hi + lo, two fp16 numbers of 11 bits each, and hi hi + hi lo + lo hi is summed in fp32 (relative error 2^-22;
 //   the missing lo lo is below it).  fp16 has few exponent bits, but the iteration bounds its operands: entries of X, X X^T and of the
 //   polynomial are below kMaxEntry (checked on the host for the given coefficients), so that one fixed scale
 //   2^13 keeps hi in range and lo of every entry that matters above the subnormals.  Where |x|_F is not far above eps, X is tiny: it is
 //   then kept times 2^e with e falling from step to step as X can grow (NsShift).  3 products at 16 times the rate of fp32's.
-//   X X^T and its square are symmetric: only tiles on and above the diagonal are formed, each is stored twice.
+//   `small` (n <= 64, at most 128 long): all steps in one block's LDS, one launch.  `wide` (n > 64): a launch per product; X X^T and its square
+//   are symmetric: only tiles on and above the diagonal are formed, each is stored twice.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -534,6 +535,140 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
         }
 }
 
+// ---- small -------------------------------------------------------------------------------------------------------------
+constexpr int kSmallThreads = 1024;          // 16 waves: one 16 x 16 tile of G and of the polynomial each
+constexpr int kSmallLong = 128;
+
+struct SmallArgs {
+    NsMatrix a;
+    int n, len;                              // short and long side
+    int steps, growth;
+    float ca, cb, cc;
+    double eps;
+};
+
+// Planes in LDS: row r of [rows][64 * G] values, 64 at a time as 32 hi, 32 lo, 32 hi, 32 lo; 16 bytes between rows spread the rows of a fragment
+// read over the banks.
+template <int G>
+struct LdsPlanes {
+    static constexpr int STRIDE = 128 * G + 8;
+    _Float16 *p;
+    __device__ __forceinline__ void put(int row, int k, float v) const {
+        _Float16 hi, lo;
+        split16(v, hi, lo);
+        _Float16 *q = p + row * STRIDE + (k >> 5) * 64 + (k & 31);
+        q[0] = hi;
+        q[32] = lo;
+    }
+    // hi and lo of the fragment of 16 rows at depth 32 c
+    __device__ __forceinline__ void frag(int row0, int c, f16x8 &hi, f16x8 &lo) const {
+        const int lane = threadIdx.x & 63;
+        const _Float16 *q = p + (row0 + (lane & 15)) * STRIDE + c * 64 + (lane >> 4) * 8;
+        hi = *reinterpret_cast<const f16x8 *>(q);
+        lo = *reinterpret_cast<const f16x8 *>(q + 32);
+    }
+};
+// acc += U V^T over depth 32 c .. of the rows at u0 and v0
+template <int GU, int GV>
+__device__ __forceinline__ void small_mma(const LdsPlanes<GU> &U, int u0, const LdsPlanes<GV> &V, int v0, int c, f32x4 &acc) {
+    f16x8 uh, ul, vh, vl;
+    U.frag(u0, c, uh, ul);
+    V.frag(v0, c, vh, vl);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ul, vh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh, vh, acc, 0, 0, 0);
+}
+
+// One matrix per block.  LT: the long side in pieces of 64.  A step: G = X X^T, then P = a I + b G + c G^2, then X <- P X; each
+// wave keeps its tile of G in registers for the sum of the second product.
+template <typename T, bool TALL, int LT>
+__global__ __launch_bounds__(kSmallThreads) void ns_small_kernel(SmallArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ns_lds[];
+    LdsPlanes<LT> X{reinterpret_cast<_Float16 *>(ns_lds)};
+    LdsPlanes<1> Xt{X.p + 64 * LdsPlanes<LT>::STRIDE}, G{Xt.p + 64 * LT * LdsPlanes<1>::STRIDE}, P{G.p + 64 * LdsPlanes<1>::STRIDE};
+    __shared__ double part[kSmallThreads / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = lane & 15, m0 = (lane >> 4) * 4;
+    const T *x = reinterpret_cast<const T *>(a.a.x) + (int64_t)blockIdx.x * a.a.x_batch;
+    T *out = reinterpret_cast<T *>(a.a.out) + (int64_t)blockIdx.x * a.a.out_batch;
+    constexpr int PER = 64 * 64 * LT / kSmallThreads;
+    const int rows = TALL ? a.len : a.n, cols = TALL ? a.n : a.len;
+    // thread t holds elements t, t + 1024, ... of the padded matrix, whose rows have W entries
+    constexpr int W = TALL ? 64 : 64 * LT;
+    float v[PER];
+    double s = 0;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        const int e = threadIdx.x + u * kSmallThreads, i = e / W, j = e % W;
+        v[u] = i < rows && j < cols ? ns_load<T>(x + i * a.a.x_row + j) : 0.f;
+        s += (double)v[u] * (double)v[u];
+    }
+    s = block_sum_f64(s, part, kSmallThreads / 64);
+    double inv = 1.0 / (sqrt(s) + a.eps);
+    const int e0 = ns_first_shift(sqrt(s) * inv);
+    inv = ldexp(inv, e0);
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+        const int e = threadIdx.x + u * kSmallThreads, i = e / W, j = e % W, sh = TALL ? j : i, lg = TALL ? i : j;
+        const float y = (float)((double)v[u] * inv);
+        X.put(sh, lg, y);
+        Xt.put(lg, sh, y);
+    }
+    __syncthreads();
+    constexpr float kInv = 1.0f / (kPlaneScale * kPlaneScale);
+    const int ti = (wave >> 2) * 16, tj = (wave & 3) * 16;
+    for (int step = 0; step < a.steps; ++step) {
+        const float now = ldexpf(1.f, max(0, e0 - step * a.growth)), next = ldexpf(1.f, max(0, e0 - (step + 1) * a.growth));
+        f32x4 g = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2 * LT; ++c) small_mma(X, ti, X, tj, c, g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            g[r] = g[r] * (kInv / now / now);
+            G.put(tj + n0, ti + m0 + r, g[r]);                       // G is symmetric: four consecutive entries of row tj + n0
+        }
+        __syncthreads();
+        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) small_mma(G, ti, G, tj, c, p);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) P.put(tj + n0, ti + m0 + r, a.cc * (p[r] * kInv) + a.cb * g[r] + (ti + m0 + r == tj + n0 ? a.ca : 0.f));
+        __syncthreads();
+        f32x4 y[LT];
+#pragma unroll
+        for (int u = 0; u < LT; ++u) {
+            y[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) small_mma(P, ti, Xt, tj + 64 * u, c, y[u]);
+        }
+        const bool last = step + 1 == a.steps;
+        const float scale = last ? kInv / now : kInv * (next / now);
+#pragma unroll
+        for (int u = 0; u < LT; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[u][r] *= scale;
+        if (last) {
+#pragma unroll
+            for (int u = 0; u < LT; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = ti + m0 + r, j = tj + 64 * u + n0;
+                    if (i < a.n && j < a.len) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, i, j), y[u][r]);
+                }
+        } else {
+            __syncthreads();                                         // X^T has been read by all
+#pragma unroll
+            for (int u = 0; u < LT; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    X.put(ti + m0 + r, tj + 64 * u + n0, y[u][r]);
+                    Xt.put(tj + 64 * u + n0, ti + m0 + r, y[u][r]);
+                }
+            __syncthreads();
+        }
+    }
+}
+
+// ---- entry points ------------------------------------------------------------------------------------------------------
 }  // namespace gatmi
 
 using namespace gatmi;
@@ -569,6 +704,11 @@ static double ns_bound(int steps, double a, double b, double c) {
     return worst;
 }
 
+// a step multiplies X by at most 2^this
+static int ns_growth(int steps, double a, double b, double c) { return std::max(1, (int)std::ceil(std::log2(ns_bound(steps, a, b, c)))); }
+
+static bool ns_is_small(int64_t s, int64_t l) { return s <= kNarrow && l <= kSmallLong; }
+
 static size_t narrow_ws(int64_t batch, int64_t n, int64_t len) {
     const size_t np = (size_t)round_up(n, 16);
     return 2 * (size_t)batch * (gram_parts(batch, len) + 1) * np * np;
@@ -582,6 +722,7 @@ static size_t wide_ws(int64_t batch, int64_t n, int64_t len) {
 extern "C" size_t gatmi_newton_schulz_ws_floats(int64_t batch, int64_t m, int64_t n) {
     if (batch <= 0 || m <= 0 || n <= 0) return 0;
     const int64_t s = std::min(m, n), l = std::max(m, n);
+    if (ns_is_small(s, l)) return 0;
     const int64_t at_once = std::min<int64_t>(batch, kBatchAtOnce);
     return s <= kNarrow ? narrow_ws(at_once, s, l) : wide_ws(at_once, s, l);
 }
@@ -637,6 +778,25 @@ static int ns_gemm(const WideArgs &a, int64_t batch, hipStream_t st) {
 }
 
 template <typename T, bool TALL>
+static int run_small(const NsMatrix &mat, int64_t batch, int steps, double ca, double cb, double cc, double eps, hipStream_t st) {
+    SmallArgs a;
+    a.a = mat;
+    a.n = (int)std::min(mat.m, mat.n);
+    a.len = (int)std::max(mat.m, mat.n);
+    a.steps = steps;
+    a.growth = ns_growth(steps, ca, cb, cc);
+    a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.eps = eps;
+    const int lt = a.len <= 64 ? 1 : 2;
+    const size_t lds = sizeof(_Float16) * (64 * (128 * lt + 8) + (64 * lt + 128) * (size_t)LdsPlanes<1>::STRIDE);
+    auto kernel = lt == 1 ? ns_small_kernel<T, TALL, 1> : ns_small_kernel<T, TALL, 2>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return fail(GATMI_EHIP, "newton_schulz: %s", hipGetErrorString(e));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)batch), dim3(kSmallThreads), lds, st, a);
+    GATMI_LAUNCH_CHECK("newton_schulz");
+    return GATMI_OK;
+}
+
+template <typename T, bool TALL>
 static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, double cb, double cc, double eps, float *ws, hipStream_t st) {
     WideArgs a;
     a.a = mat;
@@ -647,7 +807,7 @@ static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, do
     a.x_plane = 2 * a.np * a.lp;
     a.g_plane = 2 * a.np * a.np;
     a.ca = (float)ca; a.cb = (float)cb; a.cc = (float)cc; a.eps = eps;
-    a.growth = std::max(1, (int)std::ceil(std::log2(ns_bound(steps, ca, cb, cc))));
+    a.growth = ns_growth(steps, ca, cb, cc);
     a.norm = reinterpret_cast<double *>(ws);
     a.shift = reinterpret_cast<int32_t *>(ws + 2 * (size_t)batch * kNormBlocks);
     _Float16 *p = reinterpret_cast<_Float16 *>(ws + wide_head(batch));
@@ -685,7 +845,8 @@ extern "C" int gatmi_newton_schulz(int64_t batch, int64_t m, int64_t n, const vo
                   "newton_schulz: with a = %g, b = %g, c = %g the iteration can reach %g in %d steps (at most %g): the coefficients do not keep the singular values bounded",
                   a, b, c, worst, steps, kMaxEntry);
     if (batch == 0 || m == 0 || n == 0) return GATMI_OK;
-    GATMI_REQUIRE(x && out && ws, GATMI_EINVAL, "newton_schulz: null pointer");
+    const bool small = ns_is_small(std::min(m, n), std::max(m, n));
+    GATMI_REQUIRE(x && out && (ws || small), GATMI_EINVAL, "newton_schulz: null pointer");
     GATMI_REQUIRE_ALIGNED(ws);
     GATMI_REQUIRE(x_row >= n || m == 1, GATMI_EINVAL, "newton_schulz: row stride %lld below n = %lld", (long long)x_row, (long long)n);
     GATMI_REQUIRE(out_row >= n || m == 1, GATMI_EINVAL, "newton_schulz: row stride %lld of the result below n = %lld", (long long)out_row, (long long)n);
@@ -697,7 +858,8 @@ extern "C" int gatmi_newton_schulz(int64_t batch, int64_t m, int64_t n, const vo
         NsMatrix mat{static_cast<const char *>(x) + b0 * x_batch * size, static_cast<char *>(out) + b0 * out_batch * size, x_batch, x_row, out_batch, out_row, m, n};
         const int64_t now = std::min(kBatchAtOnce, batch - b0);
         int rc;
-#define RUN(T)                                                                                                                                  rc = narrow ? (tall ? run_narrow<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_narrow<T, false>(mat, now, steps, a, b, c, eps, ws, st))                 : (tall ? run_wide<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_wide<T, false>(mat, now, steps, a, b, c, eps, ws, st))
+#define RUN(T)                                                                                                                                  rc = small    ? (tall ? run_small<T, true>(mat, now, steps, a, b, c, eps, st) : run_small<T, false>(mat, now, steps, a, b, c, eps, st))            \
+         : narrow ? (tall ? run_narrow<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_narrow<T, false>(mat, now, steps, a, b, c, eps, ws, st))                   : (tall ? run_wide<T, true>(mat, now, steps, a, b, c, eps, ws, st) : run_wide<T, false>(mat, now, steps, a, b, c, eps, ws, st))
         if (dtype == GATMI_DTYPE_F32) RUN(float);
         else RUN(uint16_t);
 #undef RUN

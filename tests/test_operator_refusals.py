@@ -77,9 +77,9 @@ def test_c_entry_points_refuse_before_any_launch():
     bwd = lambda **k: lib.gatmi_embed_bwd(P, 64, k.get("n", 4), P, k.get("ld", 8), 4, 8, 0, f(1.0), k.get("out", P), k.get("ws", P), None)
     assert bwd(ld=3) == -1 and bwd(out=None) == -1 and bwd(ws=None) == -1 and bwd(ws=P + 4) == -2
 
-    def ns(m=4, n=4, row=4, dt=0, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, x=P, ws=P):
+    def ns(m=4, n=200, row=200, dt=0, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, x=P, ws=P):
         return lib.gatmi_newton_schulz(1, m, n, x, 16, row, dt, steps, a, b, c, eps, P, 16, row, ws, None)
-    assert ns(m=-1) == -1 and ns(row=3) == -1 and ns(dt=3) == -1 and ns(steps=0) == -1 and ns(steps=33) == -1 and ns(eps=0.0) == -1 and ns(x=None) == -1 and ns(ws=P + 8) == -2
+    assert ns(m=-1) == -1 and ns(row=199) == -1 and ns(dt=3) == -1 and ns(steps=0) == -1 and ns(steps=33) == -1 and ns(eps=0.0) == -1 and ns(x=None) == -1 and ns(ws=P + 8) == -2
     assert ns(a=9.0) == -3 and "bounded" in _lib.last_error()
     assert ns(a=float("nan")) == -1 and ns(c=float("inf")) == -1 and ns(eps=float("nan")) == -1
     assert ns(m=2 ** 21, n=100, row=100) == -5

@@ -1,8 +1,8 @@
 """GPU parity of ops.newton_schulz against its 64-bit form, and of the optimizer that calls it.
 
-Bounds.  Shorter side up to 64: formed in fp64, so the result is off by its own rounding (2^-24, bf16 2^-8, relative) and what fp64 rounding becomes after
+Bounds.  Shorter side up to 64 and more than 128 long: formed in fp64, so the result is off by its own rounding (2^-24, bf16 2^-8, relative) and what fp64 rounding becomes after
 five steps: an error in the directions of small singular values grows by a = 3.4445 a step on either side of Q, 485^2 n 2^-53 = 2e-9 of
-the largest entry.  Longer: a step rounds its three products and their operands to 2^-22 or better, about four such errors of the size of X, and a
+the largest entry.  All others: a step rounds its three products and their operands to 2^-22 or better, about four such errors of the size of X, and a
 later step multiplies what falls into small singular directions by a: (a^4 + a^3 + a^2 + a + 1) * 4 * 2^-22 = 2e-4 of |X|_F at the most."""
 import numpy as np
 import pytest
@@ -40,7 +40,7 @@ def _check(x, dtype, steps=5, coefficients=None, what=""):
     last = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -24
     for i, (a, g) in enumerate(zip(flat, gf)):
         ref = attn_ref.newton_schulz(a, steps, **kw)
-        if min(a.shape) <= 64:
+        if min(a.shape) <= 64 and max(a.shape) > 128:
             attn_ref.within(g, ref, last * 1.01 * abs(ref) + 2e-9 * abs(ref).max(), "%s matrix %d" % (what, i))
         else:
             err, norm = np.linalg.norm(g - ref), np.linalg.norm(ref)
@@ -48,7 +48,7 @@ def _check(x, dtype, steps=5, coefficients=None, what=""):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("m,n", [(1, 1), (1, 9), (9, 1), (2, 3), (15, 17), (16, 16), (17, 15), (33, 64), (64, 64), (48, 200), (1433, 8), (8, 1433), (64, 1000),
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 9), (9, 1), (2, 3), (15, 17), (16, 16), (17, 15), (33, 64), (64, 64), (64, 65), (64, 128), (128, 3), (31, 129), (48, 200), (1433, 8), (8, 1433), (64, 1000),
                                  (1000, 63), (5000, 31)])
 def test_narrow_shapes(m, n, dtype):
     _check(_matrices("normal", 3, m, n, seed=m + n), dtype, what="%dx%d" % (m, n))
@@ -61,25 +61,25 @@ def test_wide_shapes(m, n, dtype):
 
 
 @pytest.mark.parametrize("kind", ["low_rank", "rank_one", "one_entry"])
-@pytest.mark.parametrize("m,n", [(20, 30), (64, 64), (1433, 8), (100, 150), (200, 130)])
+@pytest.mark.parametrize("m,n", [(20, 30), (64, 64), (100, 40), (50, 300), (1433, 8), (100, 150), (200, 130)])
 def test_spectra(kind, m, n):
     _check(_matrices(kind, 2, m, n, seed=1), "f32", what="%s %dx%d" % (kind, m, n))
 
 
 @pytest.mark.parametrize("steps,abc", [(1, None), (2, None), (8, (1.5, -0.5, 0.0)), (10, (2.0, -1.5, 0.5)), (3, (3.0, -3.2, 1.2))])
-@pytest.mark.parametrize("m,n", [(30, 20), (70, 90)])
+@pytest.mark.parametrize("m,n", [(30, 20), (30, 220), (70, 90)])
 def test_steps_and_coefficients(m, n, steps, abc):
     _check(_matrices("normal", 2, m, n, seed=2), "f32", steps, abc)
 
 
-@pytest.mark.parametrize("m,n", [(10, 12), (80, 90)])
+@pytest.mark.parametrize("m,n", [(10, 12), (70, 60), (20, 200), (80, 90)])
 @pytest.mark.parametrize("size", [0.0, 1e-30, 1e-12, 1e12, 1e30])
 def test_scale_of_the_input(m, n, size):
     """Zero and tiny inputs stay small (eps), large ones do not overflow: squares are summed in fp64."""
     _check(_matrices("normal", 1, m, n, seed=3) * (size * 1e3), "f32")
 
 
-@pytest.mark.parametrize("m,n", [(10, 12), (80, 90)])
+@pytest.mark.parametrize("m,n", [(10, 12), (20, 200), (80, 90)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_not_finite_input_stays_visible_and_in_its_matrix(m, n, bad):
     from gat_amd import ops
@@ -110,7 +110,7 @@ def test_batches_strides_and_shapes():
         assert ops.newton_schulz(torch.empty(shape, device=dev)).shape == shape
 
 
-@pytest.mark.parametrize("m,n", [(40, 24), (90, 130)])
+@pytest.mark.parametrize("m,n", [(40, 24), (200, 24), (90, 130)])
 def test_streams_and_captured(m, n):
     from gat_amd import graphs, ops
     x = torch.randn((2, m, n), device="cuda:0")
