@@ -11,7 +11,7 @@
 //   2. the sorted tokens are cut into chunks of equal length whatever rows they fall on (a hub's row may own a fifth of all
 //      tokens); a lane group walks a chunk and sums runs of equal ids.  A run inside one chunk is finished there, a run that
 //      crosses a border leaves partial rows.
-//   3. one block per run that crosses borders adds its partial rows; rows that no token hit (a bit per row says so) are
+//   3. the partial rows of each run that crosses borders are added, in order; rows that no token hit (a bit per row says so) are
 //      filled with zeros by the other blocks of the same launch, so that no row of the gradient is written twice.
 #include <hip/hip_runtime.h>
 
@@ -27,7 +27,10 @@ constexpr int kSortRounds = 16;                                   // 64-token ro
 constexpr int kTile = kSortThreads * kSortRounds;                 // tokens of a block
 constexpr int kOneBlock = 4096;                                   // tokens up to which one block sorts in LDS
 constexpr int kOneThreads = 1024;
-constexpr int kChunk = 64;                                        // tokens a lane group sums
+constexpr uint32_t kShortRun = 64;                                // chunks of a run that one lane group adds up
+// Tokens a lane group sums.  16 puts four times as many groups to work, 64 leaves a quarter of the partial rows: both kernels together take 11 (16)
+// and 26 us (64) for 2708 tokens, 21.8 and 21.5 us for 252 thousand, 1074 and 828 us for four million.
+static inline uint32_t embed_chunk(int64_t tokens) { return tokens <= 65536 ? 16 : 64; }
 
 // ---- rows as units: E consecutive elements of T, one load or store ------------------------------------------------
 template <typename T, int E> struct UnitBytes { static constexpr int value = (int)sizeof(T) * E; };
@@ -68,6 +71,20 @@ __device__ __forceinline__ void store_unit(T *p, const float (&v)[E]) {
             *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
         else if constexpr (E == 2) *reinterpret_cast<uint32_t *>(p) = pack_bf16x2(v[0], v[1]);
         else *reinterpret_cast<uint16_t *>(p) = (uint16_t)pack_bf16x2(v[0], 0.f);
+    }
+}
+
+template <int E>
+__device__ __forceinline__ void load_unit_f32(const float *p, float (&v)[E]) {
+    if constexpr (E % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < E; i += 4) {
+            const float4 u = *reinterpret_cast<const float4 *>(p + i);
+            v[i] = u.x; v[i + 1] = u.y; v[i + 2] = u.z; v[i + 3] = u.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = p[i];
     }
 }
 
@@ -322,7 +339,7 @@ struct SegArgs {
     float *partial;                      // [chunks][2][width padded to whole units]
     uint32_t *bits;
     int64_t ld;                          // elements between rows of dout
-    uint32_t n, rows, units, chunks;
+    uint32_t n, rows, units, chunks, chunk;       // chunks of `chunk` tokens
     float scale;
 };
 
@@ -343,7 +360,7 @@ __global__ __launch_bounds__(256) void embed_seg_kernel(SegArgs a) {
     const uint32_t unit = blockIdx.y * L + sub;
     if (chunk >= a.chunks) return;
     const bool active = unit < a.units;
-    const uint32_t c0 = chunk * kChunk, c1 = min(a.n, c0 + kChunk);
+    const uint32_t c0 = chunk * a.chunk, c1 = min(a.n, c0 + a.chunk);
     const T *dout = reinterpret_cast<const T *>(a.dout) + (int64_t)(active ? unit : 0) * E;
     const uint32_t before = c0 > 0 ? a.key[c0 - 1] : 0xffffffffu, after = c1 < a.n ? a.key[c1] : 0xffffffffu;
     float acc[E];
@@ -360,8 +377,13 @@ __global__ __launch_bounds__(256) void embed_seg_kernel(SegArgs a) {
             store_scaled<T, E>(a, cur, unit, acc);
         } else {
             float *p = a.partial + ((size_t)(2 * chunk + (from_before ? 0 : 1)) * a.units + unit) * E;
+            if constexpr (E % 4 == 0) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) p[i] = acc[i];
+                for (int i = 0; i < E; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) p[i] = acc[i];
+            }
         }
     };
     for (uint32_t i0 = c0; i0 < c1; i0 += BATCH) {
@@ -392,69 +414,112 @@ __global__ __launch_bounds__(256) void embed_seg_kernel(SegArgs a) {
     flush(true);
 }
 
-// Blocks [0, join_blocks) look at the chunks in turn; where a run starts in the chunk and goes on behind it, its partial rows are
-// added: G lane groups take consecutive shares, their sums are added in order.  The other blocks fill the rows without
-// a bit with zeros.
+// The first fill_blocks blocks fill the rows without a bit with zeros.  In the others a lane group looks at a chunk: where a run starts in
+// it and goes on behind it, the group adds its partial rows, or, of a run over more than kShortRun chunks, the block does: its groups
+// take consecutive shares, their sums are added in order.
 template <typename T, int E, int L>
 __global__ __launch_bounds__(256) void embed_join_kernel(SegArgs a, uint32_t join_blocks, uint32_t fill_blocks) {
     constexpr int GROUPS = 256 / L;
     __shared__ float sums[GROUPS][L * E];
-    if (blockIdx.x >= join_blocks) {
+    __shared__ uint32_t long_runs, long_list[GROUPS];
+    if (blockIdx.x < fill_blocks) {
         if (blockIdx.y != 0) return;
         const uint32_t words = (a.rows + 31) / 32;
         float zero[E];
 #pragma unroll
         for (int i = 0; i < E; ++i) zero[i] = 0.f;
-        // a wave takes a word of bits, its lanes the units of the rows without one
+        // a wave takes a word of bits: its lanes walk the units of those 32 rows and store where the row has no bit
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        for (uint32_t w = (blockIdx.x - join_blocks) * 4 + wave; w < words; w += fill_blocks * 4) {
-            uint32_t unhit = ~a.bits[w];
-            if (w == words - 1 && (a.rows & 31)) unhit &= (1u << (a.rows & 31)) - 1;
-            while (unhit) {
-                const uint32_t row = w * 32 + (uint32_t)__ffs(unhit) - 1;
-                unhit &= unhit - 1;
-                T *p = reinterpret_cast<T *>(a.dtable) + (int64_t)row * a.units * E;
-                for (uint32_t u = lane; u < a.units; u += 64) store_unit<T, E>(p + (int64_t)u * E, zero);
+        for (uint32_t w = blockIdx.x * 4 + wave; w < words; w += fill_blocks * 4) {
+            const uint32_t hit = a.bits[w];
+            if (hit == 0xffffffffu) continue;
+            const uint32_t count = min(32u, a.rows - w * 32) * a.units;
+            T *p = reinterpret_cast<T *>(a.dtable) + (int64_t)w * 32 * a.units * E;
+            // e / units without a division per unit: the row moves on by 64 / units and a carry
+            uint32_t row = (uint32_t)lane / a.units, in = lane - row * a.units;
+            const uint32_t whole = 64 / a.units, rest = 64 - whole * a.units;
+            for (uint32_t e = lane; e < count; e += 64) {
+                if (!(hit >> row & 1)) store_unit<T, E>(p + (int64_t)e * E, zero);
+                row += whole;
+                in += rest;
+                if (in >= a.units) {
+                    in -= a.units;
+                    ++row;
+                }
             }
         }
         return;
     }
-    for (uint32_t chunk = blockIdx.x; chunk + 1 < a.chunks; chunk += join_blocks) {      // nothing goes on behind the last chunk
-        const uint32_t c0 = chunk * kChunk, c1 = c0 + kChunk;
-        const uint32_t run = a.key[c1 - 1];
-        if (run >= a.rows || a.key[c1] != run) continue;
-        if (a.key[c0] == run && c0 > 0 && a.key[c0 - 1] == run) continue;        // started further ahead: that chunk's block adds it
-        // the last chunk whose first key is the run: keys are sorted, so chunks with that property are consecutive
-        uint32_t lo = chunk + 1, hi = a.chunks - 1;
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
-            if (a.key[mid * (uint32_t)kChunk] == run) lo = mid;
-            else hi = mid - 1;
-        }
-        const uint32_t parts = lo - chunk + 1;
-        const int sub = threadIdx.x % L, group = threadIdx.x / L;
-        const uint32_t unit = blockIdx.y * L + sub;
-        const uint32_t share = (parts + GROUPS - 1) / GROUPS;
-        const uint32_t p0 = min(parts, group * share), p1 = min(parts, p0 + share);
-        float acc[E];
+    const int sub = threadIdx.x % L, group = threadIdx.x / L;
+    const uint32_t unit = blockIdx.y * L + sub;
+    float acc[E];
+    // partial rows [p0, p1) of the run that starts in `chunk`: its first lies in the second place of that chunk, the others in the first
+    // place of theirs
+    auto add = [&](uint32_t chunk, uint32_t p0, uint32_t p1) {
 #pragma unroll
         for (int i = 0; i < E; ++i) acc[i] = 0.f;
-        if (unit < a.units) {
-#pragma unroll 8
-            for (uint32_t p = p0; p < p1; ++p) {
-                const float *src = a.partial + ((size_t)(2 * (chunk + p) + (p == 0 ? 1 : 0)) * a.units + unit) * E;
+        if (unit >= a.units) return;
+        const float *rows = a.partial + ((size_t)(2 * chunk) * a.units + unit) * E;
+        const size_t stride = (size_t)2 * a.units * E;
+        for (uint32_t p = p0; p < p1; p += 8) {
+            float v[8][E];
 #pragma unroll
-                for (int i = 0; i < E; ++i) acc[i] += src[i];
+            for (int u = 0; u < 8; ++u) {
+                const uint32_t at = min(p + u, p1 - 1);
+                load_unit_f32<E>(rows + at * stride + (at == 0 ? stride / 2 : 0), v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (p + u < p1)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) acc[i] += v[u][i];
+        }
+    };
+    for (uint32_t base = (blockIdx.x - fill_blocks) * GROUPS; base < a.chunks; base += join_blocks * GROUPS) {
+        if (threadIdx.x == 0) long_runs = 0;
+        __syncthreads();
+        const uint32_t chunk = base + group;
+        if (chunk + 1 < a.chunks) {                                              // nothing goes on behind the last chunk
+            const uint32_t c0 = chunk * a.chunk, c1 = c0 + a.chunk, run = a.key[c1 - 1];
+            // a run that started further ahead belongs to that chunk's group
+            if (run < a.rows && a.key[c1] == run && !(a.key[c0] == run && c0 > 0 && a.key[c0 - 1] == run)) {
+                uint32_t parts = 2;
+                for (uint32_t more = L; more == L && parts <= kShortRun; parts += more) {        // L chunks at a time: how many begin with the run
+                    const uint32_t at = chunk + parts + sub;
+                    const uint64_t same = __ballot(at < a.chunks && a.key[min(at, a.chunks - 1) * a.chunk] == run) >> (threadIdx.x & 63 & ~(L - 1));
+                    const uint64_t differ = ~same & (L == 64 ? ~0ull : (1ull << (L & 63)) - 1);
+                    more = differ ? (uint32_t)__ffsll((unsigned long long)differ) - 1 : L;
+                }
+                if (parts <= kShortRun) {
+                    add(chunk, 0, parts);
+                    if (unit < a.units) store_scaled<T, E>(a, run, unit, acc);
+                } else if (sub == 0) {
+                    long_list[atomicAdd(&long_runs, 1u)] = chunk;
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i) sums[group][sub * E + i] = acc[i];
         __syncthreads();
-        if (group == 0 && unit < a.units) {
-            for (int g = 1; g < GROUPS; ++g)
+        for (uint32_t k = 0; k < long_runs; ++k) {                               // the whole block adds each of the long ones
+            const uint32_t first = long_list[k], run = a.key[first * a.chunk + a.chunk - 1];
+            // the last chunk whose first key is the run: keys are sorted, so chunks with that property are consecutive
+            uint32_t lo = first + 1, hi = a.chunks - 1;
+            while (lo < hi) {
+                const uint32_t mid = lo + (hi - lo + 1) / 2;
+                if (a.key[mid * a.chunk] == run) lo = mid;
+                else hi = mid - 1;
+            }
+            const uint32_t parts = lo - first + 1, share = (parts + GROUPS - 1) / GROUPS;
+            add(first, min(parts, group * share), min(parts, (group + 1) * share));
 #pragma unroll
-                for (int i = 0; i < E; ++i) acc[i] += sums[g][sub * E + i];
-            store_scaled<T, E>(a, run, unit, acc);
+            for (int i = 0; i < E; ++i) sums[group][sub * E + i] = acc[i];
+            __syncthreads();
+            if (group == 0 && unit < a.units) {
+                for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) acc[i] += sums[g][sub * E + i];
+                store_scaled<T, E>(a, run, unit, acc);
+            }
+            __syncthreads();
         }
         __syncthreads();
     }
@@ -531,7 +596,7 @@ static void embed_bwd_layout(int64_t tokens, int64_t rows, int32_t width, size_t
     *hist = 4 * n4;
     *bits = *hist + 256 * blocks + 256;
     *partial = (*bits + ((size_t)rows + 31) / 32 + 3) / 4 * 4;
-    *total = *partial + 2 * (((size_t)tokens + kChunk - 1) / kChunk) * (size_t)width;
+    *total = *partial + 2 * (((size_t)tokens + embed_chunk(tokens) - 1) / embed_chunk(tokens)) * (size_t)width;
 }
 
 extern "C" size_t gatmi_embed_bwd_ws_floats(int64_t tokens, int64_t rows, int32_t width) {
@@ -596,12 +661,12 @@ extern "C" int gatmi_embed_bwd(const void *ids, int32_t id_bits, int64_t tokens,
     const int E = unit_elems(width, dtype, ld_dout, dout, dtable);
     SegArgs a;
     a.key = keys[at]; a.pos = poss[at]; a.dout = dout; a.dtable = dtable; a.partial = ws + partial; a.bits = s.bits;
-    a.ld = ld_dout; a.n = s.n; a.rows = s.rows; a.units = (uint32_t)(width / E); a.chunks = (s.n + kChunk - 1) / kChunk; a.scale = scale;
+    a.ld = ld_dout; a.n = s.n; a.rows = s.rows; a.units = (uint32_t)(width / E); a.chunk = embed_chunk(tokens); a.chunks = (s.n + a.chunk - 1) / a.chunk; a.scale = scale;
     int L = 4;
     while (L < 64 && (uint32_t)L < a.units) L *= 2;
     const unsigned slices = (a.units + L - 1) / L;
-    const uint32_t joins = std::min<uint32_t>(a.chunks, 1 << 14);
-    const uint32_t fill = (uint32_t)std::min<int64_t>(2048, (s.bit_words + 3) / 4);
+    const uint32_t joins = std::min<uint32_t>((a.chunks + 256 / L - 1) / (256 / L), 1 << 14);
+    const uint32_t fill = (uint32_t)std::min<int64_t>(1024, (s.bit_words + 3) / 4);
 #define SEG(T, e, l)                                                                                                                          \
     do {                                                                                                                                      \
         hipLaunchKernelGGL((embed_seg_kernel<T, e, l>), dim3((a.chunks + 256 / l - 1) / (256 / l), slices), dim3(256), 0, st, a);             \

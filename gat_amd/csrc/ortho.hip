@@ -34,7 +34,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNarrow = 64;
-constexpr int kNarrowThreads = 512;          // of the polynomial kernel
 constexpr int kGramParts = 256;              // partial sums of G per matrix, at most
 constexpr int kMaxSteps = 32;
 constexpr int64_t kBatchAtOnce = 32768;      // matrices of one set of launches (grid.y, grid.z)
@@ -122,7 +121,8 @@ __global__ __launch_bounds__(64) void ns_gram_kernel(NarrowArgs a) {
 // until every wave has read its operands.
 template <int TILES>
 struct NsProduct {
-    static constexpr int NP = 16 * TILES, LD = NP + 2, COUNT = TILES * (TILES + 1) / 2, WAVES = kNarrowThreads / 64, PER = (COUNT + WAVES - 1) / WAVES;
+    static constexpr int NP = 16 * TILES, LD = NP + 2, COUNT = TILES * (TILES + 1) / 2, WAVES = TILES <= 2 ? 4 : 8, THREADS = 64 * WAVES;
+    static constexpr int PER = (COUNT + WAVES - 1) / WAVES;
     f64x4 acc[PER];
     __device__ static void tile(int t, int &p, int &q) {
         p = 0;
@@ -174,17 +174,17 @@ struct NsProduct {
 // Q of one matrix per block: P_k = a I + b A_k + c A_k^2, Q = P_0 P_1 ..., A_{k+1} = A_k P_k^2, from A_0 = G / (|x|_F + eps)^2.
 // The scale of x goes into Q.
 template <int TILES>
-__global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
+__global__ __launch_bounds__(NsProduct<TILES>::THREADS) void ns_poly_kernel(NarrowArgs a) {
     using Product = NsProduct<TILES>;
-    constexpr int NP = Product::NP, LD = Product::LD;
+    constexpr int NP = Product::NP, LD = Product::LD, THREADS = Product::THREADS;
     extern __shared__ double lds[];
     double *A = lds, *P = A + NP * LD, *Q = P + NP * LD;
     const double *g = a.gram + (size_t)blockIdx.x * a.parts * (NP * NP);
-    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) {
+    for (int e = threadIdx.x; e < NP * NP; e += THREADS) {
         const int row = e / NP, col = e % NP;
         const int up = row / 16 <= col / 16 ? e : col * NP + row;          // tiles below the diagonal are not formed
         double s = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int p = 0; p < a.parts; ++p) s += g[(size_t)p * (NP * NP) + up];
         A[row * LD + col] = s;
     }
@@ -194,9 +194,9 @@ __global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
     for (int d = 0; d < NP; ++d) trace += A[d * LD + d];              // zeros behind n
     const double inv = 1.0 / (sqrt(trace) + a.eps);
     __syncthreads();
-    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) A[e / NP * LD + e % NP] *= inv * inv;
+    for (int e = threadIdx.x; e < NP * NP; e += THREADS) A[e / NP * LD + e % NP] *= inv * inv;
     if (a.steps == 0)
-        for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) Q[e / NP * LD + e % NP] = e / NP == e % NP ? 1.0 : 0.0;
+        for (int e = threadIdx.x; e < NP * NP; e += THREADS) Q[e / NP * LD + e % NP] = e / NP == e % NP ? 1.0 : 0.0;
     __syncthreads();
     Product pr;
     for (int step = 0; step < a.steps; ++step) {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
         pr.store(P, a.cc, a.cb, A, a.ca);
         __syncthreads();
         if (step == 0) {
-            for (int e = threadIdx.x; e < NP * LD; e += kNarrowThreads) Q[e] = P[e];
+            for (int e = threadIdx.x; e < NP * LD; e += THREADS) Q[e] = P[e];
         } else {
             pr.multiply(Q, P);
             __syncthreads();
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kNarrowThreads) void ns_poly_kernel(NarrowArgs a) {
         __syncthreads();
     }
     double *q = a.q + (size_t)blockIdx.x * (NP * NP);
-    for (int e = threadIdx.x; e < NP * NP; e += kNarrowThreads) q[e] = Q[e / NP * LD + e % NP] * inv;
+    for (int e = threadIdx.x; e < NP * NP; e += THREADS) q[e] = Q[e / NP * LD + e % NP] * inv;
 }
 
 // out = X Q, 16 places of the long side per wave
@@ -677,7 +677,7 @@ static int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; 
 
 static int gram_parts(int64_t batch, int64_t len) {
     const int64_t per_matrix = std::max<int64_t>(1, 512 / std::max<int64_t>(1, batch));
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kGramParts, per_matrix), (len + 127) / 128));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kGramParts, per_matrix), (len + 63) / 64));
 }
 
 // Largest entry that X, X X^T or the polynomial can reach: |X|_2 <= s with s_0 = 1 and s_{k+1} = max over t in [0, s_k] of
@@ -747,7 +747,7 @@ static int run_narrow(const NsMatrix &mat, int64_t batch, int steps, double ca, 
         hipLaunchKernelGGL((ns_gram_kernel<T, TALL, t>), dim3(a.parts, (unsigned)batch), dim3(64), 0, st, a);                               \
         if (3 * one > 48 * 1024) e = hipFuncSetAttribute(reinterpret_cast<const void *>(&ns_poly_kernel<t>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * one)); \
         if (e != hipSuccess) return fail(GATMI_EHIP, "newton_schulz: %s", hipGetErrorString(e));                                            \
-        hipLaunchKernelGGL((ns_poly_kernel<t>), dim3((unsigned)batch), dim3(kNarrowThreads), 3 * one, st, a);                               \
+        hipLaunchKernelGGL((ns_poly_kernel<t>), dim3((unsigned)batch), dim3(NsProduct<t>::THREADS), 3 * one, st, a);                               \
         hipLaunchKernelGGL((ns_apply_kernel<T, TALL, t>), dim3(apply, (unsigned)batch), dim3(256), one, st, a);                             \
     }
     RUN(1) RUN(2) RUN(3) RUN(4)
