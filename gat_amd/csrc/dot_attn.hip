@@ -183,7 +183,7 @@ __device__ __forceinline__ Frag<T> frag_row(const char *tile, int row0, int c) {
     return frag_load<T, DP>(tile + S::at(row0 + (lane & 15), c * 4 * S::PIECE + (lane >> 4) * S::PIECE));
 }
 
-// how a kernel gets the mask: there is none; as floats (single rows, and columns that shared heads walk); as bits
+// how a kernel gets the mask: there is none; as floats (the few rows of KEYW); as bits
 constexpr int kNoMask = 0, kFloats = 1, kBits = 2;
 
 // ---- arguments ---------------------------------------------------------------------------------------------------------
@@ -242,29 +242,72 @@ __device__ __forceinline__ DotBlock dot_block(const DotArgs &a) {
     return r;
 }
 
-// ---- staging: KT rows of two tensors, straight from memory to LDS by WAVES waves --------------------------------------------
-// Rows behind the last one and pieces behind D are replaced by ones that exist: what is computed from them is masked, multiplied
-// by zeros of the other operand, or not stored.  row(x, r): element offset of row r (r < count).
-template <typename T, int DP, int KT, int WAVES, typename Row>
-__device__ __forceinline__ void stage(char *lds, const DotRows &x, const DotRows &y, int count, int D, int wave, Row &&row) {
+// ---- staging: tiles of KT rows of two tensors, straight from memory to LDS by WAVES waves ------------------------------------
+// A load is 1 KB: 64 / CPR rows.  Loads whose rows are a multiple of 16 apart share the permutation of their pieces, hence an address that
+// differs by whole rows: a wave keeps one address per tensor for each of BASES such sets and moves them on from tile to tile.
+// Only the last tile looks at every row: rows behind the last one are replaced by it (what is computed from them is masked or not
+// stored; memory behind a graph's own rows is not read).  Pieces behind D are replaced by the row's first: the other operand has zeros there.
+template <typename T, int DP, int KT, int WAVES>
+struct Stager {
     using S = Shape<T, DP>;
-    constexpr int LOADS = KT * S::ROW / 1024, TOTAL = 2 * LOADS;
-    const int lane = threadIdx.x & 63;
+    static constexpr int ROWS = 64 / S::CPR, LOADS = KT / ROWS;             // of a load; of one tensor's tile
+    static constexpr bool APART = LOADS < WAVES;                            // a wave has loads of one tensor only
+    static constexpr int LANES = APART ? WAVES / 2 : WAVES;                 // waves that share a tensor's loads
+    static constexpr int OWN = LOADS / LANES;                               // loads of a wave and tensor: rows (u * LANES + w) * ROWS ..
+    static constexpr int BASES = LANES * ROWS >= 16 ? 1 : 16 / (LANES * ROWS), APARTS = OWN / BASES;
+    static_assert(LOADS % LANES == 0 && OWN % BASES == 0 && (LANES * ROWS >= 16 ? LANES * ROWS % 16 == 0 : 16 % (LANES * ROWS) == 0), "loads do not divide");
+    const char *base[2][BASES];
+    int64_t node[2];                                                        // bytes
+    int w, tensor;                                                          // this wave's place, and its tensor if APART
+    __device__ __forceinline__ int row_of(int set, int lane) const { return (set * LANES + w) * ROWS + lane / S::CPR; }
+    __device__ __forceinline__ int byte_of(int r, int lane, int D) const {
+        const int c = (lane % S::CPR) ^ S::swizzle(r);
+        return c * (16 / S::SIZE) < D ? c * 16 : 0;
+    }
+    // x0, y0: element offsets of the first row
+    __device__ __forceinline__ void init(const DotRows &x, const DotRows &y, int64_t x0, int64_t y0, int D, int wave) {
+        const int lane = threadIdx.x & 63;
+        w = wave % LANES;
+        tensor = wave / LANES;
+        node[0] = x.node * S::SIZE;
+        node[1] = y.node * S::SIZE;
 #pragma unroll
-    for (int u = 0; u < (TOTAL + WAVES - 1) / WAVES; ++u) {
-        const int load = u * WAVES + wave;                                  // the same for the whole wave
-        if (TOTAL % WAVES == 0 || load < TOTAL) {
-            const bool second = load >= LOADS;
-            const DotRows &z = second ? y : x;
-            const int piece = (load - (second ? LOADS : 0)) * 64 + lane, r = piece / S::CPR;
-            int c = (piece % S::CPR) ^ S::swizzle(r);
-            c = c * (16 / S::SIZE) < D ? c : 0;
-            const T *src = reinterpret_cast<const T *>(z.p) + row(z, min(r, count - 1)) + c * (16 / S::SIZE);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                             (__attribute__((address_space(3))) void *)(lds + load * 1024), 16, 0, 0);
+        for (int s = 0; s < BASES; ++s) {
+            const int r = row_of(s, lane), byte = byte_of(r, lane, D);
+            base[0][s] = reinterpret_cast<const char *>(x.p) + x0 * S::SIZE + r * node[0] + byte;
+            base[1][s] = reinterpret_cast<const char *>(y.p) + y0 * S::SIZE + r * node[1] + byte;
         }
     }
-}
+    __device__ __forceinline__ void move(int64_t bx, int64_t by) {
+#pragma unroll
+        for (int s = 0; s < BASES; ++s) {
+            base[0][s] += bx;
+            base[1][s] += by;
+        }
+    }
+    // the tile at the present place, `count` rows of it, into lds (the first tensor's, then the second's); then on to the next
+    __device__ __forceinline__ void load(char *lds, int count) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            if (APART && z != tensor) continue;
+#pragma unroll
+            for (int s = 0; s < BASES; ++s)
+#pragma unroll
+                for (int u = 0; u < APARTS; ++u) {
+                    const int set = u * BASES + s, apart = u * BASES * LANES * ROWS;        // rows from this set's base
+                    const char *src = base[z][s] + apart * node[z];
+                    if (count < KT) {
+                        const int r = row_of(set, lane);
+                        src -= max(0, r - (count - 1)) * node[z];
+                    }
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                                     (__attribute__((address_space(3))) void *)(lds + (z * LOADS + set * LANES + w) * 1024), 16, 0, 0);
+                }
+        }
+        move(KT * node[0], KT * node[1]);
+    }
+};
 // what this wave (BLOCK: every wave) has asked for is in LDS; nobody reads the other buffer any more
 template <bool BLOCK>
 __device__ __forceinline__ void arrived() {
@@ -332,10 +375,6 @@ __device__ __forceinline__ f32x4 bias4(const float *row, int j, int nk) {
     }
     return v;
 }
-__device__ __forceinline__ bool some_attended(f32x4 bias) {
-    return __ballot(fmaxf(fmaxf(bias[0], bias[1]), fmaxf(bias[2], bias[3])) > kAttended) != 0;
-}
-
 // The mask of one lane's row over a tile of KT keys.  In a lane only the bits of its own keys (16 t + 4 q .. + 3) count.
 template <int MASK, int KT>
 struct RowMask {
@@ -454,12 +493,13 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    const int64_t kb = b * a.k.batch + blk.hk * a.k.head, vb = b * a.v.batch + blk.hk * a.v.head;
-    auto fetch = [&](char *to, int j) {
-        stage<T, DP, KT, KEYW ? 1 : 4>(to, a.k, a.v, j1 - j, a.D, KEYW ? 0 : wave,
-                                   [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
-    };
     int j = j0 + (KEYW ? wave * KT : 0), at = 0;
+    Stager<T, DP, KT, KEYW ? 1 : 4> rows;
+    rows.init(a.k, a.v, b * a.k.batch + blk.hk * a.k.head + j * a.k.node, b * a.v.batch + blk.hk * a.v.head + j * a.v.node, a.D, KEYW ? 0 : wave);
+    auto fetch = [&](char *to, int from) {
+        rows.load(to, j1 - from);
+        if constexpr (KEYW) rows.move((STEP - KT) * rows.node[0], (STEP - KT) * rows.node[1]);
+    };
     if (j < j1) {
         fetch(buf(0), j);
 #pragma unroll
@@ -729,10 +769,9 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
     const int64_t b = blk.b;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
     auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
-    const int64_t kb = b * a.k.batch + blk.hk * a.k.head, vb = b * a.v.batch + blk.hk * a.v.head;
-    auto fetch = [&](char *to, int j) {
-        stage<T, DP, KT, 4>(to, a.k, a.v, keys - j, a.D, wave, [&](const DotRows &x, int r) { return (&x == &a.k ? kb : vb) + (int64_t)(j + r) * x.node; });
-    };
+    Stager<T, DP, KT, 4> rows;
+    rows.init(a.k, a.v, b * a.k.batch + blk.hk * a.k.head, b * a.v.batch + blk.hk * a.v.head, a.D, wave);
+    auto fetch = [&](char *to, int from) { rows.load(to, keys - from); };
     if (keys > 0) fetch(buf(0), 0);
     int qi[NQ], head[NQ];
     float lse[NQ], delta[NQ];
@@ -879,38 +918,44 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 }
 
 // ---- backward: dk and dv -----------------------------------------------------------------------------------------------------
-// A wave owns NK x 16 keys (one per lane of a row of 16) and walks all rows of the sharing heads.  Rows behind the last one come with
-// lse = inf: their probabilities are zero.
+// A wave owns NK x 16 keys (one per lane of a row of 16) and walks the queries of each sharing head in turn.  Rows behind the last
+// one come with lse = inf: their probabilities are zero.
 template <typename T, int DP, int NK, int MASK>
 __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_bwd_kv_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int QT = S::KT, DT = S::DT, KEYS = 64 * NK, PER = S::CHUNK / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
-    __shared__ const float *bias_rows[2][MASK ? QT : 1];
     const DotBlock blk = dot_block<MASK>(a);
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
-    const int rows = queries * a.group;
     auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
-    auto fetch = [&](int to, int r0) {
-        stage<T, DP, QT, 4>(buf(to), a.q, a.d_o, rows - r0, a.D, wave, [&](const DotRows &x, int r) {
-            const int row = r0 + r, i = row / a.group;
-            return b * x.batch + (int64_t)i * x.node + (blk.hk * a.group + row - i * a.group) * x.head;
-        });
+    const int head0 = blk.hk * a.group;
+    Stager<T, DP, QT, 4> rows;
+    rows.init(a.q, a.d_o, b * a.q.batch + head0 * a.q.head, b * a.d_o.batch + head0 * a.d_o.head, a.D, wave);
+    const int tiles = (queries + QT - 1) / QT;
+    // of the tile that is fetched next: its head in the group and its first query
+    int next_head = 0, next_i = 0;
+    auto fetch = [&](int to) {
+        rows.load(buf(to), queries - next_i);
         if (threadIdx.x < QT) {
-            const int row = min(r0 + (int)threadIdx.x, rows - 1), i = row / a.group;
-            const int64_t at = (b * a.H + blk.hk * a.group + row - i * a.group) * a.Nq + i;
-            lses[to][threadIdx.x] = r0 + (int)threadIdx.x < rows ? a.lse[at] : INFINITY;
+            const int i = next_i + (int)threadIdx.x;
+            const int64_t at = (b * a.H + head0 + next_head) * a.Nq + min(i, queries - 1);
+            lses[to][threadIdx.x] = i < queries ? a.lse[at] : INFINITY;
             deltas[to][threadIdx.x] = a.delta[at];
-            if constexpr (MASK != kNoMask) bias_rows[to][threadIdx.x] = a.bias + b * a.bias_batch + i * a.bias_row;
+        }
+        next_i += QT;
+        if (next_i >= queries) {                      // on to the next head: back to its first row
+            rows.move(a.q.head * S::SIZE - (int64_t)tiles * QT * rows.node[0], a.d_o.head * S::SIZE - (int64_t)tiles * QT * rows.node[1]);
+            next_i = 0;
+            ++next_head;
         }
     };
-    if (rows > 0) fetch(0, 0);
+    if (queries > 0) fetch(0);
     int key[NK], col[NK];
-    const ulonglong2 *words[NK];          // the mask of this lane's key over the queries (kBits: rows are queries, the heads are not shared)
+    const ulonglong2 *words[NK];          // the mask of this lane's key over the queries
     ulonglong2 next[NK];
     Frag<T> kf[NK][S::FRAGS], vf[NK][S::FRAGS];
     f32x4 dk[NK][DT], dv[NK][DT];
@@ -927,29 +972,31 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
         }
         if constexpr (MASK == kBits) {
             words[u] = a.col_words + b * a.col_words_batch + (int64_t)col[u] * ((a.Nq + 63) / 64);
-            if (rows > 0) next[u] = words[u][0];
+            if (queries > 0) next[u] = words[u][0];
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[u][t] = dv[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
-    for (int r0 = 0, at = 0; r0 < rows; r0 += QT, at ^= 1) {
+    for (int it = 0, i0 = 0, at = 0; it < tiles * a.group; ++it, at ^= 1) {
         arrived<true>();
         const char *qs = buf(at), *ds = qs + S::TILE;
-        if (r0 + QT < rows) fetch(at ^ 1, r0 + QT);
+        if (it + 1 < tiles * a.group) fetch(at ^ 1);
         uint32_t lo[NK], hi[NK];
         bool soft[NK];
+        const int here0 = i0;                         // the tile's first query
+        i0 = i0 + QT >= queries ? 0 : i0 + QT;
 #pragma unroll
         for (int u = 0; u < NK; ++u) {
-            soft[u] = MASK == kFloats;
+            soft[u] = false;
             if constexpr (MASK == kBits) {
-                const uint64_t w = next[u].x >> (r0 & 63);
-                soft[u] = __ballot(next[u].y >> (r0 & 63) != 0) != 0;
+                const uint64_t w = next[u].x >> (here0 & 63);
+                soft[u] = __ballot(next[u].y >> (here0 & 63) != 0) != 0;
                 lo[u] = (uint32_t)(w >> (4 * q4));
                 hi[u] = (uint32_t)(w >> (4 * q4) >> 32);
-                if (r0 + QT < rows) next[u] = words[u][(r0 + QT) >> 6];
+                next[u] = words[u][i0 >> 6];
             }
         }
-        bool has[NK][QT / 16], full = MASK != kFloats;
+        bool has[NK][QT / 16], full = true;
 #pragma unroll
         for (int u = 0; u < NK; ++u)
 #pragma unroll
@@ -974,13 +1021,12 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                     for (int u = 0; u < NK; ++u) {
                         z[u][t] = dp[u] = p[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
                         some[u] = has[u][s0 / 16];
-                        if constexpr (MASK != kNoMask) {
+                        if constexpr (MASK == kBits) {
                             if (soft[u]) {
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) bias[u][r] = bias_rows[at][s0 + 4 * q4 + r][col[u]];
+                                for (int r = 0; r < 4; ++r) bias[u][r] = a.bias[b * a.bias_batch + (int64_t)min(here0 + s0 + 4 * q4 + r, queries - 1) * a.bias_row + col[u]];
                             }
                         }
-                        if constexpr (MASK == kFloats) some[u] = some_attended(bias[u]);
                         use[u] |= some[u];
                         here |= some[u];
                     }
@@ -1003,17 +1049,14 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                     for (int u = 0; u < NK; ++u)
                         if (!SKIP || some[u]) {
                             float factor = a.scale2;
-                            if constexpr (MASK != kNoMask) {
+                            if constexpr (MASK == kBits) {
                                 if (soft[u]) {
                                     factor = 1.f;
 #pragma unroll
                                     for (int r = 0; r < 4; ++r) z[u][t][r] = fmaf(z[u][t][r], a.scale2, bias[u][r] * kLog2e);
                                 }
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    if constexpr (MASK == kBits) z[u][t][r] = where_bit(s0 < 32 ? lo[u] : hi[u], (s0 & 31) + r, z[u][t][r]);
-                                    else z[u][t][r] = bias[u][r] > kAttended ? z[u][t][r] : -INFINITY;
-                                }
+                                for (int r = 0; r < 4; ++r) z[u][t][r] = where_bit(s0 < 32 ? lo[u] : hi[u], (s0 & 31) + r, z[u][t][r]);
                             }
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
@@ -1259,7 +1302,7 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
             int rc;
 #define RUN(kernel, n, mask) dot_launch("dot_attn_bwd", kernel<T, DP, n, mask>, a, 4 * S::TILE, st)
 #define RUN_Q(n) (a.bias ? RUN(dot_bwd_q_kernel, n, kBits) : RUN(dot_bwd_q_kernel, n, kNoMask))
-#define RUN_KV(n) (a.bias ? (a.group == 1 ? RUN(dot_bwd_kv_kernel, n, kBits) : RUN(dot_bwd_kv_kernel, n, kFloats)) : RUN(dot_bwd_kv_kernel, n, kNoMask))
+#define RUN_KV(n) (a.bias ? RUN(dot_bwd_kv_kernel, n, kBits) : RUN(dot_bwd_kv_kernel, n, kNoMask))
             if (pass == 0) rc = wide ? RUN_Q(S::NQ) : RUN_Q(1);
             else rc = wide ? RUN_KV(S::NK) : RUN_KV(1);
 #undef RUN_KV
