@@ -53,7 +53,8 @@ template <typename T, int DP> struct Shape {
     static constexpr int KTW = ROW >= 512 ? 16 : (ROW >= 128 ? 32 : 64);               // where each wave stages tiles of its own
     static constexpr int TILE = KT * ROW;
     // 16-row tiles of a wave: two where the accumulators and operands of two fit the 256 registers that leave two waves on a SIMD
-    static constexpr int NQ = SIZE == 4 && DP >= 64 ? 1 : 2, NK = ROW >= 256 ? 1 : 2;
+    static constexpr int NQ = SIZE == 4 && DP >= 64 ? 1 : 2;
+    static constexpr int nk(bool masked) { return (SIZE == 4 && DP >= 64) || (DP == 128 && masked) ? 1 : 2; }
     __device__ static __forceinline__ int swizzle(int r) {      // the same for r and r + 16
         if constexpr (CPR >= 16) return r & 15;
         else return (r / (16 / CPR)) & (CPR - 1);
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
     float sum[NQ];
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
-        if constexpr (ONES) sum[u] = __shfl(o[u][0][0], 32 + n, 64);                   // row 8 of the transposed result
+        if constexpr (ONES) sum[u] = __shfl(o[u][0][0], 32 + n, 64);              // row 8 of the transposed result
         else sum[u] = over_groups_sum(l[u]);
     }
     if constexpr (KEYW) {                                                            // NQ = 1: join the four waves
@@ -1293,7 +1294,7 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
         const int64_t count = pass == 0 ? rows : a.Nk;
         if (count == 0) continue;
         const bool wide = count > 64;
-        const int per = 64 * (wide ? (pass == 0 ? S::NQ : S::NK) : 1);
+        const int per = 64 * (wide ? (pass == 0 ? S::NQ : S::nk(a.bias != nullptr)) : 1);
         a.tiles = (int)((count + per - 1) / per);
         const int64_t step = dot_graphs(a);
         for (int64_t b0 = 0; b0 < B; b0 += step) {
@@ -1304,7 +1305,7 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
 #define RUN_Q(n) (a.bias ? RUN(dot_bwd_q_kernel, n, kBits) : RUN(dot_bwd_q_kernel, n, kNoMask))
 #define RUN_KV(n) (a.bias ? RUN(dot_bwd_kv_kernel, n, kBits) : RUN(dot_bwd_kv_kernel, n, kNoMask))
             if (pass == 0) rc = wide ? RUN_Q(S::NQ) : RUN_Q(1);
-            else rc = wide ? RUN_KV(S::NK) : RUN_KV(1);
+            else rc = !wide ? RUN_KV(1) : (a.bias ? RUN(dot_bwd_kv_kernel, S::nk(true), kBits) : RUN(dot_bwd_kv_kernel, S::nk(false), kNoMask));
 #undef RUN_KV
 #undef RUN_Q
 #undef RUN
