@@ -17,6 +17,11 @@
 // across the lanes): a lane then holds four consecutive keys of ONE query, the softmax statistics are one register each,
 // and the probabilities sit in the operand layout of the second product as they are: they never go through LDS.  bf16 rounds P and
 // dz to bf16 for that product (half a step of 2^-8, as its other operand has and its result is stored with).
+//
+// fp32 rows are computed in one of two ways.  A few rows: on v_mfma_f32_16x16x4_f32 (256 flop / clock / CU, which the vector units cannot use
+// meanwhile).  Otherwise (Split3): every number x is split exactly into three bf16, h + m + l with 8 bits each, and a product is the six
+// terms hh + hm + mh + mm + hl + lh on the bf16 instructions (16 times the rate, beside the vector units; what is left out is below 2^-23
+// of the product).  q, k, v and dout are split once into rows of three parts, probabilities and dz in registers.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -35,6 +40,15 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 struct __attribute__((packed, aligned(4))) f32x4_u { float v[4]; };       // a 16-byte access at 4-byte alignment
 
 constexpr float kAttended = -1e8f;
+// two numbers as h + m + l, bf16 each (exact: what is left of 24 bits after two roundings to 8 has 8 at most), packed pairwise
+__device__ __forceinline__ void split3_pack(float a, float b, uint32_t &h, uint32_t &m, uint32_t &l) {
+    h = pack_bf16x2(a, b);
+    a -= __uint_as_float(h << 16);
+    b -= __uint_as_float(h & 0xffff0000u);
+    m = pack_bf16x2(a, b);
+    l = pack_bf16x2(a - __uint_as_float(m << 16), b - __uint_as_float(m & 0xffff0000u));
+}
+
 constexpr int kSplitsMax = 256;
 
 // ---- rows in LDS and operand fragments -----------------------------------------------------------------------------------
@@ -43,15 +57,22 @@ constexpr int kSplitsMax = 256;
 // one LDS read, which want the same piece of many rows, find them in different banks.
 // A fragment is what a lane holds of 16 rows x KD elements: lane (n = l & 15, q = l >> 4) the PIECE bytes at q * PIECE of the
 // fragment's part of row n.
+struct Split3 {};                                        // fp32 as three bf16
+template <typename T> struct ElemOf { using type = T; };
+template <> struct ElemOf<Split3> { using type = float; };
+template <typename T> using Elem = typename ElemOf<T>::type;              // what results are stored as
+template <typename T> constexpr bool kSplit = std::is_same_v<T, Split3>;
+
 template <typename T, int DP> struct Shape {
+    static constexpr int PLANES = 1;
     static constexpr int SIZE = (int)sizeof(T), ROW = DP * SIZE, CPR = ROW / 16;         // bytes and 16-byte pieces of a row
     static constexpr bool NARROW = ROW == 32;                                              // one fragment of 8 bytes a lane
-    static constexpr int PIECE = NARROW ? 8 : 16, FRAGS = ROW / (4 * PIECE), ELEMS = PIECE / SIZE, KD = 4 * ELEMS;
+    static constexpr int PIECE = NARROW ? 8 : 16, FRAGS = ROW / (4 * PIECE), ELEMS = PIECE / SIZE, KD = 4 * ELEMS, GROUPS = FRAGS;
     static constexpr int CHUNK = SIZE == 4 ? 16 : 32;                                      // rows that one fragment of the second product covers
     static constexpr int KT = (SIZE == 4 && DP == 128) ? 32 : 64;                         // rows of a staged tile
     static constexpr int DT = (DP + 15) / 16;                                            // 16-wide tiles of a result row
     static constexpr int KTW = ROW >= 512 ? 16 : (ROW >= 128 ? 32 : 64);               // where each wave stages tiles of its own
-    static constexpr int TILE = KT * ROW;
+    static constexpr int PLANE = KT * ROW, TILE = PLANE;
     // 16-row tiles of a wave: two where the accumulators and operands of two fit the 256 registers that leave two waves on a SIMD
     static constexpr int NQ = SIZE == 4 && DP >= 64 ? 1 : 2;
     static constexpr int nk(bool masked) { return (SIZE == 4 && DP >= 64) || (DP == 128 && masked) ? 1 : 2; }
@@ -62,16 +83,28 @@ template <typename T, int DP> struct Shape {
     __device__ static __forceinline__ int at(int r, int byte) { return r * ROW + (((byte >> 4) ^ swizzle(r)) << 4) + (byte & 15); }
 };
 
+// Rows of three parts: planes of their own (h of the whole row, then m, then l), and the six terms are six instructions over the same fragments.
+template <int DP> struct Shape<Split3, DP> : Shape<uint16_t, DP> {
+    using H = Shape<uint16_t, DP>;
+    static constexpr int PLANES = 3, COLS = 3 * DP, FRAGS = 3 * H::GROUPS, KT = DP >= 64 ? 32 : 64, PLANE = KT * H::ROW, TILE = 3 * PLANE;
+    static constexpr int NQ = 2;
+    static constexpr int nk(bool masked) { return DP == 32 || (DP == 128 && !masked) ? 2 : 1; }
+};
+
 struct FragF { float v[4]; };
 struct FragH { uint4 v; };
 template <typename T> struct FragOf;
 template <> struct FragOf<float> { using type = FragF; };
 template <> struct FragOf<uint16_t> { using type = FragH; };
+template <> struct FragOf<Split3> { using type = FragH; };
 template <typename T> using Frag = typename FragOf<T>::type;
+// operands of the second product: one fragment, or one of each part
+template <typename T> struct ManyOf { Frag<T> p[1]; };
+template <> struct ManyOf<Split3> { FragH p[3]; };
 
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> frag_load(const char *p) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (std::is_same_v<T, float>) {
         if constexpr (Shape<T, DP>::NARROW) {
             const float2 u = *reinterpret_cast<const float2 *>(p);
             return FragF{{u.x, u.y, 0.f, 0.f}};
@@ -90,26 +123,32 @@ __device__ __forceinline__ Frag<T> frag_load(const char *p) {
 }
 // the fragments of one row in memory: zeros behind its D elements and where there is no row
 template <typename T, int DP>
-__device__ __forceinline__ void row_frags(const T *row, int D, bool ok, Frag<T> (&f)[Shape<T, DP>::FRAGS]) {
+__device__ __forceinline__ void row_frags(const char *row, int D, bool ok, Frag<T> (&f)[Shape<T, DP>::FRAGS]) {
     using S = Shape<T, DP>;
     const int q = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int c = 0; c < S::FRAGS; ++c) {
-        const int e = c * S::KD + q * S::ELEMS;
-        if (ok && e < D) f[c] = frag_load<T, DP>(reinterpret_cast<const char *>(row + e));
-        else f[c] = Frag<T>{};
+        if constexpr (kSplit<T>) {                                      // the parts come padded with zeros
+            const int byte = (c / S::GROUPS) * S::ROW + (c % S::GROUPS) * 64 + q * 16;
+            if (ok) f[c] = frag_load<T, DP>(row + byte);
+            else f[c] = Frag<T>{};
+        } else {
+            const int e = c * S::KD + q * S::ELEMS;
+            if (ok && e < D) f[c] = frag_load<T, DP>(row + e * S::SIZE);
+            else f[c] = Frag<T>{};
+        }
     }
 }
 template <typename T>
 __device__ __forceinline__ Frag<T> frag_negated(Frag<T> f) {
-    if constexpr (sizeof(T) == 4) return FragF{{-f.v[0], -f.v[1], -f.v[2], -f.v[3]}};
+    if constexpr (std::is_same_v<T, float>) return FragF{{-f.v[0], -f.v[1], -f.v[2], -f.v[3]}};
     else return FragH{make_uint4(f.v.x ^ 0x80008000u, f.v.y ^ 0x80008000u, f.v.z ^ 0x80008000u, f.v.w ^ 0x80008000u)};
 }
 
 // acc += A B over the KD elements of one fragment
 template <typename T, int DP>
 __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
         for (int t = 0; t < Shape<T, DP>::ELEMS; ++t) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[t], b.v[t], acc, 0, 0, 0);
     } else if constexpr (Shape<T, DP>::NARROW) {
@@ -118,9 +157,9 @@ __device__ __forceinline__ void mma(const Frag<T> &a, const Frag<T> &b, f32x4 &a
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v), __builtin_bit_cast(bf16x8, b.v), acc, 0, 0, 0);
     }
 }
-// acc += A B over the CHUNK rows of one fragment of the second product
-template <typename T>
-__device__ __forceinline__ void mma_rows(const Frag<T> &a, const Frag<T> &b, f32x4 &acc) { mma<T, 64>(a, b, acc); }
+// the terms of a product of parts, small ones first: part of A, part of B
+constexpr int kTerms = 6;
+constexpr int kTermA[kTerms] = {2, 0, 1, 1, 0, 0}, kTermB[kTerms] = {0, 2, 1, 0, 1, 0};
 
 // Results of matrix instructions that a branch stands between them and their first other reader: hipcc (ROCm 7.2) counts the wait states such a
 // reader needs (10 at most here) along straight code and can miss them behind a branch, and the hardware does not wait by itself.  The
@@ -153,35 +192,94 @@ __device__ __forceinline__ void settle(f32x4 (&z)[M][N]) {
 // The second product sums over CHUNK staged rows.  Its B operand is made of score tiles (C layout: row 4 q + r of a
 // tile in register r), its A operand reads the staged rows column-wise in the same order of rows.
 template <typename T>
-__device__ __forceinline__ Frag<T> frag_scores(const f32x4 *tile) {
-    if constexpr (sizeof(T) == 4) return FragF{{tile[0][0], tile[0][1], tile[0][2], tile[0][3]}};
-    else return FragH{make_uint4(pack_bf16x2(tile[0][0], tile[0][1]), pack_bf16x2(tile[0][2], tile[0][3]), pack_bf16x2(tile[1][0], tile[1][1]), pack_bf16x2(tile[1][2], tile[1][3]))};
+__device__ __forceinline__ ManyOf<T> frag_scores(const f32x4 *tile) {
+    if constexpr (std::is_same_v<T, float>) {
+        return {FragF{{tile[0][0], tile[0][1], tile[0][2], tile[0][3]}}};
+    } else if constexpr (!kSplit<T>) {
+        return {FragH{make_uint4(pack_bf16x2(tile[0][0], tile[0][1]), pack_bf16x2(tile[0][2], tile[0][3]), pack_bf16x2(tile[1][0], tile[1][1]), pack_bf16x2(tile[1][2], tile[1][3]))}};
+    } else {
+        ManyOf<T> f;
+        uint32_t w[3][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split3_pack(tile[i >> 1][2 * (i & 1)], tile[i >> 1][2 * (i & 1) + 1], w[0][i], w[1][i], w[2][i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) f.p[k] = FragH{make_uint4(w[k][0], w[k][1], w[k][2], w[k][3])};
+        return f;
+    }
 }
-// row0 a multiple of CHUNK, d0 of 16
-template <typename T, int DP>
-__device__ __forceinline__ Frag<T> frag_turned(const char *tile, int row0, int d0) {
-    using S = Shape<T, DP>;
+// the 16 columns from byte `col` on of CHUNK staged 16-bit rows: ds_read_b64_tr_b16, in which 16 lanes give the addresses of a 4 x 16 block
+// (lane i: row i / 4, columns 4 (i % 4) ..) and each gets a column of it
+template <typename S>
+__device__ __forceinline__ FragH turned_h(const char *plane, int row0, int col) {
     const int lane = threadIdx.x & 63;
-    if constexpr (sizeof(T) == 4) {
-        const int n = DP == 8 ? lane & 7 : lane & 15;                  // DP = 8: the upper eight columns are not used
+    const char *p = plane + S::at(row0 + 4 * (lane >> 4) + ((lane & 15) >> 2), col + (lane & 3) * 8);
+    using lds4 = __attribute__((address_space(3))) i16x4;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 16 * S::ROW));
+    return FragH{__builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7))};
+}
+// row0 a multiple of CHUNK; result columns 16 t ..
+template <typename T, int DP>
+__device__ __forceinline__ ManyOf<T> frag_turned(const char *tile, int row0, int t) {
+    using S = Shape<T, DP>;
+    if constexpr (std::is_same_v<T, float>) {
+        const int lane = threadIdx.x & 63, n = DP == 8 ? lane & 7 : lane & 15;                  // DP = 8: the upper eight columns are not used
         FragF f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const float *>(tile + S::at(row0 + 4 * (lane >> 4) + r, (d0 + n) * 4));
-        return f;
+        for (int r = 0; r < 4; ++r) f.v[r] = *reinterpret_cast<const float *>(tile + S::at(row0 + 4 * (lane >> 4) + r, (16 * t + n) * 4));
+        return {f};
+    } else if constexpr (!kSplit<T>) {
+        return {turned_h<S>(tile, row0, 32 * t)};
     } else {
-        // ds_read_b64_tr_b16: 16 lanes give the addresses of a 4 x 16 block (lane i: row i / 4, columns 4 (i % 4) ..), each gets a column of it
-        const char *p = tile + S::at(row0 + 4 * (lane >> 4) + ((lane & 15) >> 2), (d0 + (lane & 3) * 4) * 2);
-        using lds4 = __attribute__((address_space(3))) i16x4;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
-        const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 16 * S::ROW));
-        return FragH{__builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7))};
+        return {turned_h<S>(tile, row0, 32 * t), turned_h<S>(tile + S::PLANE, row0, 32 * t), turned_h<S>(tile + 2 * S::PLANE, row0, 32 * t)};
+    }
+}
+// acc[u] += A B[u] over CHUNK rows
+template <typename T, int DP, int N, bool SKIP>
+__device__ __forceinline__ void mma_rows(const ManyOf<T> &a, const ManyOf<T> (&b)[N], const bool (&use)[N], f32x4 *const (&acc)[N]) {
+    if constexpr (!kSplit<T>) {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (use[u]) mma<T, 64>(a.p[0], b[u].p[0], *acc[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (use[u]) {
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k) mma<T, 64>(a.p[kTermA[k]], b[u].p[kTermB[k]], *acc[u]);
+            }
+        if constexpr (SKIP) settle_sums();                              // branches stand between: see settle
     }
 }
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> frag_row(const char *tile, int row0, int c) {
     using S = Shape<T, DP>;
-    const int lane = threadIdx.x & 63;
-    return frag_load<T, DP>(tile + S::at(row0 + (lane & 15), c * 4 * S::PIECE + (lane >> 4) * S::PIECE));
+    const int lane = threadIdx.x & 63, q = lane >> 4, row = row0 + (lane & 15);
+    return frag_load<T, DP>(tile + (c / S::GROUPS) * S::PLANE + S::at(row, (c % S::GROUPS) * 4 * S::PIECE + q * S::PIECE));
+}
+// acc[u] += (16 staged rows from row0) . (row in registers b[u]), over the whole width
+template <typename T, int DP, int N, bool SKIP>
+__device__ __forceinline__ void mma_scores(const char *tile, int row0, const Frag<T> (&b)[N][Shape<T, DP>::FRAGS], const bool (&use)[N], f32x4 *const (&acc)[N]) {
+    using S = Shape<T, DP>;
+#pragma unroll
+    for (int c = 0; c < S::GROUPS; ++c) {
+        Frag<T> a[S::PLANES];
+#pragma unroll
+        for (int k = 0; k < S::PLANES; ++k) a[k] = frag_row<T, DP>(tile, row0, k * S::GROUPS + c);
+        if constexpr (S::PLANES == 1) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (use[u]) mma<T, DP>(a[0], b[u][c], *acc[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (use[u]) {
+#pragma unroll
+                    for (int k = 0; k < kTerms; ++k) mma<T, DP>(a[kTermA[k]], b[u][kTermB[k] * S::GROUPS + c], *acc[u]);
+                }
+        }
+    }
+    if constexpr (SKIP && kSplit<T>) settle_sums();
 }
 
 // how a kernel gets the mask: there is none; as floats (the few rows of KEYW); as bits
@@ -209,6 +307,11 @@ struct DotArgs {
     float *part_o, *part_ml;            // split forward: [rows of the launch][splits][D], [..][2]
 };
 
+// row i of a head of graph b
+template <typename S>
+__device__ __forceinline__ const char *row_of(const DotRows &x, int64_t b, int64_t i, int head) {
+    return reinterpret_cast<const char *>(x.p) + (b * x.batch + i * x.node + head * x.head) * S::SIZE;
+}
 __device__ __forceinline__ int graph_size(const int32_t *sizes, int64_t b, int n) { return sizes ? max(0, min(sizes[b], n)) : n; }
 
 // Which (graph, key/value head, tile, split) a block of the 1-d grid works on.  Blocks go to the eight dies in turn and each die has an
@@ -263,7 +366,7 @@ struct Stager {
     __device__ __forceinline__ int row_of(int set, int lane) const { return (set * LANES + w) * ROWS + lane / S::CPR; }
     __device__ __forceinline__ int byte_of(int r, int lane, int D) const {
         const int c = (lane % S::CPR) ^ S::swizzle(r);
-        return c * (16 / S::SIZE) < D ? c * 16 : 0;
+        return kSplit<T> || c * (16 / S::SIZE) < D ? c * 16 : 0;
     }
     // x0, y0: element offsets of the first row
     __device__ __forceinline__ void init(const DotRows &x, const DotRows &y, int64_t x0, int64_t y0, int D, int wave) {
@@ -302,8 +405,10 @@ struct Stager {
                         const int r = row_of(set, lane);
                         src -= max(0, r - (count - 1)) * node[z];
                     }
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                                     (__attribute__((address_space(3))) void *)(lds + (z * LOADS + set * LANES + w) * 1024), 16, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < S::PLANES; ++k)
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + k * S::ROW),
+                                                         (__attribute__((address_space(3))) void *)(lds + ((z * S::PLANES + k) * LOADS + set * LANES + w) * 1024), 16, 0, 0);
                 }
         }
         move(KT * node[0], KT * node[1]);
@@ -453,10 +558,10 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {
 // fewer, the four waves have the same rows and walk different tiles, each staging its own, and join at the end.
 // SPLIT: the block covers one range of the keys and leaves its unnormalised sums.
 template <typename T, int DP, bool KEYW, int NQ, bool SPLIT, int MASK>
-__global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
+__global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot_fwd_kernel(DotArgs a) {
     using S = Shape<T, DP>;
-    constexpr int KT = KEYW ? S::KTW : S::KT, TILE = KT * S::ROW, KS = KT / 16, DT = S::DT, ROWS = KEYW ? 16 : 64 * NQ, OWNERS = KEYW ? 4 : 1, STEP = OWNERS * KT;
-    constexpr bool ONES = DP == 8 && S::SIZE == 4;              // eight columns of the last product are free: one of them sums the probabilities
+    constexpr int KT = KEYW ? S::KTW : S::KT, TILE = KT * S::ROW * S::PLANES, KS = KT / 16, DT = S::DT, ROWS = KEYW ? 16 : 64 * NQ, OWNERS = KEYW ? 4 : 1, STEP = OWNERS * KT;
+    constexpr bool ONES = DP == 8 && std::is_same_v<T, float>;              // eight columns of the last product are free: one of them sums the probabilities
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const DotBlock blk = dot_block<MASK>(a);
     if (!blk.ok) return;
@@ -478,7 +583,7 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
         head[u] = blk.hk * a.group + row[u] - qi[u] * a.group;
         live[u] = qi[u] < queries;
         const int64_t i = live[u] ? qi[u] : 0;
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + i * a.q.node + head[u] * a.q.head, a.D, live[u], qf[u]);
+        row_frags<T, DP>(row_of<S>(a.q, b, i, head[u]), a.D, live[u], qf[u]);
         if (a.scale < 0.f) {
 #pragma unroll
             for (int c = 0; c < S::FRAGS; ++c) qf[u][c] = frag_negated<T>(qf[u][c]);
@@ -535,13 +640,14 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
                     z[u][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
                 }
                 if (any) {
+                    bool use[NQ];
+                    f32x4 *to[NQ];
 #pragma unroll
-                    for (int c = 0; c < S::FRAGS; ++c) {
-                        const Frag<T> kf = frag_row<T, DP>(ks, 16 * t, c);
-#pragma unroll
-                        for (int u = 0; u < NQ; ++u)
-                            if (!SKIP || has[u][t]) mma<T, DP>(kf, qf[u][c], z[u][t]);
+                    for (int u = 0; u < NQ; ++u) {
+                        use[u] = !SKIP || has[u][t];
+                        to[u] = &z[u][t];
                     }
+                    mma_scores<T, DP, NQ, SKIP>(ks, 16 * t, qf, use, to);
                     if constexpr (SKIP) {
                         if constexpr (NQ == 1) settle(z[0][t]);
                         else settle(z[0][t], z[1][t]);
@@ -597,19 +703,23 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
                     any |= use[u];
                 }
                 if (!any) continue;
-                Frag<T> pf[NQ];
+                ManyOf<T> pf[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) pf[u] = frag_scores<T>(&z[u][c * PER]);       // a tile without attended keys holds zeros
+                for (int u = 0; u < NQ; ++u) {
+                    pf[u] = frag_scores<T>(&z[u][c * PER]);       // a tile without attended keys holds zeros
+                    use[u] |= !SKIP;
+                }
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    Frag<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, 16 * t);
+                    ManyOf<T> vf = frag_turned<T, DP>(vs, c * S::CHUNK, t);
                     if constexpr (ONES) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) vf.v[r] = n == 8 ? 1.f : vf.v[r];
+                        for (int r = 0; r < 4; ++r) vf.p[0].v[r] = n == 8 ? 1.f : vf.p[0].v[r];
                     }
+                    f32x4 *to[NQ];
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u)
-                        if (!SKIP || use[u]) mma_rows<T>(vf, pf[u], o[u][t]);
+                    for (int u = 0; u < NQ; ++u) to[u] = &o[u][t];
+                    mma_rows<T, DP, NQ, SKIP>(vf, pf, use, to);
                 }
             }
             settle_sums();
@@ -672,14 +782,14 @@ __global__ __launch_bounds__(256, 2) void dot_fwd_kernel(DotArgs a) {
             }
         } else {
             const float inv = !live[u] || sum[u] == 0.f ? 0.f : 1.0f / sum[u];
-            T *orow = reinterpret_cast<T *>(a.out) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
+            Elem<T> *orow = reinterpret_cast<Elem<T> *>(a.out) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
                 if (16 * t + 4 * q4 < a.D) {
                     f32x4 v = o[u][t];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = inv == 0.f ? 0.f : v[r] * inv;
-                    store4<T>(orow + 16 * t + 4 * q4, v);
+                    store4<Elem<T>>(orow + 16 * t + 4 * q4, v);
                 }
             if (a.lse && q4 == 0) a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] = inv == 0.f ? INFINITY : m[u] + log2f(sum[u]);
         }
@@ -693,7 +803,7 @@ __device__ __forceinline__ void store_joined(const DotArgs &a, int64_t b, int qi
     f32x4 v = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = inv == 0.f ? 0.f : v[k] * inv;
-    store4<T>(reinterpret_cast<T *>(a.out) + ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d, v);
+    store4<Elem<T>>(reinterpret_cast<Elem<T> *>(a.out) + ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d, v);
     if (a.lse && d == 0) a.lse[(b * a.H + head) * a.Nq + qi] = inv == 0.f ? INFINITY : top + log2f(sum);
 }
 
@@ -760,7 +870,7 @@ __global__ __launch_bounds__(256) void dot_join_kernel(DotArgs a, int64_t rows) 
 
 // ---- backward: dq and delta ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int NQ, int MASK>
-__global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
+__global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot_bwd_q_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int KT = S::KT, DT = S::DT, ROWS = 64 * NQ, PER = S::CHUNK / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -785,29 +895,37 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
         head[u] = blk.hk * a.group + row - qi[u] * a.group;
         const bool live = qi[u] < queries;
         const int64_t i = live ? qi[u] : 0;
-        Frag<T> of[S::FRAGS];
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.q.p) + b * a.q.batch + i * a.q.node + head[u] * a.q.head, a.D, live, qf[u]);
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.d_o.p) + b * a.d_o.batch + i * a.d_o.node + head[u] * a.d_o.head, a.D, live, df[u]);
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.o.p) + b * a.o.batch + i * a.o.node + head[u] * a.o.head, a.D, live, of);
-        float dot = 0.f;
+        row_frags<T, DP>(row_of<S>(a.q, b, i, head[u]), a.D, live, qf[u]);
+        row_frags<T, DP>(row_of<S>(a.d_o, b, i, head[u]), a.D, live, df[u]);
+        const int64_t at = (b * a.H + head[u]) * a.Nq + min(qi[u], a.Nq - 1);
+        lse[u] = live ? a.lse[at] : INFINITY;
+        if constexpr (kSplit<T>) {                                       // formed where dout was split
+            delta[u] = live ? a.delta[at] : 0.f;
+        } else {
+            Frag<T> of[S::FRAGS];
+            row_frags<T, DP>(row_of<S>(a.o, b, i, head[u]), a.D, live, of);
+            float dot = 0.f;
 #pragma unroll
-        for (int c = 0; c < S::FRAGS; ++c) {
-            if constexpr (S::SIZE == 4) {
+            for (int c = 0; c < S::FRAGS; ++c) {
+                if constexpr (S::SIZE == 4) {
 #pragma unroll
-                for (int t = 0; t < S::ELEMS; ++t) dot = fmaf(df[u][c].v[t], of[c].v[t], dot);
-            } else {
-                const uint32_t x[4] = {df[u][c].v.x, df[u][c].v.y, df[u][c].v.z, df[u][c].v.w}, y[4] = {of[c].v.x, of[c].v.y, of[c].v.z, of[c].v.w};
+                    for (int t = 0; t < S::ELEMS; ++t) dot = fmaf(df[u][c].v[t], of[c].v[t], dot);
+                } else {
+                    const uint32_t x[4] = {df[u][c].v.x, df[u][c].v.y, df[u][c].v.z, df[u][c].v.w}, y[4] = {of[c].v.x, of[c].v.y, of[c].v.z, of[c].v.w};
 #pragma unroll
-                for (int t = 0; t < S::ELEMS / 2; ++t) {
-                    dot = fmaf(__uint_as_float(x[t] << 16), __uint_as_float(y[t] << 16), dot);
-                    dot = fmaf(__uint_as_float(x[t] & 0xffff0000u), __uint_as_float(y[t] & 0xffff0000u), dot);
+                    for (int t = 0; t < S::ELEMS / 2; ++t) {
+                        dot = fmaf(__uint_as_float(x[t] << 16), __uint_as_float(y[t] << 16), dot);
+                        dot = fmaf(__uint_as_float(x[t] & 0xffff0000u), __uint_as_float(y[t] & 0xffff0000u), dot);
+                    }
                 }
             }
-            if (a.scale < 0.f) qf[u][c] = frag_negated<T>(qf[u][c]);
+            delta[u] = over_groups_sum(dot);
+            if (q4 == 0 && qi[u] < a.Nq) a.delta[at] = delta[u];
         }
-        delta[u] = over_groups_sum(dot);
-        lse[u] = live ? a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] : INFINITY;
-        if (q4 == 0 && qi[u] < a.Nq) a.delta[(b * a.H + head[u]) * a.Nq + qi[u]] = delta[u];
+        if (a.scale < 0.f) {
+#pragma unroll
+            for (int c = 0; c < S::FRAGS; ++c) qf[u][c] = frag_negated<T>(qf[u][c]);
+        }
         mask[u].init(a, b, i);
     }
     if (keys > 0) {
@@ -862,16 +980,16 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
                     }
                     any |= here;
                     if (!here) continue;
+                    bool some[NQ];
+                    f32x4 *zt[NQ], *dt[NQ];
 #pragma unroll
-                    for (int f = 0; f < S::FRAGS; ++f) {
-                        const Frag<T> kf = frag_row<T, DP>(ks, r0, f), vf = frag_row<T, DP>(vs, r0, f);
-#pragma unroll
-                        for (int u = 0; u < NQ; ++u)
-                            if (!SKIP || has[u][r0 / 16]) {
-                                mma<T, DP>(kf, qf[u][f], z[u][t]);
-                                mma<T, DP>(vf, df[u][f], dp[u]);
-                            }
+                    for (int u = 0; u < NQ; ++u) {
+                        some[u] = !SKIP || has[u][r0 / 16];
+                        zt[u] = &z[u][t];
+                        dt[u] = &dp[u];
                     }
+                    mma_scores<T, DP, NQ, SKIP>(ks, r0, qf, some, zt);
+                    mma_scores<T, DP, NQ, SKIP>(vs, r0, df, some, dt);
                     if constexpr (NQ == 1) settle(z[0][t], dp[0]);
                     else settle(z[0][t], dp[0], z[1][t], dp[1]);
 #pragma unroll
@@ -883,15 +1001,18 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
                         }
                 }
                 if (!any) continue;
-                Frag<T> zf[NQ];
+                ManyOf<T> zf[NQ];
 #pragma unroll
-                for (int u = 0; u < NQ; ++u) zf[u] = frag_scores<T>(z[u]);
+                for (int u = 0; u < NQ; ++u) {
+                    zf[u] = frag_scores<T>(z[u]);
+                    use[u] |= !SKIP;
+                }
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    const Frag<T> kf = frag_turned<T, DP>(ks, c * S::CHUNK, 16 * t);
+                    f32x4 *to[NQ];
 #pragma unroll
-                    for (int u = 0; u < NQ; ++u)
-                        if (!SKIP || use[u]) mma_rows<T>(kf, zf[u], acc[u][t]);
+                    for (int u = 0; u < NQ; ++u) to[u] = &acc[u][t];
+                    mma_rows<T, DP, NQ, SKIP>(frag_turned<T, DP>(ks, c * S::CHUNK, t), zf, use, to);
                 }
             }
             settle_sums();
@@ -906,14 +1027,14 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 #pragma unroll
     for (int u = 0; u < NQ; ++u) {
         if (qi[u] >= a.Nq) continue;
-        T *row = reinterpret_cast<T *>(a.dq) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
+        Elem<T> *row = reinterpret_cast<Elem<T> *>(a.dq) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             if (16 * t + 4 * q4 < a.D) {
                 f32x4 v = acc[u][t];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] *= a.scale;
-                store4<T>(row + 16 * t + 4 * q4, v);
+                store4<Elem<T>>(row + 16 * t + 4 * q4, v);
             }
     }
 }
@@ -922,7 +1043,7 @@ __global__ __launch_bounds__(256, 2) void dot_bwd_q_kernel(DotArgs a) {
 // A wave owns NK x 16 keys (one per lane of a row of 16) and walks the queries of each sharing head in turn.  Rows behind the last
 // one come with lse = inf: their probabilities are zero.
 template <typename T, int DP, int NK, int MASK>
-__global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_bwd_kv_kernel(DotArgs a) {
+__global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 || Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot_bwd_kv_kernel(DotArgs a) {
     using S = Shape<T, DP>;
     constexpr int QT = S::KT, DT = S::DT, KEYS = 64 * NK, PER = S::CHUNK / 16;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -965,8 +1086,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
         key[u] = blk.tile * KEYS + (wave * NK + u) * 16 + n;
         const bool live = key[u] < keys;
         col[u] = live ? key[u] : 0;
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.k.p) + b * a.k.batch + (int64_t)col[u] * a.k.node + blk.hk * a.k.head, a.D, live, kf[u]);
-        row_frags<T, DP>(reinterpret_cast<const T *>(a.v.p) + b * a.v.batch + (int64_t)col[u] * a.v.node + blk.hk * a.v.head, a.D, live, vf[u]);
+        row_frags<T, DP>(row_of<S>(a.k, b, col[u], blk.hk), a.D, live, kf[u]);
+        row_frags<T, DP>(row_of<S>(a.v, b, col[u], blk.hk), a.D, live, vf[u]);
         if (a.scale < 0.f) {
 #pragma unroll
             for (int c = 0; c < S::FRAGS; ++c) kf[u][c] = frag_negated<T>(kf[u][c]);
@@ -1033,16 +1154,15 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                     }
                     any |= here;
                     if (!here) continue;
+                    f32x4 *zt[NK], *dt[NK];
 #pragma unroll
-                    for (int f = 0; f < S::FRAGS; ++f) {
-                        const Frag<T> qf = frag_row<T, DP>(qs, s0, f), df = frag_row<T, DP>(ds, s0, f);
-#pragma unroll
-                        for (int u = 0; u < NK; ++u)
-                            if (!SKIP || some[u]) {
-                                mma<T, DP>(qf, kf[u][f], z[u][t]);
-                                mma<T, DP>(df, vf[u][f], dp[u]);
-                            }
+                    for (int u = 0; u < NK; ++u) {
+                        some[u] |= !SKIP;
+                        zt[u] = &z[u][t];
+                        dt[u] = &dp[u];
                     }
+                    mma_scores<T, DP, NK, SKIP>(qs, s0, kf, some, zt);
+                    mma_scores<T, DP, NK, SKIP>(ds, s0, vf, some, dt);
                     if constexpr (NK == 1) settle(z[0][t], dp[0]);
                     else settle(z[0][t], dp[0], z[1][t], dp[1]);
                     const f32x4 lse = *reinterpret_cast<const f32x4 *>(&lses[at][s0 + 4 * q4]), delta = *reinterpret_cast<const f32x4 *>(&deltas[at][s0 + 4 * q4]);
@@ -1067,21 +1187,23 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                         }
                 }
                 if (!any) continue;
-                Frag<T> pf[NK], zf[NK];
+                ManyOf<T> pf[NK], zf[NK];
 #pragma unroll
                 for (int u = 0; u < NK; ++u) {
                     pf[u] = frag_scores<T>(p[u]);
                     zf[u] = frag_scores<T>(z[u]);
+                    use[u] |= !SKIP;
                 }
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    const Frag<T> df = frag_turned<T, DP>(ds, c * S::CHUNK, 16 * t), qf = frag_turned<T, DP>(qs, c * S::CHUNK, 16 * t);
+                    f32x4 *vt[NK], *kt[NK];
 #pragma unroll
-                    for (int u = 0; u < NK; ++u)
-                        if (!SKIP || use[u]) {
-                            mma_rows<T>(df, pf[u], dv[u][t]);
-                            mma_rows<T>(qf, zf[u], dk[u][t]);
-                        }
+                    for (int u = 0; u < NK; ++u) {
+                        vt[u] = &dv[u][t];
+                        kt[u] = &dk[u][t];
+                    }
+                    mma_rows<T, DP, NK, SKIP>(frag_turned<T, DP>(ds, c * S::CHUNK, t), pf, use, vt);
+                    mma_rows<T, DP, NK, SKIP>(frag_turned<T, DP>(qs, c * S::CHUNK, t), zf, use, kt);
                 }
             }
             settle_sums();
@@ -1103,9 +1225,56 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 ? 1 : 2)) void dot_b
                     x[r] = keep == 0.f ? 0.f : x[r] * a.scale;
                     y[r] = keep == 0.f ? 0.f : y[r];
                 }
-                store4<T>(reinterpret_cast<T *>(a.dk) + at + 16 * t + 4 * q4, x);
-                store4<T>(reinterpret_cast<T *>(a.dv) + at + 16 * t + 4 * q4, y);
+                store4<Elem<T>>(reinterpret_cast<Elem<T> *>(a.dk) + at + 16 * t + 4 * q4, x);
+                store4<Elem<T>>(reinterpret_cast<Elem<T> *>(a.dv) + at + 16 * t + 4 * q4, y);
             }
+    }
+}
+
+// ---- rows of three parts -------------------------------------------------------------------------------------------------------
+struct SplitArgs {
+    DotRows x[3];                       // fp32 rows of up to three tensors, one to a blockIdx.y
+    void *out[3];                       // their [B, N, heads] rows of 3 x DP bf16
+    int64_t rows[3];                    // B * N * heads
+    int N[3], heads[3], D;
+    DotRows o;                          // DELTA: the forward's result, rows as x[0]
+    float *delta;                       // [B, heads, N]: <x, o>
+};
+
+// DP / 8 lanes a row, eight elements a lane: 4 bytes read and 6 written per element (5.2 TB/s for 26 M elements)
+template <int DP, bool DELTA>
+__global__ __launch_bounds__(256) void dot_split_kernel(SplitArgs a) {
+    constexpr int LANES = DP / 8;
+    const int lane = threadIdx.x % LANES, e = lane * 8, z = blockIdx.y, heads = a.heads[z], N = a.N[z];
+    const DotRows x = a.x[z];
+    // whole lane groups leave the loop together
+    for (int64_t rr = blockIdx.x * (int64_t)(256 / LANES) + threadIdx.x / LANES; rr < a.rows[z]; rr += (int64_t)gridDim.x * (256 / LANES)) {
+        const int64_t bi = rr / heads, b = bi / N;
+        const int h = (int)(rr - bi * heads), i = (int)(bi - b * N);
+        auto load = [&](const DotRows &r, float (&f)[8]) {
+            const float *p = reinterpret_cast<const float *>(r.p) + b * r.batch + i * r.node + h * r.head + e;
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const float4 u = e + k < a.D ? *reinterpret_cast<const float4 *>(p + k) : make_float4(0.f, 0.f, 0.f, 0.f);      // D is a multiple of 4
+                f[k] = u.x; f[k + 1] = u.y; f[k + 2] = u.z; f[k + 3] = u.w;
+            }
+        };
+        float v[8], o[8];
+        load(x, v);
+        if constexpr (DELTA) load(a.o, o);
+        uint32_t w[3][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) split3_pack(v[2 * k], v[2 * k + 1], w[0][k], w[1][k], w[2][k]);
+        uint16_t *out = reinterpret_cast<uint16_t *>(a.out[z]) + rr * (3 * DP) + e;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(out + k * DP) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+        if constexpr (DELTA) {
+            float dot = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dot = fmaf(v[k], o[k], dot);
+            dot = group_sum<LANES>(dot);
+            if (lane == 0) a.delta[(b * heads + h) * N + i] = dot;
+        }
     }
 }
 
@@ -1207,38 +1376,92 @@ extern "C" size_t gatmi_dot_attn_fwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk
     return splits == 1 ? 0 : (size_t)B * Hkv * rows * splits * (D + 2);
 }
 
+// Whether fp32 rows are computed as three parts.  Splitting costs as much as so many rows by keys cost on the fp32 instructions; fp32 against parts,
+// forward with backward / forward alone, 4 heads, masks of 10 %, in us:
+//   32 wide: 256 graphs of 100: 116 / 29 - 117 / 40; of 150: 277 / 68 - 235 / 70; 64 of 512: 401 / 98 - 301 / 85
+//   64 wide: 256 of 100: 228 / 58 - 215 / 70;  64 of 256: 222 / 56 - 176 / 54;  16 of 1024: 733 / 185 - 480 / 121
+//   128 wide: 256 of 150: 844 / 192 - 934 / 305;  256 of 200: 1403 / 318 - 1365 / 419;  16 of 1024: 1509 / 344 - 1134 / 290
+// Up to 16 wide the vector units, not the products, take the time, and parts add to their work (8 wide: 256 of 100: 59 - 83; 16 of 1024: 213 - 196).
+static bool dot_splits_parts(int32_t dtype, int64_t rows, int32_t Nk, int32_t D, bool backward) {
+    return dtype == GATMI_DTYPE_F32 && D > 16 && std::min<int64_t>(rows, Nk) > (backward ? (D > 64 ? 192 : 96) : (D > 64 ? 768 : 256));
+}
+static size_t dot_part_row_floats(int D) { return (D <= 32 ? 32 : (D <= 64 ? 64 : 128)) * 3 / 2; }
+
+// where the parts of q, k and v of one call lie
+template <int DP>
+static void dot_part_rows(const DotArgs &a, int64_t B, float *planes, DotRows (&r)[3]) {
+    constexpr int64_t COLS = Shape<Split3, DP>::COLS;
+    uint16_t *p = reinterpret_cast<uint16_t *>(planes);
+    const int64_t q = (int64_t)a.Nq * a.H * COLS, k = (int64_t)a.Nk * a.Hkv * COLS;
+    r[0] = DotRows{p, q, a.H * COLS, COLS};
+    r[1] = DotRows{p + B * q, k, a.Hkv * COLS, COLS};
+    r[2] = DotRows{p + B * (q + k), k, a.Hkv * COLS, COLS};
+}
+template <int DP, bool DELTA>
+static void dot_split_launch(const SplitArgs &a, int count, hipStream_t st) {
+    const int64_t most = std::max(a.rows[0], std::max(a.rows[1], a.rows[2])), per = 256 / (DP / 8);
+    hipLaunchKernelGGL((dot_split_kernel<DP, DELTA>), dim3((unsigned)std::min<int64_t>(1 << 20, (most + per - 1) / per), count), dim3(256), 0, st, a);
+}
+
 template <typename T, int DP>
-static int dot_fwd_run(DotArgs a, int64_t B, hipStream_t st) {
+static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
     using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
-    const int per = dot_rows_per_block(rows, S::NQ);
+    if constexpr (kSplit<T>) {
+        DotRows r[3];
+        dot_part_rows<DP>(a, B, planes, r);
+        SplitArgs s = {};
+        s.D = a.D;
+        const DotRows *from[3] = {&a.q, &a.k, &a.v};
+        for (int z = 0; z < 3; ++z) {
+            s.x[z] = *from[z];
+            s.out[z] = const_cast<void *>(r[z].p);
+            s.N[z] = z ? a.Nk : a.Nq;
+            s.heads[z] = z ? a.Hkv : a.H;
+            s.rows[z] = B * s.N[z] * s.heads[z];
+        }
+        dot_split_launch<DP, false>(s, 3, st);
+        a.q = r[0]; a.k = r[1]; a.v = r[2];
+    }
+    constexpr int NQ = S::NQ;
+    const int per = rows <= 16 && !kSplit<T> ? 16 : (rows <= 64 ? 64 : 64 * NQ);
     a.tiles = (int)((rows + per - 1) / per);
     const int64_t step = a.splits > 1 ? B : dot_graphs(a);              // split launches are small by construction
     const size_t lds = 4 * S::TILE, lds_keyw = std::max<size_t>(16 * S::KTW * S::ROW, 512 + 4 * S::DT * 1024);
     for (int64_t b0 = 0; b0 < B; b0 += step) {
         a.b0 = b0;
         a.B = (int)std::min(step, B - b0);
-        int rc;
+        int rc = GATMI_OK;
 #define RUN(keyw, nq, split, bytes)                                                                                                      \
     (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, keyw ? kFloats : kBits>, a, bytes, st)                   \
             : dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, kNoMask>, a, bytes, st))
-        if (per == 16) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
-        else if (per == 64) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);
-        else rc = a.splits > 1 ? RUN(false, S::NQ, true, lds) : RUN(false, S::NQ, false, lds);
+        if (per == 16) {
+            if constexpr (!kSplit<T>) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
+        } else if (per == 64) {
+            if constexpr (!kSplit<T>) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);          // parts: more rows than that
+        } else {
+            if constexpr (NQ > 1) rc = a.splits > 1 ? RUN(false, NQ, true, lds) : RUN(false, NQ, false, lds);
+        }
 #undef RUN
         if (rc) return rc;
     }
     if (a.splits > 1) {
+        a.b0 = 0;
         const int64_t total = B * a.Hkv * rows;
         const int64_t per_block = 256 / (a.D / 4);
-        if (a.splits <= 16) hipLaunchKernelGGL((dot_join_few_kernel<T>), dim3((unsigned)((total + per_block - 1) / per_block)), dim3(256), 0, st, a, total);
-        else hipLaunchKernelGGL((dot_join_kernel<T>), dim3((unsigned)std::min<int64_t>(1 << 16, total)), dim3(256), 0, st, a, total);
+        if (a.splits <= 16) hipLaunchKernelGGL((dot_join_few_kernel<Elem<T>>), dim3((unsigned)((total + per_block - 1) / per_block)), dim3(256), 0, st, a, total);
+        else hipLaunchKernelGGL((dot_join_kernel<Elem<T>>), dim3((unsigned)std::min<int64_t>(1 << 16, total)), dim3(256), 0, st, a, total);
     }
     GATMI_LAUNCH_CHECK("dot_attn_fwd");
     return GATMI_OK;
 }
 
-#define GATMI_DOT_DISPATCH(RUN)                                                                    \
+#define GATMI_DOT_DISPATCH(RUN, parts)                                                             \
+    if (dtype == GATMI_DTYPE_F32 && (parts)) {                                                     \
+        if (D <= 32) return RUN(Split3, 32);                                                       \
+        if (D <= 64) return RUN(Split3, 64);                                                       \
+        return RUN(Split3, 128);                                                                   \
+    }                                                                                              \
     if (dtype == GATMI_DTYPE_F32) {                                                                \
         if (D <= 8) return RUN(float, 8);                                                          \
         if (D <= 16) return RUN(float, 16);                                                        \
@@ -1251,9 +1474,18 @@ static int dot_fwd_run(DotArgs a, int64_t B, hipStream_t st) {
     if (D <= 64) return RUN(uint16_t, 64);                                                         \
     return RUN(uint16_t, 128);
 
+extern "C" size_t gatmi_dot_attn_planes_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, int32_t backward) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || !dot_splits_parts(dtype, (int64_t)Nq * (H / Hkv), Nk, D, backward != 0)) return 0;
+    return dot_part_row_floats(D) * (size_t)B * ((size_t)Nq * H + 2 * (size_t)Nk * Hkv);
+}
+
+extern "C" size_t gatmi_dot_attn_bwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype) {
+    return gatmi_dot_attn_planes_floats(B, Nq, Nk, H, Hkv, D, dtype, 1) ? dot_part_row_floats(D) * (size_t)B * Nq * H : 0;
+}
+
 extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
                                   const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const float *bias, int64_t bias_batch,
-                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse, float *mask_words, float *ws, void *stream) {
+                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse, float *mask_words, float *planes, float *ws, void *stream) {
     if (int rc = dot_check("dot_attn_fwd", B, Nq, Nk, H, Hkv, D, dtype)) return rc;
     GATMI_REQUIRE(std::isfinite(scale), GATMI_EINVAL, "dot_attn_fwd: scale %g", (double)scale);
     if (B == 0 || Nq == 0) return GATMI_OK;
@@ -1280,34 +1512,53 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (a.bias && (mask_words || dot_wants_words(rows)))
         if (int rc = dot_mask_words("dot_attn_fwd", &a, bias_batch ? B : 1, mask_words, true, st)) return rc;
-#define RUN(T, dp) dot_fwd_run<T, dp>(a, B, st)
-    GATMI_DOT_DISPATCH(RUN)
+    GATMI_REQUIRE_ALIGNED(planes);
+#define RUN(T, dp) dot_fwd_run<T, dp>(a, B, planes, st)
+    GATMI_DOT_DISPATCH(RUN, planes && dot_splits_parts(dtype, rows, Nk, D, lse != nullptr))
 #undef RUN
 }
 
 template <typename T, int DP>
-static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
+static int dot_bwd_run(DotArgs a, int64_t B, float *planes, float *ws, hipStream_t st) {
     using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
+    if constexpr (kSplit<T>) {                                          // q, k, v as the forward left them; dout now, with delta
+        DotRows r[3];
+        dot_part_rows<DP>(a, B, planes, r);
+        SplitArgs s = {};
+        s.D = a.D;
+        s.x[0] = a.d_o;
+        s.o = a.o;
+        s.delta = a.delta;
+        s.out[0] = ws;
+        s.N[0] = a.Nq;
+        s.heads[0] = a.H;
+        s.rows[0] = B * a.Nq * a.H;
+        dot_split_launch<DP, true>(s, 1, st);
+        a.q = r[0]; a.k = r[1]; a.v = r[2];
+        a.d_o = DotRows{ws, r[0].batch, r[0].node, r[0].head};
+    }
     a.splits = 1;
+    constexpr int NQ = S::NQ, NK = S::nk(false), NKM = S::nk(true);
     for (int pass = 0; pass < 2; ++pass) {
         const int64_t count = pass == 0 ? rows : a.Nk;
         if (count == 0) continue;
         const bool wide = count > 64;
-        const int per = 64 * (wide ? (pass == 0 ? S::NQ : S::nk(a.bias != nullptr)) : 1);
+        const int per = 64 * (wide ? (pass == 0 ? NQ : (a.bias ? NKM : NK)) : 1);
         a.tiles = (int)((count + per - 1) / per);
         const int64_t step = dot_graphs(a);
         for (int64_t b0 = 0; b0 < B; b0 += step) {
             a.b0 = b0;
             a.B = (int)std::min(step, B - b0);
-            int rc;
+            int rc = GATMI_OK;
 #define RUN(kernel, n, mask) dot_launch("dot_attn_bwd", kernel<T, DP, n, mask>, a, 4 * S::TILE, st)
-#define RUN_Q(n) (a.bias ? RUN(dot_bwd_q_kernel, n, kBits) : RUN(dot_bwd_q_kernel, n, kNoMask))
-#define RUN_KV(n) (a.bias ? RUN(dot_bwd_kv_kernel, n, kBits) : RUN(dot_bwd_kv_kernel, n, kNoMask))
-            if (pass == 0) rc = wide ? RUN_Q(S::NQ) : RUN_Q(1);
-            else rc = !wide ? RUN_KV(1) : (a.bias ? RUN(dot_bwd_kv_kernel, S::nk(true), kBits) : RUN(dot_bwd_kv_kernel, S::nk(false), kNoMask));
-#undef RUN_KV
-#undef RUN_Q
+            if (pass == 0) {
+                if (wide) rc = a.bias ? RUN(dot_bwd_q_kernel, NQ, kBits) : RUN(dot_bwd_q_kernel, NQ, kNoMask);
+                else if constexpr (!kSplit<T>) rc = a.bias ? RUN(dot_bwd_q_kernel, 1, kBits) : RUN(dot_bwd_q_kernel, 1, kNoMask);
+            } else {
+                if (wide) rc = a.bias ? RUN(dot_bwd_kv_kernel, NKM, kBits) : RUN(dot_bwd_kv_kernel, NK, kNoMask);
+                else if constexpr (!kSplit<T>) rc = a.bias ? RUN(dot_bwd_kv_kernel, 1, kBits) : RUN(dot_bwd_kv_kernel, 1, kNoMask);
+            }
 #undef RUN
             if (rc) return rc;
         }
@@ -1319,8 +1570,8 @@ static int dot_bwd_run(DotArgs a, int64_t B, hipStream_t st) {
 extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
                                   const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const void *out, const void *dout,
                                   const int64_t *dout_stride, const float *lse, const float *bias, int64_t bias_batch, int64_t bias_row,
-                                  const int32_t *key_sizes, const int32_t *query_sizes, float scale, float *mask_words, void *dq, void *dk, void *dv,
-                                  float *delta, void *stream) {
+                                  const int32_t *key_sizes, const int32_t *query_sizes, float scale, float *mask_words, float *planes, void *dq, void *dk, void *dv,
+                                  float *delta, float *ws, void *stream) {
     if (int rc = dot_check("dot_attn_bwd", B, Nq, Nk, H, Hkv, D, dtype)) return rc;
     GATMI_REQUIRE(std::isfinite(scale), GATMI_EINVAL, "dot_attn_bwd: scale %g", (double)scale);
     if (B == 0 || (Nq == 0 && Nk == 0)) return GATMI_OK;
@@ -1348,7 +1599,11 @@ extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (a.bias)
         if (int rc = dot_mask_words("dot_attn_bwd", &a, bias_batch ? B : 1, mask_words, false, st)) return rc;
-#define RUN(T, dp) dot_bwd_run<T, dp>(a, B, st)
-    GATMI_DOT_DISPATCH(RUN)
+    const bool parts = planes && dot_splits_parts(dtype, (int64_t)Nq * a.group, Nk, D, true);
+    GATMI_REQUIRE(!parts || ws, GATMI_EINVAL, "dot_attn_bwd: workspace is null");
+    GATMI_REQUIRE_ALIGNED(planes);
+    GATMI_REQUIRE_ALIGNED(ws);
+#define RUN(T, dp) dot_bwd_run<T, dp>(a, B, planes, ws, st)
+    GATMI_DOT_DISPATCH(RUN, parts)
 #undef RUN
 }

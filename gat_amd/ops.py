@@ -914,7 +914,8 @@ def _attn_rows(t, width):
 
 
 def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
-    """(rows of q, k, v as the kernels read them, out with padded width, lse or None, the mask as bits or None, bias strides)"""
+    """(rows of q, k, v as the kernels read them, out with padded width, lse or None, the mask as bits or None, fp32 rows
+    in parts or None, bias strides)"""
     B, Nq, H, D = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
     dtype = _FLOATS[q.dtype]
@@ -930,9 +931,13 @@ def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
         strides = (bias.stride(0) if bias.shape[0] > 1 else 0, bias.stride(1))
         if need or Nq * H > 16 * Hkv:                             # a few rows read the floats themselves
             words = _scratch(_lib.lib.gatmi_dot_attn_mask_floats(B, Nq, Nk, strides[0]), dev)
+    planes = None
+    if dtype == _lib.DTYPE_F32:
+        planes = _scratch(_lib.lib.gatmi_dot_attn_planes_floats(B, Nq, Nk, H, Hkv, width, dtype, need), dev)
     _launch(dev, "gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr), vr.data_ptr(), _strides(vr),
-            ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(lse), ptr(words), ptr(ws))
-    return qr, kr, vr, out, lse, words, strides
+            ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(lse), ptr(words),
+            ptr(planes), ptr(ws))
+    return qr, kr, vr, out, lse, words, planes, strides
 
 
 class DotAttentionFn(torch.autograd.Function):
@@ -941,23 +946,24 @@ class DotAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, key_sizes, query_sizes, scale):
         D = q.shape[3]
-        qr, kr, vr, out, lse, words, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
-        ctx.save_for_backward(qr, kr, vr, out, lse, bias, words, key_sizes, query_sizes)
+        qr, kr, vr, out, lse, words, planes, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
+        ctx.save_for_backward(qr, kr, vr, out, lse, bias, words, planes, key_sizes, query_sizes)
         ctx.scale, ctx.D, ctx.bias_strides = scale, D, strides
         return out[..., :D] if out.shape[3] != D else out
 
     @staticmethod
     def backward(ctx, dout):
-        qr, kr, vr, out, lse, bias, words, key_sizes, query_sizes = ctx.saved_tensors
+        qr, kr, vr, out, lse, bias, words, planes, key_sizes, query_sizes = ctx.saved_tensors
         B, Nq, H, width = qr.shape
         Nk, Hkv = kr.shape[1], kr.shape[2]
         D = ctx.D
         dr = _attn_rows(dout, width)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (qr, kr, vr))
         delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
+        ws = None if planes is None else _scratch(_lib.lib.gatmi_dot_attn_bwd_ws_floats(B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype]), qr.device)
         _launch(qr.device, "gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr),
                 vr.data_ptr(), _strides(vr), out.data_ptr(), dr.data_ptr(), _strides(dr), lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
-                ptr(query_sizes), ctx.scale, ptr(words), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr())
+                ptr(query_sizes), ctx.scale, ptr(words), ptr(planes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), ptr(ws))
         if width != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
         return dq, dk, dv, None, None, None, None

@@ -94,6 +94,52 @@ def test_padded_graphs(Nq, Nk, density, dtype):
     _check(_case(5, Nq, Nk, 4, 2, 24, dtype, density=density, sizes=True, seed=Nk), dtype)
 
 
+# many rows of fp32 wider than 16: computed as three parts (for the gradients from 97 rows and keys on, 193 above 64 wide; alone from 257 and 769)
+@pytest.mark.parametrize("D,Nq,Nk,H,G", [(20, 97, 97, 2, 2), (32, 97, 130, 2, 2), (32, 50, 200, 4, 2), (40, 129, 97, 2, 1), (64, 200, 128, 2, 2), (64, 192, 97, 3, 1),
+                                         (96, 193, 193, 1, 1), (100, 97, 257, 2, 1), (128, 260, 193, 1, 1), (128, 321, 200, 2, 2)])
+@pytest.mark.parametrize("density,soft,sizes", [(None, False, False), (0.1, False, False), (0.5, True, True), (0.02, False, True)])
+def test_rows_in_parts(D, Nq, Nk, H, G, density, soft, sizes):
+    _check(_case(3, Nq, Nk, H, G, D, "f32", density=density, soft=soft, sizes=sizes, seed=D + Nq), "f32", what="%d wide" % D)
+
+
+@pytest.mark.parametrize("D,N", [(32, 256), (32, 257), (64, 300), (128, 768), (128, 769)])
+@pytest.mark.parametrize("density", [None, 0.1])
+def test_rows_in_parts_forward_alone(D, N, density):
+    _check(_case(1, N, N, 2, 1, D, "f32", density=density, seed=N), "f32", grad=False)
+
+
+def test_rows_in_parts_keys_split():
+    _check(_case(1, 300, 5000, 2, 2, 64, "f32", seed=4), "f32", grad=False)
+    _check(_case(2, 97, 2100, 1, 1, 32, "f32", sizes=True, seed=4), "f32")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 30.0])
+def test_rows_in_parts_scale(scale):
+    _check(_case(1, 100, 100, 2, 2, 32, "f32", density=0.3, seed=6), "f32", scale=scale)
+
+
+def test_rows_in_parts_keep_a_large_range():
+    c = _case(1, 100, 120, 1, 1, 32, "f32", seed=5)
+    c["q"] *= 1e-12
+    c["k"] *= 1e12
+    c["v"] *= torch.logspace(-20, 20, 32, device="cuda:0")
+    c["dout"] *= torch.logspace(20, -20, 32, device="cuda:0")
+    _check(c, "f32")
+
+
+def test_padding_of_rows_in_parts_is_not_used():
+    c = _case(4, 130, 130, 2, 2, 32, "f32", sizes=True, seed=3)
+    want = _run(c)
+    for n in ("q", "k", "v", "dout"):
+        x = c[n].clone()
+        for b in range(4):
+            x[b, int(c["ks"][b]):] = float("nan")
+        c[n] = x
+    got = _run(c)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_rows_behind_the_sizes_are_not_read(dtype):
     c = _case(4, 70, 70, 2, 2, 16, dtype, sizes=True, seed=3)
