@@ -291,6 +291,8 @@ struct WideArgs {
     float ca, cb, cc;
     double eps;
     int step, growth;             // a step multiplies X by at most 2^growth
+    float *parts;                 // sums of pieces of tiles, or null: see ns_piece_kernel
+    int batch, workers;           // of the launch with pieces
 };
 
 // X is stored times 2^e, e = max(0, e_0 - step growth): |X| 2^e_0 is in [1/2, 1) before the first step where eps makes X small, and
@@ -406,28 +408,26 @@ __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
     }
 }
 
-// C = U V^T over depth K for planes U [.][K] and V [.][K], a WT x WT tile per block, a quarter per wave.
-// MODE: what becomes of C.
+// MODE: what becomes of a product.
 constexpr int kNsGram = 0, kNsPoly = 1, kNsStep = 2, kNsLast = 3;
-template <int MODE, int WT, typename T, bool TALL>
-__global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
+template <int MODE> struct NsMode { static constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly; };
+
+template <int MODE>
+__device__ __forceinline__ const _Float16 *ns_left(const WideArgs &a, int64_t b) {
+    return MODE == kNsGram ? a.x.p + b * a.x_plane : (MODE == kNsPoly ? a.g.p : a.p.p) + b * a.g_plane;
+}
+template <int MODE>
+__device__ __forceinline__ const _Float16 *ns_right(const WideArgs &a, int64_t b) {
+    return MODE == kNsPoly ? a.g.p + b * a.g_plane : (MODE == kNsGram ? a.x.p : a.xt.p) + b * a.x_plane;
+}
+
+// acc += U V^T over the depths k0 .. k1 of planes U [WT rows][K], V [WT rows][K] (from k0 on; k1 - k0 a multiple of kWK), a quarter of the
+// WT x WT tile per wave.  STAGES of U and V in LDS, rows of 128 bytes, all but one on their way.
+template <int WT, int STAGES>
+__device__ __forceinline__ void ns_product(const _Float16 *U, const _Float16 *V, int64_t K, int64_t k0, int64_t k1, char *lds, f32x4 (&acc)[WT / 32][WT / 32]) {
     constexpr int WV = WT / 2, F = WV / 16;                                       // a wave's part of the tile, in fragments
-    // Stages of U and V, rows of 128 bytes.  The symmetric products have about one block to a compute unit: three stages, two of them on their way.
-    constexpr int STAGES = MODE == kNsGram || MODE == kNsPoly ? 3 : 2;
-    extern __shared__ __attribute__((aligned(16))) char ns_lds[];
-    _Float16 (*buf)[2][WT * 2 * kWK] = reinterpret_cast<_Float16 (*)[2][WT * 2 * kWK]>(ns_lds);
+    _Float16 (*buf)[2][WT * 2 * kWK] = reinterpret_cast<_Float16 (*)[2][WT * 2 * kWK]>(lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t b = blockIdx.z;
-    // Blocks go to the eight dies in turn; each die gets an eighth of the tiles in one piece, ordered by squares of 4 x 4 tiles: the blocks
-    // that run together on a die then share rows of U and V in its L2.
-    constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
-    const uint32_t ty = (uint32_t)(a.np / WT), tx = SYM ? ty : (uint32_t)(a.lp / WT), sx = (tx + 3) / 4, per = (((ty + 3) / 4) * sx * 16 + 7) / 8;
-    const uint32_t slot = (blockIdx.x & 7) * per + (blockIdx.x >> 3), sq = slot >> 4;
-    const int ti = (int)(sq / sx * 4 + ((slot >> 2) & 3)), tj = (int)(sq % sx * 4 + (slot & 3));
-    if ((uint32_t)ti >= ty || (uint32_t)tj >= tx || (SYM && tj < ti)) return;        // of a symmetric result only the upper tiles
-    const int64_t K = MODE == kNsGram ? a.lp : a.np;
-    const _Float16 *U = (MODE == kNsGram ? a.x.p + b * a.x_plane : (MODE == kNsPoly ? a.g.p : a.p.p) + b * a.g_plane) + ti * (int64_t)WT * 2 * K;
-    const _Float16 *V = (MODE == kNsPoly ? a.g.p + b * a.g_plane : (MODE == kNsGram ? a.x.p : a.xt.p) + b * a.x_plane) + tj * (int64_t)WT * 2 * K;
     // Rows go straight to LDS, eight a load of 64 lanes x 16 bytes; piece c of row r lies at place c ^ (r / 2 % 8), so that the lanes of a
     // fragment read, which want one piece of 16 rows, find them in different banks.
     const _Float16 *mine = (wave < 2 ? U : V) + (lane >> 3) * 2 * K + ((lane & 7) ^ ((lane >> 4) & 3)) * 8;
@@ -450,21 +450,17 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
         __syncthreads();
     };
-    f32x4 acc[F][F];
-#pragma unroll
-    for (int i = 0; i < F; ++i)
-#pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const int wi = (wave >> 1) * WV, wj = (wave & 1) * WV;
     const int turn = ((lane & 15) >> 1) & 7, row0 = (lane & 15) * 64;
     const int at_hi = row0 + ((lane >> 4) ^ turn) * 8, at_lo = row0 + (((lane >> 4) + 4) ^ turn) * 8;
     constexpr int64_t AHEAD = (STAGES - 1) * kWK;
 #pragma unroll
-    for (int g = 0; g < STAGES - 1; ++g) stage(g, g * kWK);                       // K is a multiple of 128: there are that many
-    arrived(STAGES == 2);
+    for (int g = 0; g < STAGES - 1; ++g)
+        if (k0 + g * kWK < k1) stage(g, k0 + g * kWK);
+    arrived(STAGES == 2 || k0 + kWK >= k1);
     int s = 0;
-    for (int64_t k = 0; k < K; k += kWK, s = s + 1 == STAGES ? 0 : s + 1) {
-        const bool more = k + AHEAD < K;
+    for (int64_t k = k0; k < k1; k += kWK, s = s + 1 == STAGES ? 0 : s + 1) {
+        const bool more = k + AHEAD < k1;
         if (more) stage(s == 0 ? STAGES - 1 : s - 1, k + AHEAD);
         f16x8 uh[F], ul[F], vh[F], vl[F];
 #pragma unroll
@@ -490,49 +486,156 @@ __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
             for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
         arrived(STAGES == 2 || !more);
     }
+}
+
+// Stores the four results of a lane, rows row .. row + 3 of column col of the product of matrix b.  turn: also where the tile lies mirrored.
+template <int MODE, typename T, bool TALL>
+__device__ __forceinline__ void ns_finish(const WideArgs &a, int64_t b, const NsShift &sh, int64_t row, int64_t col, f32x4 sum, bool turn) {
+    constexpr bool SYM = NsMode<MODE>::SYM;
     constexpr float kInv = 1.0f / (kPlaneScale * kPlaneScale);
-    const NsShift sh = ns_shift(a, b);
     const float unscale = MODE == kNsGram ? kInv / sh.now / sh.now : (MODE == kNsStep ? kInv * (sh.next / sh.now) : (MODE == kNsLast ? kInv / sh.now : kInv));
-    const int n0 = lane & 15, m0 = (lane >> 4) * 4;                               // C: row m0 + r, column n0
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = sum[r] * unscale;
+    if constexpr (MODE == kNsLast) {
+        T *out = reinterpret_cast<T *>(a.a.out) + b * a.a.out_batch;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (row + r < a.n && col < a.len) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, row + r, col), v[r]);
+    } else {
+        const Planes C = MODE == kNsGram ? a.g : (MODE == kNsPoly ? a.p : a.x);
+        const Planes Ct = MODE == kNsStep ? a.xt_new : C;
+        const int64_t off = SYM ? b * a.g_plane : b * a.x_plane, ld = SYM ? a.np : a.lp;
+        const int64_t turned = off + Planes::at(col, row, a.np);                   // four consecutive numbers of row `col`
+        if constexpr (MODE == kNsPoly) {                                           // a I + b G + c G^2, G symmetric
+            const f16x4 gh = *reinterpret_cast<const f16x4 *>(a.g.p + turned), gl = *reinterpret_cast<const f16x4 *>(a.g.p + turned + 32);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                v[r] = a.cc * v[r] + a.cb * (((float)gh[r] + (float)gl[r]) * (1.0f / kPlaneScale)) + (row + r == col ? a.ca : 0.f);
+        }
+        f16x4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            _Float16 h, l;
+            split16(v[r], h, l);
+            hi[r] = h;
+            lo[r] = l;
+            C.put(off + Planes::at(row + r, col, ld), h, l);
+        }
+        if (turn) {
+            *reinterpret_cast<f16x4 *>(Ct.p + turned) = hi;
+            *reinterpret_cast<f16x4 *>(Ct.p + turned + 32) = lo;
+        }
+    }
+}
+
+struct NsTile { int64_t b; int ti, tj; };
+__device__ __forceinline__ NsTile ns_tile(int ty, int64_t tile) {         // tiles of a matrix: tj >= ti, row by row
+    const int per = ty * (ty + 1) / 2;
+    NsTile t;
+    t.b = tile / per;
+    int r = (int)(tile - t.b * per);
+    for (t.ti = 0; r >= ty - t.ti; ++t.ti) r -= ty - t.ti;
+    t.tj = t.ti + r;
+    return t;
+}
+
+// One product, a tile per block.
+template <int MODE, int WT, typename T, bool TALL>
+__global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
+    constexpr int WV = WT / 2, F = WV / 16;
+    // The symmetric products have about one block to a compute unit: three stages.
+    constexpr int STAGES = NsMode<MODE>::SYM ? 3 : 2;
+    extern __shared__ __attribute__((aligned(16))) char ns_lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t b = blockIdx.z;
+    // Blocks go to the eight dies in turn; each die gets an eighth of the tiles in one piece, ordered by squares of 4 x 4 tiles: the blocks
+    // that run together on a die then share rows of U and V in its L2.
+    constexpr bool SYM = NsMode<MODE>::SYM;
+    const int ty = (int)(a.np / WT), tx = SYM ? ty : (int)(a.lp / WT), sx = (tx + 3) / 4, squares = SYM ? sx * (sx + 1) / 2 : (ty + 3) / 4 * sx, per = squares * 2;
+    const int slot = (blockIdx.x & 7) * per + (int)(blockIdx.x >> 3), sq = slot >> 4;
+    const NsTile at = SYM ? ns_tile(sx, sq) : NsTile{0, sq / sx, sq % sx};             // of a symmetric result only the upper tiles
+    const int ti = at.ti * 4 + ((slot >> 2) & 3), tj = at.tj * 4 + (slot & 3);
+    if (ti >= ty || tj >= tx || (SYM && tj < ti)) return;
+    const int64_t K = MODE == kNsGram ? a.lp : a.np;
+    f32x4 acc[F][F];
 #pragma unroll
     for (int i = 0; i < F; ++i)
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-            const int64_t row = ti * (int64_t)WT + wi + 16 * i + m0, col = tj * (int64_t)WT + wj + 16 * j + n0;
-            float v[4];
+        for (int j = 0; j < F; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    ns_product<WT, STAGES>(ns_left<MODE>(a, b) + ti * (int64_t)WT * 2 * K, ns_right<MODE>(a, b) + tj * (int64_t)WT * 2 * K, K, 0, K, ns_lds, acc);
+    const NsShift sh = ns_shift(a, b);
+    const int wi = (wave >> 1) * WV, wj = (wave & 1) * WV, n0 = lane & 15, m0 = (lane >> 4) * 4;       // C: row m0 + r, column n0
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * unscale;
-            if constexpr (MODE == kNsLast) {
-                T *out = reinterpret_cast<T *>(a.a.out) + b * a.a.out_batch;
+    for (int i = 0; i < F; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (row + r < a.n && col < a.len) ns_store<T>(out + ns_at<T, TALL>(a.a.out_row, row + r, col), v[r]);
-            } else {
-                const Planes C = MODE == kNsGram ? a.g : (MODE == kNsPoly ? a.p : a.x);
-                const Planes Ct = MODE == kNsStep ? a.xt_new : C;
-                const int64_t off = SYM ? b * a.g_plane : b * a.x_plane, ld = SYM ? a.np : a.lp;
-                const int64_t turned = off + Planes::at(col, row, a.np);               // four consecutive numbers of row `col`
-                if constexpr (MODE == kNsPoly) {                                       // a I + b G + c G^2, G symmetric
-                    const f16x4 gh = *reinterpret_cast<const f16x4 *>(a.g.p + turned), gl = *reinterpret_cast<const f16x4 *>(a.g.p + turned + 32);
+        for (int j = 0; j < F; ++j)
+            ns_finish<MODE, T, TALL>(a, b, sh, ti * (int64_t)WT + wi + 16 * i + m0, tj * (int64_t)WT + wj + 16 * j + n0, acc[i][j], !SYM || ti != tj);
+}
+
+// ---- symmetric products in pieces -------------------------------------------------------------------------------------------
+// A symmetric product has few tiles: 136 of 128 x 128 for 2048 rows, on 256 compute units.  Its steps (tile by tile, depth by depth) are therefore
+// cut into as many equal ranges as there are units.  A range crosses at most one border between tiles (there are no more tiles than
+// ranges); what it has of each of its two tiles is left as a piece, and ns_join_kernel adds the pieces of a tile in order.
+struct NsRange { int64_t from, to; };               // steps
+__host__ __device__ __forceinline__ NsRange ns_range(int64_t total, int workers, int w) { return NsRange{total * w / workers, total * (w + 1) / workers}; }
+constexpr int kPieceFloats = 128 * 128;
+
+template <int MODE>
+__global__ __launch_bounds__(256) void ns_piece_kernel(WideArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char ns_lds[];
+    const int per_die = (a.workers + 7) / 8, w = (blockIdx.x & 7) * per_die + (blockIdx.x >> 3);       // neighbours on one die share rows in its L2
+    if ((int)(blockIdx.x >> 3) >= per_die || w >= a.workers) return;
+    const int ty = (int)(a.np / 128), per = ty * (ty + 1) / 2;
+    const int64_t K = MODE == kNsGram ? a.lp : a.np, steps = K / kWK;
+    const NsRange range = ns_range(steps * per * a.batch, a.workers, w);
+    int64_t at = range.from;
+    for (int piece = 0; at < range.to; ++piece) {
+        const int64_t tile = at / steps, end = min(range.to, (tile + 1) * steps);
+        const NsTile t = ns_tile(ty, tile);
+        f32x4 acc[4][4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        v[r] = a.cc * v[r] + a.cb * (((float)gh[r] + (float)gl[r]) * (1.0f / kPlaneScale)) + (row + r == col ? a.ca : 0.f);
-                }
-                f16x4 hi, lo;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    _Float16 h, l;
-                    split16(v[r], h, l);
-                    hi[r] = h;
-                    lo[r] = l;
-                    C.put(off + Planes::at(row + r, col, ld), h, l);
-                }
-                if (!SYM || ti != tj) {
-                    *reinterpret_cast<f16x4 *>(Ct.p + turned) = hi;
-                    *reinterpret_cast<f16x4 *>(Ct.p + turned + 32) = lo;
-                }
-            }
+            for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        ns_product<128, 3>(ns_left<MODE>(a, t.b) + t.ti * 128ll * 2 * K, ns_right<MODE>(a, t.b) + t.tj * 128ll * 2 * K, K, (at - tile * steps) * kWK, (end - tile * steps) * kWK, ns_lds, acc);
+        float4 *out = reinterpret_cast<float4 *>(a.parts + (2ll * w + piece) * kPieceFloats) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[(i * 4 + j) * 256] = make_float4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]);
+        at = end;
+    }
+}
+
+// four blocks a tile
+template <int MODE>
+__global__ __launch_bounds__(256) void ns_join_kernel(WideArgs a) {
+    const int ty = (int)(a.np / 128), per = ty * (ty + 1) / 2;
+    const int64_t steps = (MODE == kNsGram ? a.lp : a.np) / kWK, total = steps * per * a.batch, tile = blockIdx.x >> 2, from = tile * steps, to = from + steps;
+    const int i = blockIdx.x & 3;
+    int w = (int)(from * a.workers / total);                             // the range that `from` lies in, or a neighbour of it
+    while (w > 0 && ns_range(total, a.workers, w).from > from) --w;
+    while (ns_range(total, a.workers, w).to <= from) ++w;
+    f32x4 acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (; w < a.workers; ++w) {
+        const NsRange range = ns_range(total, a.workers, w);
+        if (range.from >= to) break;
+        const float4 *in = reinterpret_cast<const float4 *>(a.parts + (2ll * w + (range.from < from ? 1 : 0)) * kPieceFloats) + threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 v = in[(i * 4 + j) * 256];
+            acc[j] += (f32x4){v.x, v.y, v.z, v.w};
         }
+    }
+    const NsTile t = ns_tile(ty, tile);
+    const NsShift sh = ns_shift(a, t.b);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = t.ti * 128ll + (wave >> 1) * 64 + 16 * i + (lane >> 4) * 4, col = t.tj * 128ll + (wave & 1) * 64 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ns_finish<MODE, float, false>(a, t.b, sh, row, col + 16 * j, acc[j], t.ti != t.tj);
 }
 
 // ---- small -------------------------------------------------------------------------------------------------------------
@@ -714,9 +817,20 @@ static size_t narrow_ws(int64_t batch, int64_t n, int64_t len) {
     return 2 * (size_t)batch * (gram_parts(batch, len) + 1) * np * np;
 }
 static size_t wide_head(int64_t batch) { return 2 * (size_t)batch * kNormBlocks + ((size_t)batch + 3) / 4 * 4; }      // norms and shifts
+// Ranges of a symmetric product of depth K, 0: a block per tile.  Writing, reading and joining the pieces takes what 64 steps take (all five steps
+// in us, without - with pieces: 1024 x 1024: 348 - 408, 1536 x 1536: 666 - 687, 2048 x 2048: 1063 - 989, 2816 x 2816: 2923 - 2298; long sides: 128 x 512: 120 -
+// 155, 512 x 2048: 348 - 320, 2048 x 4096: 1482 - 1319, 90 x 100000: 8879 - 1567).
+constexpr int64_t kPieceDepth = 2048;
+static int ns_workers(int64_t batch, int64_t np, int64_t K) {
+    const int64_t ty = np / 128, tiles = ty * (ty + 1) / 2 * batch;
+    if (tiles > 256 || K < kPieceDepth) return 0;
+    return (int)std::min<int64_t>(256, tiles * (K / kWK) / 4);                // four steps or more each: no fewer ranges than tiles, none empty
+}
+static size_t wide_planes(int64_t batch, size_t np, size_t lp) { return wide_head(batch) + (size_t)batch * (3 * np * lp + 2 * np * np); }      // X, X^T twice, G, P: two fp16 a float
 static size_t wide_ws(int64_t batch, int64_t n, int64_t len) {
-    const size_t np = (size_t)round_up(n, kWT), lp = (size_t)round_up(len, kWT);
-    return wide_head(batch) + (size_t)batch * (3 * np * lp + 2 * np * np);      // planes of X, X^T twice, G, P: two fp16 a float
+    const int64_t np = round_up(n, kWT), lp = round_up(len, kWT);
+    // a last, smaller set of matrices may have pieces where the others have none: it needs less than their planes take
+    return wide_planes(batch, (size_t)np, (size_t)lp) + 2 * (size_t)kPieceFloats * std::max(ns_workers(batch, np, lp), ns_workers(batch, np, np));
 }
 
 extern "C" size_t gatmi_newton_schulz_ws_floats(int64_t batch, int64_t m, int64_t n) {
@@ -760,11 +874,24 @@ static int run_narrow(const NsMatrix &mat, int64_t batch, int steps, double ca, 
 constexpr int64_t kTileBlocks = 128;
 template <int MODE, typename T, bool TALL>
 static int ns_gemm(const WideArgs &a, int64_t batch, hipStream_t st) {
-    constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly;
+    constexpr bool SYM = NsMode<MODE>::SYM;
+    if constexpr (SYM) {
+        WideArgs p = a;
+        p.batch = (int)batch;
+        p.workers = ns_workers(batch, a.np, MODE == kNsGram ? a.lp : a.np);
+        if (p.workers) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&ns_piece_kernel<MODE>), hipFuncAttributeMaxDynamicSharedMemorySize, 3 * 128 * 256);
+            if (e != hipSuccess) return fail(GATMI_EHIP, "newton_schulz: %s", hipGetErrorString(e));
+            const int64_t t = a.np / 128;
+            hipLaunchKernelGGL((ns_piece_kernel<MODE>), dim3((unsigned)((p.workers + 7) / 8 * 8)), dim3(256), 3 * 128 * 256, st, p);
+            hipLaunchKernelGGL((ns_join_kernel<MODE>), dim3((unsigned)(4 * t * (t + 1) / 2 * batch)), dim3(256), 0, st, p);
+            return GATMI_OK;
+        }
+    }
     const int64_t ty = a.np / 128, tx = SYM ? ty : a.lp / 128;
     auto blocks = [&](int64_t w) {
-        const int64_t y = a.np / w, x = SYM ? y : a.lp / w;
-        return dim3((unsigned)((((y + 3) / 4) * ((x + 3) / 4) * 16 + 7) / 8 * 8), 1, (unsigned)batch);
+        const int64_t y = (a.np / w + 3) / 4, x = SYM ? y : (a.lp / w + 3) / 4;
+        return dim3((unsigned)((SYM ? y * (y + 1) / 2 : y * x) * 16), 1, (unsigned)batch);
     };
     const bool wide = (SYM ? ty * (ty + 1) / 2 : ty * tx) * batch >= kTileBlocks;
     const size_t lds = (SYM ? 3 : 2) * (wide ? 128 : 64) * 256;
@@ -817,6 +944,7 @@ static int run_wide(const NsMatrix &mat, int64_t batch, int steps, double ca, do
     a.xt_new.p = p + 2 * xs;
     a.g.p = p + 3 * xs;
     a.p.p = p + 3 * xs + gs;
+    a.parts = ws + wide_planes(batch, (size_t)a.np, (size_t)a.lp);
     const bool vec = mat.x_row % 4 == 0 && mat.x_batch % 4 == 0 && reinterpret_cast<uintptr_t>(mat.x) % (4 * sizeof(T)) == 0;
     if (vec) hipLaunchKernelGGL((ns_norm_kernel<T, true>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(kNormBlocks, (unsigned)batch), dim3(256), 0, st, a);

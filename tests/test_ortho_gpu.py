@@ -60,6 +60,23 @@ def test_wide_shapes(m, n, dtype):
     _check(_matrices("normal", 2, m, n, seed=m + n), dtype, what="%dx%d" % (m, n))
 
 
+# symmetric products of a depth of 2048 and more are computed in pieces
+@pytest.mark.parametrize("b,m,n,dtype", [(1, 70, 1921, "f32"), (2, 1920, 128, "f32"), (3, 66, 2048, "bf16"), (1, 2300, 200, "f32"), (2, 130, 5000, "bf16"), (1, 90, 40000, "f32"),
+                                         (1, 1930, 2050, "f32")])
+def test_deep_products(b, m, n, dtype):
+    _check(_matrices("normal", b, m, n, seed=m + n), dtype, what="%dx%d" % (m, n))
+
+
+def test_deep_products_of_many_matrices_and_of_one():
+    from gat_amd import ops
+    x = torch.tensor(_matrices("normal", 26, 400, 2000, seed=1), dtype=torch.float32).cuda()      # 260 tiles: a block each; alone: pieces
+    many = ops.newton_schulz(x)
+    for i in (0, 25):
+        one = ops.newton_schulz(x[i])
+        assert (many[i] - one).norm() <= 2 * (WIDE + 2.0 ** -24) * one.norm()
+        assert torch.equal(one, ops.newton_schulz(x[i]))
+
+
 @pytest.mark.parametrize("kind", ["low_rank", "rank_one", "one_entry"])
 @pytest.mark.parametrize("m,n", [(20, 30), (64, 64), (100, 40), (50, 300), (1433, 8), (100, 150), (200, 130)])
 def test_spectra(kind, m, n):
