@@ -299,6 +299,8 @@ struct DotArgs {
     int64_t bias_batch, bias_row;
     const ulonglong2 *row_words, *col_words;      // the mask as bits (dot_mask_kernel), or null
     int64_t row_words_batch, col_words_batch;     // of one graph; 0: one mask for all
+    const int32_t *sparse;                        // per mask: 1 where the kernels that walk single entries do the work; or null
+    int sparse_batch;                             // 1, or 0: one mask for all
     const int32_t *key_sizes, *query_sizes;
     int64_t b0;                         // first graph of this launch
     int B, Nq, Nk, H, Hkv, group, D;    // B: graphs of this launch
@@ -307,6 +309,7 @@ struct DotArgs {
     float *part_o, *part_ml;            // split forward: [rows of the launch][splits][D], [..][2]
 };
 
+__device__ __forceinline__ bool by_entries(const DotArgs &a, int64_t b) { return a.sparse && a.sparse[b * a.sparse_batch] != 0; }
 // row i of a head of graph b
 template <typename S>
 __device__ __forceinline__ const char *row_of(const DotRows &x, int64_t b, int64_t i, int head) {
@@ -426,8 +429,9 @@ __device__ __forceinline__ void arrived() {
 // Every head of every pass reads the mask of a row; as floats that was most of the bytes of small heads.  Read once, it becomes 64 entries
 // a word, along the rows and along the columns: {attended, attended with a bias other than 0}.  Hard masks need the first only; where a tile has a
 // bit in the second, the kernels read the floats too.
-__global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_t bias_batch, int64_t bias_row, int Nq, int Nk, ulonglong2 *row_words, ulonglong2 *col_words) {
+__global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_t bias_batch, int64_t bias_row, int Nq, int Nk, ulonglong2 *row_words, ulonglong2 *col_words, int32_t *counts) {
     __shared__ uint16_t part[2][4][64];
+    __shared__ int count[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rw = (Nk + 63) / 64, cw = (Nq + 63) / 64;
     const uint32_t tj = blockIdx.x % rw, ti = blockIdx.x / rw % cw;
@@ -435,6 +439,7 @@ __global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_
     const int j = tj * 64 + lane;
     const float *p = bias + b * bias_batch + j;
     uint32_t seen = 0, soft = 0;
+    int entries = 0;
     float v[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -447,18 +452,32 @@ __global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_
         const bool a = v[r] > kAttended, s = a && v[r] != 0.f;
         const uint64_t wa = __ballot(a), ws = __ballot(s);
         if (lane == 0 && i < Nq) row_words[(b * Nq + i) * rw + tj] = make_ulonglong2(wa, ws);
+        entries += __popcll(wa);
         seen |= (uint32_t)a << r;
         soft |= (uint32_t)s << r;
     }
     part[0][wave][lane] = (uint16_t)seen;
     part[1][wave][lane] = (uint16_t)soft;
+    if (lane == 0) count[wave] = entries;
     __syncthreads();
+    if (counts && threadIdx.x == 0) counts[blockIdx.x] = (count[0] + count[1]) + (count[2] + count[3]);
     if (wave == 0 && j < Nk) {
         uint64_t w[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) w[k] = (uint64_t)part[k][0][lane] | (uint64_t)part[k][1][lane] << 16 | (uint64_t)part[k][2][lane] << 32 | (uint64_t)part[k][3][lane] << 48;
         col_words[(b * Nk + j) * cw + ti] = make_ulonglong2(w[0], w[1]);
     }
+}
+// flags[b] = few of the mask's entries are attended
+__global__ __launch_bounds__(256) void dot_mask_count_kernel(const int32_t *counts, int per, int64_t limit, int32_t *flags) {
+    __shared__ int64_t part[4];
+    int64_t n = 0;
+    for (int i = threadIdx.x; i < per; i += 256) n += counts[(int64_t)blockIdx.x * per + i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) flags[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]) <= limit;
 }
 // the first `n` of 64 entries
 __device__ __forceinline__ uint64_t first_bits(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0 : (1ull << n) - 1); }
@@ -567,6 +586,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
+    if (MASK != kNoMask && by_entries(a, b)) return;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
     const int share = SPLIT ? ((keys + a.splits - 1) / a.splits + 63) / 64 * 64 : keys;           // of this graph's own keys
     const int j0 = SPLIT ? blk.split * share : 0, j1 = min(keys, j0 + share);
@@ -815,6 +835,7 @@ __global__ __launch_bounds__(256) void dot_join_few_kernel(DotArgs a, int64_t ro
     if (g >= groups || rr >= rows) return;
     const int r = (int)(rr % per), hk = (int)(rr / per % a.Hkv), qi = r / a.group, head = hk * a.group + r % a.group;
     const int64_t b = a.b0 + rr / per / a.Hkv;
+    if (by_entries(a, b)) return;
     const float *ml = a.part_ml + 2 * rr * a.splits, *po = a.part_o + rr * a.splits * a.D + d;
     float top = -INFINITY, sum = 0.f;
     for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[2 * s]);
@@ -838,6 +859,7 @@ __global__ __launch_bounds__(256) void dot_join_kernel(DotArgs a, int64_t rows) 
         const int64_t per = (int64_t)a.Nq * a.group;
         const int r = (int)(rr % per), hk = (int)(rr / per % a.Hkv), qi = r / a.group, head = hk * a.group + r % a.group;
         const int64_t b = a.b0 + rr / per / a.Hkv;
+        if (by_entries(a, b)) continue;
         const bool has = (int)threadIdx.x < a.splits;
         const float *ml = a.part_ml + 2 * (rr * a.splits + (has ? threadIdx.x : 0));
         const float ms = has ? ml[0] : -INFINITY, ls = has ? ml[1] : 0.f;
@@ -878,6 +900,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
+    if (MASK != kNoMask && by_entries(a, b)) return;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
     auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
     Stager<T, DP, KT, 4> rows;
@@ -1052,6 +1075,7 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 || Shape<T, DP>::TIL
     if (!blk.ok) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q4 = lane >> 4;
     const int64_t b = blk.b;
+    if (MASK != kNoMask && by_entries(a, b)) return;
     const int keys = graph_size(a.key_sizes, b, a.Nk), queries = graph_size(a.query_sizes, b, a.Nq);
     auto buf = [&](int at) { return lds + at * 2 * S::TILE; };
     const int head0 = blk.hk * a.group;
@@ -1231,6 +1255,189 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 || Shape<T, DP>::TIL
     }
 }
 
+// ---- masks with few entries ------------------------------------------------------------------------------------------------------
+// A 16 x 16 tile with one attended entry costs what a full one costs.  Where a mask has few entries they are walked one by one: a group of lanes
+// has a row (a query, or a key for dk and dv), DL lanes eight elements each of its width, WS of these sets different words of the mask; their results
+// are added in a fixed order.  Probabilities stay in fp32 for bf16, too.
+template <int DP> struct Entries {
+    static constexpr int DL = DP / 8, WS = DL <= 2 ? 4 : (DL <= 8 ? 2 : 1), LANES = DL * WS, ROWS = 256 / LANES;
+};
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int e, int D, float (&f)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+            const float4 u = e + k < D ? *reinterpret_cast<const float4 *>(p + e + k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            f[k] = u.x; f[k + 1] = u.y; f[k + 2] = u.z; f[k + 3] = u.w;
+        }
+    } else {
+        const uint4 u = e < D ? *reinterpret_cast<const uint4 *>(p + e) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f[2 * k] = __uint_as_float(w[k] << 16);
+            f[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, int e, int D, const float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k += 4)
+        if (e + k < D) store4<T>(p + e + k, (f32x4){f[k], f[k + 1], f[k + 2], f[k + 3]});
+}
+template <typename T>
+__device__ __forceinline__ const T *entry_row(const DotRows &x, int64_t b, int64_t i, int head) {
+    return reinterpret_cast<const T *>(x.p) + b * x.batch + i * x.node + head * x.head;
+}
+template <int DL>
+__device__ __forceinline__ float dot8(const float (&x)[8], const float (&y)[8]) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
+    return group_sum<DL>(s);
+}
+// each(entry, whether its bias is other than 0) for the attended ones among the first n, every WS-th word from `first` on
+template <int WS, typename F>
+__device__ __forceinline__ void walk_entries(const ulonglong2 *words, int n, int first, F each) {
+    const int count = (n + 63) / 64;
+    for (int w0 = first; w0 < count; w0 += 4 * WS) {
+        ulonglong2 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = w0 + u * WS < count ? words[w0 + u * WS] : make_ulonglong2(0, 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int base = (w0 + u * WS) * 64;
+            for (uint64_t bits = x[u].x & first_bits(n - base); bits; bits &= bits - 1) {
+                const int e = __builtin_ctzll(bits);
+                each(base + e, (x[u].y >> e & 1) != 0);
+            }
+        }
+    }
+}
+template <int DL, int LANES>
+__device__ __forceinline__ void over_sets(float (&f)[8]) {
+#pragma unroll
+    for (int o = DL; o < LANES; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] += __shfl_xor(f[k], o, 64);
+}
+
+// The heads of a query lie next to each other, among the lanes as in memory.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void dot_entries_fwd_kernel(DotArgs a, int64_t rows) {
+    using E = Entries<DP>;
+    const int e = threadIdx.x % E::DL * 8, set = threadIdx.x / E::DL % E::WS;
+    for (int64_t rr = blockIdx.x * (int64_t)E::ROWS + threadIdx.x / E::LANES; rr < rows; rr += (int64_t)gridDim.x * E::ROWS) {
+        const int64_t bi = rr / a.H, b = bi / a.Nq;
+        if (!by_entries(a, b)) continue;
+        const int head = (int)(rr - bi * a.H), hk = head / a.group, i = (int)(bi - b * a.Nq);
+        const bool live = i < graph_size(a.query_sizes, b, a.Nq);
+        float q[8], o[8] = {0.f}, m = -INFINITY, l = 0.f;
+        load8<T>(entry_row<T>(a.q, b, i, head), e, live ? a.D : 0, q);
+        walk_entries<E::WS>(a.row_words + b * a.row_words_batch + (int64_t)i * ((a.Nk + 63) / 64), live ? graph_size(a.key_sizes, b, a.Nk) : 0, set, [&](int j, bool soft) {
+            float k[8], v[8];
+            load8<T>(entry_row<T>(a.k, b, j, hk), e, a.D, k);
+            load8<T>(entry_row<T>(a.v, b, j, hk), e, a.D, v);
+            float z = dot8<E::DL>(q, k) * (a.scale * kLog2e);
+            if (soft) z = fmaf(a.bias[b * a.bias_batch + i * a.bias_row + j], kLog2e, z);
+            const float top = fmaxf(m, z), base = top == -INFINITY ? 0.f : top, shrink = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(z - base);
+            m = top;
+            l = fmaf(l, shrink, p);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) o[r] = fmaf(o[r], shrink, p * v[r]);
+        });
+        float top = m;
+#pragma unroll
+        for (int w = E::DL; w < E::LANES; w <<= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
+        const float part = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+        l *= part;
+#pragma unroll
+        for (int w = E::DL; w < E::LANES; w <<= 1) l += __shfl_xor(l, w, 64);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] *= part;
+        over_sets<E::DL, E::LANES>(o);
+        if (set != 0) continue;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o[r] = inv == 0.f ? 0.f : o[r] * inv;
+        store8<T>(reinterpret_cast<T *>(a.out) + rr * a.D, e, a.D, o);
+        if (a.lse && e == 0) a.lse[(b * a.H + head) * a.Nq + i] = inv == 0.f ? INFINITY : top + log2f(l);
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void dot_entries_q_kernel(DotArgs a, int64_t rows) {
+    using E = Entries<DP>;
+    const int e = threadIdx.x % E::DL * 8, set = threadIdx.x / E::DL % E::WS;
+    for (int64_t rr = blockIdx.x * (int64_t)E::ROWS + threadIdx.x / E::LANES; rr < rows; rr += (int64_t)gridDim.x * E::ROWS) {
+        const int64_t bi = rr / a.H, b = bi / a.Nq;
+        if (!by_entries(a, b)) continue;
+        const int head = (int)(rr - bi * a.H), hk = head / a.group, i = (int)(bi - b * a.Nq);
+        const bool live = i < graph_size(a.query_sizes, b, a.Nq);
+        const int64_t at = (b * a.H + head) * a.Nq + i;
+        float q[8], d[8], o[8], dq[8] = {0.f};
+        load8<T>(entry_row<T>(a.q, b, i, head), e, live ? a.D : 0, q);
+        load8<T>(entry_row<T>(a.d_o, b, i, head), e, live ? a.D : 0, d);
+        load8<T>(entry_row<T>(a.o, b, i, head), e, live ? a.D : 0, o);
+        const float delta = dot8<E::DL>(d, o), lse = a.lse[at];
+        walk_entries<E::WS>(a.row_words + b * a.row_words_batch + (int64_t)i * ((a.Nk + 63) / 64), live ? graph_size(a.key_sizes, b, a.Nk) : 0, set, [&](int j, bool soft) {
+            float k[8], v[8];
+            load8<T>(entry_row<T>(a.k, b, j, hk), e, a.D, k);
+            load8<T>(entry_row<T>(a.v, b, j, hk), e, a.D, v);
+            float z = dot8<E::DL>(q, k) * (a.scale * kLog2e);
+            if (soft) z = fmaf(a.bias[b * a.bias_batch + i * a.bias_row + j], kLog2e, z);
+            const float dz = __builtin_amdgcn_exp2f(z - lse) * (dot8<E::DL>(d, v) - delta);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) dq[r] = fmaf(dz, k[r], dq[r]);
+        });
+        over_sets<E::DL, E::LANES>(dq);
+        if (set != 0) continue;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) dq[r] *= a.scale;
+        store8<T>(reinterpret_cast<T *>(a.dq) + rr * a.D, e, a.D, dq);
+        if (e == 0) a.delta[at] = delta;
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void dot_entries_kv_kernel(DotArgs a, int64_t rows) {
+    using E = Entries<DP>;
+    const int e = threadIdx.x % E::DL * 8, set = threadIdx.x / E::DL % E::WS;
+    for (int64_t rr = blockIdx.x * (int64_t)E::ROWS + threadIdx.x / E::LANES; rr < rows; rr += (int64_t)gridDim.x * E::ROWS) {
+        const int64_t bj = rr / a.Hkv, b = bj / a.Nk;
+        if (!by_entries(a, b)) continue;
+        const int hk = (int)(rr - bj * a.Hkv), j = (int)(bj - b * a.Nk);
+        const bool live = j < graph_size(a.key_sizes, b, a.Nk);
+        float k[8], v[8], dk[8] = {0.f}, dv[8] = {0.f};
+        load8<T>(entry_row<T>(a.k, b, j, hk), e, live ? a.D : 0, k);
+        load8<T>(entry_row<T>(a.v, b, j, hk), e, live ? a.D : 0, v);
+        walk_entries<E::WS>(a.col_words + b * a.col_words_batch + (int64_t)j * ((a.Nq + 63) / 64), live ? graph_size(a.query_sizes, b, a.Nq) : 0, set, [&](int i, bool soft) {
+            const float bias = soft ? a.bias[b * a.bias_batch + i * a.bias_row + j] * kLog2e : 0.f;
+            for (int g = 0; g < a.group; ++g) {
+                const int head = hk * a.group + g;
+                const int64_t at = (b * a.H + head) * a.Nq + i;
+                float q[8], d[8];
+                load8<T>(entry_row<T>(a.q, b, i, head), e, a.D, q);
+                load8<T>(entry_row<T>(a.d_o, b, i, head), e, a.D, d);
+                const float p = __builtin_amdgcn_exp2f(fmaf(dot8<E::DL>(q, k), a.scale * kLog2e, bias) - a.lse[at]), dz = p * (dot8<E::DL>(d, v) - a.delta[at]);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    dk[r] = fmaf(dz, q[r], dk[r]);
+                    dv[r] = fmaf(p, d[r], dv[r]);
+                }
+            }
+        });
+        over_sets<E::DL, E::LANES>(dk);
+        over_sets<E::DL, E::LANES>(dv);
+        if (set != 0) continue;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) dk[r] *= a.scale;
+        store8<T>(reinterpret_cast<T *>(a.dk) + rr * a.D, e, a.D, dk);
+        store8<T>(reinterpret_cast<T *>(a.dv) + rr * a.D, e, a.D, dv);
+    }
+}
+
 // ---- rows of three parts -------------------------------------------------------------------------------------------------------
 struct SplitArgs {
     DotRows x[3];                       // fp32 rows of up to three tensors, one to a blockIdx.y
@@ -1334,32 +1541,48 @@ static int dot_launch(const char *what, K kernel, const DotArgs &a, size_t lds, 
 
 using namespace gatmi;
 
-// floats that hold the words of `graphs` masks: rows, then columns
+// Masks of fewer entries than this are never walked entry by entry: finding out and the idle launches would cost more.
+constexpr int64_t kEntriesMask = 512 * 512;
+static bool dot_maybe_entries(int64_t Nq, int64_t Nk) { return Nq * Nk >= kEntriesMask; }
+// "Few" is one entry of 16 for fp32, of 64 for bf16.  Forward and backward in us, 16 graphs of 1024 nodes, 4 heads, tiles - entries:
+//   fp32, 8 wide: 0.2 % 168 - 39, 1.6 % 213 - 70, 6.4 % 211 - 154;  64 wide: 392 - 90, 438 - 189, 433 - 440;  128 wide: 1101 - 137, 1112 - 353, 1080 - 863
+//   bf16, 64 wide: 0.2 % 175 - 87, 1.6 % 179 - 176, 3.2 % 165 - 254;  128 wide: 290 - 105, 306 - 236, 288 - 372
+static int64_t dot_entries_share(int32_t dtype) { return dtype == GATMI_DTYPE_F32 ? 16 : 64; }
+
+// floats that hold the words of `graphs` masks (rows, then columns), with the counts and flags of large ones
 static size_t dot_mask_floats(int64_t graphs, int64_t Nq, int64_t Nk) {
-    return 4 * (size_t)graphs * ((size_t)Nq * ((Nk + 63) / 64) + (size_t)Nk * ((Nq + 63) / 64));
+    const size_t rw = (Nk + 63) / 64, cw = (Nq + 63) / 64;
+    return (size_t)graphs * (4 * (Nq * rw + Nk * cw) + (dot_maybe_entries(Nq, Nk) ? rw * cw + 1 : 0));
 }
 
 // builds the words of the mask of one call (graphs: B, or 1 where all share it) and points `a` at them
-static int dot_mask_words(const char *what, DotArgs *a, int64_t graphs, float *words, bool build, hipStream_t st) {
+static int dot_mask_words(const char *what, DotArgs *a, int64_t graphs, float *words, int32_t dtype, bool build, hipStream_t st) {
     GATMI_REQUIRE(words, GATMI_EINVAL, "%s: mask words are null", what);
     GATMI_REQUIRE_ALIGNED(words);
     const int64_t rw = (a->Nk + 63) / 64, cw = (a->Nq + 63) / 64, per = rw * cw;
     ulonglong2 *rows = reinterpret_cast<ulonglong2 *>(words), *cols = rows + graphs * a->Nq * rw;
+    int32_t *counts = dot_maybe_entries(a->Nq, a->Nk) ? reinterpret_cast<int32_t *>(cols + graphs * a->Nk * cw) : nullptr, *flags = counts + (counts ? graphs * per : 0);
     a->row_words = rows;
     a->col_words = cols;
     a->row_words_batch = graphs > 1 ? a->Nq * rw : 0;
     a->col_words_batch = graphs > 1 ? a->Nk * cw : 0;
+    a->sparse = flags;
+    a->sparse_batch = graphs > 1;
     if (!build) return GATMI_OK;
     GATMI_REQUIRE(per <= kDotBlocks, GATMI_ERANGE, "%s: a mask of %d x %d", what, a->Nq, a->Nk);
     const int64_t step = std::max<int64_t>(1, kDotBlocks / per);
     for (int64_t b0 = 0; b0 < graphs; b0 += step) {
         const int64_t now = std::min(step, graphs - b0);
+        int32_t *count = counts ? counts + b0 * per : nullptr;
         hipLaunchKernelGGL(dot_mask_kernel, dim3((unsigned)(now * per)), dim3(256), 0, st, a->bias + b0 * a->bias_batch, a->bias_batch, a->bias_row, a->Nq, a->Nk,
-                           rows + b0 * a->Nq * rw, cols + b0 * a->Nk * cw);
+                           rows + b0 * a->Nq * rw, cols + b0 * a->Nk * cw, count);
+        if (counts) hipLaunchKernelGGL(dot_mask_count_kernel, dim3((unsigned)now), dim3(256), 0, st, count, (int)per, (int64_t)a->Nq * a->Nk / dot_entries_share(dtype), flags + b0);
     }
     GATMI_LAUNCH_CHECK("dot_attn (mask)");
     return GATMI_OK;
 }
+template <int DP>
+static dim3 dot_entries_grid(int64_t rows) { return dim3((unsigned)std::min<int64_t>(4096, (rows + Entries<DP>::ROWS - 1) / Entries<DP>::ROWS)); }
 
 // whether the passes read the mask as words: more than one wave of rows walks it
 static bool dot_wants_words(int64_t rows) { return rows > 16; }
@@ -1407,6 +1630,7 @@ template <typename T, int DP>
 static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
     using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
+    if (a.sparse) hipLaunchKernelGGL((dot_entries_fwd_kernel<Elem<T>, DP>), dot_entries_grid<DP>(B * a.Nq * a.H), dim3(256), 0, st, a, B * a.Nq * a.H);
     if constexpr (kSplit<T>) {
         DotRows r[3];
         dot_part_rows<DP>(a, B, planes, r);
@@ -1511,7 +1735,7 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (a.bias && (mask_words || dot_wants_words(rows)))
-        if (int rc = dot_mask_words("dot_attn_fwd", &a, bias_batch ? B : 1, mask_words, true, st)) return rc;
+        if (int rc = dot_mask_words("dot_attn_fwd", &a, bias_batch ? B : 1, mask_words, dtype, true, st)) return rc;
     GATMI_REQUIRE_ALIGNED(planes);
 #define RUN(T, dp) dot_fwd_run<T, dp>(a, B, planes, st)
     GATMI_DOT_DISPATCH(RUN, planes && dot_splits_parts(dtype, rows, Nk, D, lse != nullptr))
@@ -1522,6 +1746,10 @@ template <typename T, int DP>
 static int dot_bwd_run(DotArgs a, int64_t B, float *planes, float *ws, hipStream_t st) {
     using S = Shape<T, DP>;
     const int64_t rows = (int64_t)a.Nq * a.group;
+    if (a.sparse) {
+        hipLaunchKernelGGL((dot_entries_q_kernel<Elem<T>, DP>), dot_entries_grid<DP>(B * a.Nq * a.H), dim3(256), 0, st, a, B * a.Nq * a.H);
+        hipLaunchKernelGGL((dot_entries_kv_kernel<Elem<T>, DP>), dot_entries_grid<DP>(B * a.Nk * a.Hkv), dim3(256), 0, st, a, B * a.Nk * a.Hkv);
+    }
     if constexpr (kSplit<T>) {                                          // q, k, v as the forward left them; dout now, with delta
         DotRows r[3];
         dot_part_rows<DP>(a, B, planes, r);
@@ -1598,7 +1826,7 @@ extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     if (a.bias)
-        if (int rc = dot_mask_words("dot_attn_bwd", &a, bias_batch ? B : 1, mask_words, false, st)) return rc;
+        if (int rc = dot_mask_words("dot_attn_bwd", &a, bias_batch ? B : 1, mask_words, dtype, false, st)) return rc;
     const bool parts = planes && dot_splits_parts(dtype, (int64_t)Nq * a.group, Nk, D, true);
     GATMI_REQUIRE(!parts || ws, GATMI_EINVAL, "dot_attn_bwd: workspace is null");
     GATMI_REQUIRE_ALIGNED(planes);

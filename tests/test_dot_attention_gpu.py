@@ -94,6 +94,48 @@ def test_padded_graphs(Nq, Nk, density, dtype):
     _check(_case(5, Nq, Nk, 4, 2, 24, dtype, density=density, sizes=True, seed=Nk), dtype)
 
 
+# masks of 512 x 512 entries and more with at most one in 16 (fp32) or 64 (bf16) attended: walked entry by entry
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,Nq,Nk,H,G", [(8, 600, 600, 4, 4), (8, 4200, 90, 2, 1), (12, 513, 700, 4, 2), (16, 520, 520, 6, 2), (32, 512, 512, 2, 2), (40, 700, 512, 2, 1),
+                                         (64, 600, 600, 3, 3), (100, 520, 530, 2, 1), (128, 512, 600, 2, 2)])
+@pytest.mark.parametrize("density,soft,sizes,shared", [(0.004, False, False, False), (0.002, True, True, False), (0.01, True, False, True)])
+def test_masks_of_few_entries(D, Nq, Nk, H, G, density, soft, sizes, shared, dtype):
+    _check(_case(3 if sizes else 2, Nq, Nk, H, G, D, dtype, density=density, soft=soft, sizes=sizes, shared_mask=shared, seed=D), dtype, what="%d wide" % D)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("entries", [0, 1, 4095, 4096, 4097, 16383, 16384, 16385, 512 * 512])
+def test_few_entries_or_many(entries, dtype):
+    """On both sides of one entry in 64 (bf16) and in 16 (fp32), two graphs of different kinds in one batch."""
+    c = _case(2, 512, 512, 2, 2, 16, dtype, seed=entries)
+    rng = np.random.default_rng(entries)
+    bm = np.full((2, 512 * 512), -1e9)
+    bm[0, rng.permutation(512 * 512)[:entries]] = 0.0
+    bm[1, rng.permutation(512 * 512)[:20000]] = 0.0
+    c["bias"] = torch.tensor(bm.reshape(2, 512, 512), dtype=torch.float32, device="cuda:0")
+    _check(c, dtype)
+    c["q"], c["dout"] = c["q"][:, :3].contiguous(), c["dout"][:, :3].contiguous()
+    c["bias"] = c["bias"][:, :3].contiguous()
+    _check(c, dtype)
+
+
+def test_few_entries_of_few_rows():
+    """One query on 262144 keys with gradients: the mask is large though it has one row."""
+    _check(_case(1, 1, 1 << 18, 2, 1, 8, "f32", density=0.001, seed=1), "f32")
+    _check(_case(1, 1, 1 << 18, 2, 1, 8, "f32", density=0.001, seed=1), "f32", grad=False)
+
+
+def test_few_entries_captured_twice_the_same_and_not_finite_where_masked():
+    c = _case(2, 600, 600, 2, 2, 16, "f32", density=0.003, seed=2)
+    never = (c["bias"] < -1e8).all(1)[0]                                 # keys that no query of the first graph attends
+    want = _run(c)
+    for n in ("k", "v"):
+        c[n] = c[n].clone()
+        c[n][0, never] = float("nan")
+    again = _run(c)
+    assert torch.equal(want["out"], again["out"]) and torch.equal(want["dq"], again["dq"]) and torch.equal(want["dv"][:, ~never], again["dv"][:, ~never])
+
+
 # many rows of fp32 wider than 16: computed as three parts (for the gradients from 97 rows and keys on, 193 above 64 wide; alone from 257 and 769)
 @pytest.mark.parametrize("D,Nq,Nk,H,G", [(20, 97, 97, 2, 2), (32, 97, 130, 2, 2), (32, 50, 200, 4, 2), (40, 129, 97, 2, 1), (64, 200, 128, 2, 2), (64, 192, 97, 3, 1),
                                          (96, 193, 193, 1, 1), (100, 97, 257, 2, 1), (128, 260, 193, 1, 1), (128, 321, 200, 2, 2)])
