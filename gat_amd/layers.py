@@ -359,7 +359,7 @@ class DotHeads(nn.Module):
         rows = ops.tall_linear(seq, self.W.reshape(F, -1).t()).reshape(B, N, H + 2 * G, D)
         if self.storage == "bf16":
             rows = rows.to(torch.bfloat16)
-        q, k, v = rows[:, :, :H], rows[:, :, H:H + G], rows[:, :, H + G:]
+        q, k, v = rows.split((H, G, G), 2)
         out = ops.dot_attention(q, k, v, bias_mat, key_sizes=sizes, query_sizes=sizes).to(seq.dtype).reshape(B, N, H * D)
         if self.has_res:
             out = out + ops.tall_linear(seq, self.W_res.reshape(F, -1).t(), self.b_res.reshape(-1))

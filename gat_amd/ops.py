@@ -952,6 +952,7 @@ class DotAttentionFn(torch.autograd.Function):
         return out[..., :D] if out.shape[3] != D else out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         qr, kr, vr, out, lse, bias, words, planes, key_sizes, query_sizes = ctx.saved_tensors
         B, Nq, H, width = qr.shape
@@ -1041,6 +1042,7 @@ class EmbeddingFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
         n, rows, width = flat.numel(), ctx.rows, dout.shape[-1]

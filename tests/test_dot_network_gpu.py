@@ -171,3 +171,40 @@ def test_dot_attn_head_uses_the_variable_store():
     p = {n: q.detach().double().cpu() for n, q in m.named_parameters()}
     ref = _heads_ref(m, p, x.double().cpu(), d["bias"].double().cpu(), torch.ones((B, N), dtype=torch.bool), "identity", True)
     assert_close(b.detach().cpu().numpy(), ref.numpy(), rtol=1e-4, atol_scale=1e-5)
+
+
+def test_two_streams_at_once():
+    """Calls of every kind on two streams without a wait between them, each with workspaces of its own."""
+    from gat_amd import ops
+    g = torch.Generator(device="cuda:0").manual_seed(1)
+    r = lambda *s: torch.randn(*s, device="cuda:0", generator=g)
+    q, k, v, ids, table, x = r(2, 600, 4, 32), r(2, 600, 4, 32), r(2, 600, 4, 32), torch.randint(0, 50, (9000,), device="cuda:0", generator=g), r(50, 24), r(2, 300, 2100)
+    bias = torch.where(r(2, 600, 600) > 1.0, 0.0, -1e9)
+
+    def work():
+        a = [t.detach().requires_grad_() for t in (q, k, v, table)]
+        o, e = ops.dot_attention(a[0], a[1], a[2], bias), ops.embedding(ids, a[3])
+        return [o.detach(), e.detach(), ops.newton_schulz(x), *torch.autograd.grad(o, a[:3], q), *torch.autograd.grad(e, a[3], e.detach())]
+    want = work()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for res in got:
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    from gat_amd import ops
+    q = torch.randn(1, 5, 1, 8, device="cuda:0", requires_grad=True)
+    (first,) = torch.autograd.grad(ops.dot_attention(q, q.detach(), q.detach()).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), q)
+    table = torch.randn(4, 8, device="cuda:0", requires_grad=True)
+    (first,) = torch.autograd.grad((ops.embedding(torch.tensor([1, 2], device="cuda:0"), table) ** 2).sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), table)
