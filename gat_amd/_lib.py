@@ -102,8 +102,8 @@ _SIGNATURES = {
     "gatmi_dot_attn_bwd_ws_floats": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "gatmi_dot_attn_fwd_ws_floats": (c_size_t, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "gatmi_dot_attn_fwd": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, c_int64, c_int64, P, P, c_float,
-                                   P, P, P, P, P, P]),
-    "gatmi_dot_attn_bwd": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, P, P, P, P, c_int64, c_int64, P, P,
+                                   P, P, P, P, P, P, P]),
+    "gatmi_dot_attn_bwd": (c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, P, P, P, P, P, P, P, P, P, P, P, P, c_int64, c_int64, P, P,
                                    c_float, P, P, P, P, P, P, P, P]),
     "gatmi_embed_fwd": (c_int, [P, c_int32, c_int64, P, c_int64, c_int64, c_int32, c_int32, c_float, P, P]),
     "gatmi_embed_bwd_ws_floats": (c_size_t, [c_int64, c_int64, c_int32]),

@@ -15,12 +15,13 @@
 //
 // Matrix instructions: v_mfma_f32_16x16x4_f32 and v_mfma_f32_16x16x32_bf16, sums in fp32.  The scores are formed transposed (keys down, queries
 // across the lanes): a lane then holds four consecutive keys of ONE query, the softmax statistics are one register each,
-// and the probabilities sit in the operand layout of the second product as they are: they never go through LDS.  bf16 rounds P and
-// dz to bf16 for that product (half a step of 2^-8, as its other operand has and its result is stored with).
+// and the probabilities sit in the operand layout of the second product as they are: they never go through LDS.  For that
+// product bf16 rows have P and dz as two bf16 each, high and low (Wide16), or, of many rows without a mask, rounded to one (uint16_t: half a step of 2^-8, as its
+// other operand has and its result is stored with).
 //
 // A mask with few entries is walked entry by entry (dot_entries_*), a denser one in tiles, without the 16 x 16 parts that it leaves empty.
 //
-// What the tiles measure, forward / dq / dk, dv: 4 graphs of 2048 to 4096 nodes, 16 heads on 4 of 128, bf16: 500 / 650 / 1149 us, 618 / 714 / 538
+// What the tiles measure, forward / dq / dk, dv: 4 graphs of 2048 to 4096 nodes, 16 heads on 4 of 128, bf16: 520 / 655 / 1180 us, 594 / 708 / 524
 // TFLOP/s of products (a large bf16 product reaches 1140): the matrix instructions wait for LDS reads, most of all in dk, dv with
 // two operands that are read column-wise.  16 x 1024 nodes, 4 heads of 64, fp32: 92 / 121 / 164 us, 187 / 213 / 210 TFLOP/s of fp32 accuracy (a
 // large fp32 product: 153).  1024 graphs of 246 nodes, 8 heads of 8, 10 % attended: 375 / 419 / 589 us for 2 / 3 / 4 products of 8 wide operands each:
@@ -67,8 +68,10 @@ constexpr int kSplitsMax = 256;
 // A fragment is what a lane holds of 16 rows x KD elements: lane (n = l & 15, q = l >> 4) the PIECE bytes at q * PIECE of the
 // fragment's part of row n.
 struct Split3 {};                                        // fp32 as three bf16
+struct Wide16 {};                                        // bf16, P and dz as two bf16
 template <typename T> struct ElemOf { using type = T; };
 template <> struct ElemOf<Split3> { using type = float; };
+template <> struct ElemOf<Wide16> { using type = uint16_t; };
 template <typename T> using Elem = typename ElemOf<T>::type;              // what results are stored as
 template <typename T> constexpr bool kSplit = std::is_same_v<T, Split3>;
 
@@ -84,7 +87,7 @@ template <typename T, int DP> struct Shape {
     static constexpr int PLANE = KT * ROW, TILE = PLANE;
     // 16-row tiles of a wave: two where the accumulators and operands of two fit the 256 registers that leave two waves on a SIMD
     static constexpr int NQ = SIZE == 4 && DP >= 64 ? 1 : 2;
-    static constexpr int nk(bool masked) { return (SIZE == 4 && DP >= 64) || (DP == 128 && masked) ? 1 : 2; }
+    static constexpr int nk(bool) { return SIZE == 4 && DP >= 64 ? 1 : 2; }
     __device__ static __forceinline__ int swizzle(int r) {      // the same for r and r + 16
         if constexpr (CPR >= 16) return r & 15;
         else return (r / (16 / CPR)) & (CPR - 1);
@@ -100,16 +103,23 @@ template <int DP> struct Shape<Split3, DP> : Shape<uint16_t, DP> {
     static constexpr int nk(bool masked) { return DP == 32 || (DP == 128 && !masked) ? 2 : 1; }
 };
 
+template <int DP> struct Shape<Wide16, DP> : Shape<uint16_t, DP> {
+    static constexpr int NQ = DP == 128 ? 1 : 2;
+    static constexpr int nk(bool masked) { return DP == 128 || (DP == 64 && masked) ? 1 : 2; }
+};
+
 struct FragF { float v[4]; };
 struct FragH { uint4 v; };
 template <typename T> struct FragOf;
 template <> struct FragOf<float> { using type = FragF; };
 template <> struct FragOf<uint16_t> { using type = FragH; };
 template <> struct FragOf<Split3> { using type = FragH; };
+template <> struct FragOf<Wide16> { using type = FragH; };
 template <typename T> using Frag = typename FragOf<T>::type;
 // operands of the second product: one fragment, or one of each part
 template <typename T> struct ManyOf { Frag<T> p[1]; };
 template <> struct ManyOf<Split3> { FragH p[3]; };
+template <> struct ManyOf<Wide16> { FragH p[2]; };
 
 template <typename T, int DP>
 __device__ __forceinline__ Frag<T> frag_load(const char *p) {
@@ -204,6 +214,15 @@ template <typename T>
 __device__ __forceinline__ ManyOf<T> frag_scores(const f32x4 *tile) {
     if constexpr (std::is_same_v<T, float>) {
         return {FragF{{tile[0][0], tile[0][1], tile[0][2], tile[0][3]}}};
+    } else if constexpr (std::is_same_v<T, Wide16>) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = tile[i >> 1][2 * (i & 1)], y = tile[i >> 1][2 * (i & 1) + 1];
+            h[i] = pack_bf16x2(x, y);
+            l[i] = pack_bf16x2(x - __uint_as_float(h[i] << 16), y - __uint_as_float(h[i] & 0xffff0000u));
+        }
+        return {FragH{make_uint4(h[0], h[1], h[2], h[3])}, FragH{make_uint4(l[0], l[1], l[2], l[3])}};
     } else if constexpr (!kSplit<T>) {
         return {FragH{make_uint4(pack_bf16x2(tile[0][0], tile[0][1]), pack_bf16x2(tile[0][2], tile[0][3]), pack_bf16x2(tile[1][0], tile[1][1]), pack_bf16x2(tile[1][2], tile[1][3]))}};
     } else {
@@ -249,7 +268,10 @@ __device__ __forceinline__ void mma_rows(const ManyOf<T> &a, const ManyOf<T> (&b
     if constexpr (!kSplit<T>) {
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (use[u]) mma<T, 64>(a.p[0], b[u].p[0], *acc[u]);
+            if (use[u]) {
+                if constexpr (std::is_same_v<T, Wide16>) mma<T, 64>(a.p[0], b[u].p[1], *acc[u]);
+                mma<T, 64>(a.p[0], b[u].p[0], *acc[u]);
+            }
     } else {
 #pragma unroll
         for (int u = 0; u < N; ++u)
@@ -303,6 +325,7 @@ struct DotRows {              // [B, N, heads, D] rows: element strides, D conti
 struct DotArgs {
     DotRows q, k, v, o, d_o;
     void *out, *dq, *dk, *dv;           // contiguous [B, N, heads, D]
+    uint16_t *out_low;                  // what rounding to bf16 took from out, rows as it; or null
     float *lse, *delta;                 // [B, H, Nq]: log2 of the row's sum of exponentials; <do, out>
     const float *bias;
     int64_t bias_batch, bias_row;
@@ -581,6 +604,12 @@ __device__ __forceinline__ void store4(T *p, f32x4 v) {
     else *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
+// what rounding to bf16 takes from v
+__device__ __forceinline__ f32x4 low_part(f32x4 v) {
+    const uint32_t a = pack_bf16x2(v[0], v[1]), b = pack_bf16x2(v[2], v[3]);
+    return (f32x4){v[0] - __uint_as_float(a << 16), v[1] - __uint_as_float(a & 0xffff0000u), v[2] - __uint_as_float(b << 16), v[3] - __uint_as_float(b & 0xffff0000u)};
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------
 // A wave owns NQ x 16 rows.  KEYW = false: four waves with rows of their own walk the staged tiles together.  KEYW = true: for 16 rows or
 // fewer, the four waves have the same rows and walk different tiles, each staging its own, and join at the end.
@@ -811,7 +840,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot
             }
         } else {
             const float inv = !live[u] || sum[u] == 0.f ? 0.f : 1.0f / sum[u];
-            Elem<T> *orow = reinterpret_cast<Elem<T> *>(a.out) + ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
+            const int64_t oat = ((b * a.Nq + qi[u]) * a.H + head[u]) * (int64_t)a.D;
+            Elem<T> *orow = reinterpret_cast<Elem<T> *>(a.out) + oat;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
                 if (16 * t + 4 * q4 < a.D) {
@@ -819,6 +849,8 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = inv == 0.f ? 0.f : v[r] * inv;
                     store4<Elem<T>>(orow + 16 * t + 4 * q4, v);
+                    if constexpr (S::SIZE == 2 && !kSplit<T>)
+                        if (a.out_low) store4<uint16_t>(a.out_low + oat + 16 * t + 4 * q4, low_part(v));
                 }
             if (a.lse && q4 == 0) a.lse[(b * a.H + head[u]) * a.Nq + qi[u]] = inv == 0.f ? INFINITY : m[u] + log2f(sum[u]);
         }
@@ -832,7 +864,10 @@ __device__ __forceinline__ void store_joined(const DotArgs &a, int64_t b, int qi
     f32x4 v = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = inv == 0.f ? 0.f : v[k] * inv;
-    store4<Elem<T>>(reinterpret_cast<Elem<T> *>(a.out) + ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d, v);
+    const int64_t at = ((b * a.Nq + qi) * a.H + head) * (int64_t)a.D + d;
+    store4<T>(reinterpret_cast<T *>(a.out) + at, v);
+    if constexpr (sizeof(T) == 2)
+        if (a.out_low) store4<uint16_t>(a.out_low + at, low_part(v));
     if (a.lse && d == 0) a.lse[(b * a.H + head) * a.Nq + qi] = inv == 0.f ? INFINITY : top + log2f(sum);
 }
 
@@ -948,6 +983,21 @@ __global__ __launch_bounds__(256, (Shape<T, DP>::TILE > 20480 ? 1 : 2)) void dot
                     for (int t = 0; t < S::ELEMS / 2; ++t) {
                         dot = fmaf(__uint_as_float(x[t] << 16), __uint_as_float(y[t] << 16), dot);
                         dot = fmaf(__uint_as_float(x[t] & 0xffff0000u), __uint_as_float(y[t] & 0xffff0000u), dot);
+                    }
+                }
+            }
+            if constexpr (S::SIZE == 2) {
+                if (a.out_low) {                                             // rows as those of out
+                    Frag<T> low[S::FRAGS];
+                    row_frags<T, DP>(row_of<S>(DotRows{a.out_low, a.o.batch, a.o.node, a.o.head}, b, i, head[u]), a.D, live, low);
+#pragma unroll
+                    for (int c = 0; c < S::FRAGS; ++c) {
+                        const uint32_t x[4] = {df[u][c].v.x, df[u][c].v.y, df[u][c].v.z, df[u][c].v.w}, y[4] = {low[c].v.x, low[c].v.y, low[c].v.z, low[c].v.w};
+#pragma unroll
+                        for (int t = 0; t < S::ELEMS / 2; ++t) {
+                            dot = fmaf(__uint_as_float(x[t] << 16), __uint_as_float(y[t] << 16), dot);
+                            dot = fmaf(__uint_as_float(x[t] & 0xffff0000u), __uint_as_float(y[t] & 0xffff0000u), dot);
+                        }
                     }
                 }
             }
@@ -1372,6 +1422,12 @@ __global__ __launch_bounds__(256) void dot_entries_fwd_kernel(DotArgs a, int64_t
 #pragma unroll
         for (int r = 0; r < 8; ++r) o[r] = inv == 0.f ? 0.f : o[r] * inv;
         store8<T>(reinterpret_cast<T *>(a.out) + rr * a.D, e, a.D, o);
+        if constexpr (sizeof(T) == 2)
+            if (a.out_low) {
+#pragma unroll
+                for (int r = 0; r < 8; r += 4)
+                    if (e < a.D) store4<uint16_t>(a.out_low + rr * a.D + e + r, low_part((f32x4){o[r], o[r + 1], o[r + 2], o[r + 3]}));
+            }
         if (a.lse && e == 0) a.lse[(b * a.H + head) * a.Nq + i] = inv == 0.f ? INFINITY : top + log2f(l);
     }
 }
@@ -1390,6 +1446,13 @@ __global__ __launch_bounds__(256) void dot_entries_q_kernel(DotArgs a, int64_t r
         load8<T>(entry_row<T>(a.q, b, i, head), e, live ? a.D : 0, q);
         load8<T>(entry_row<T>(a.d_o, b, i, head), e, live ? a.D : 0, d);
         load8<T>(entry_row<T>(a.o, b, i, head), e, live ? a.D : 0, o);
+        if constexpr (sizeof(T) == 2)
+            if (a.out_low) {
+                float low[8];
+                load8<T>(a.out_low + rr * a.D, e, live ? a.D : 0, low);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) o[r] += low[r];
+            }
         const float delta = dot8<E::DL>(d, o), lse = a.lse[at];
         walk_entries<E::WS>(a.row_words + b * a.row_words_batch + (int64_t)i * ((a.Nk + 63) / 64), live ? graph_size(a.key_sizes, b, a.Nk) : 0, set, [&](int j, bool soft) {
             float k[8], v[8];
@@ -1658,7 +1721,8 @@ static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
         a.q = r[0]; a.k = r[1]; a.v = r[2];
     }
     constexpr int NQ = S::NQ;
-    const int per = rows <= 16 && !kSplit<T> ? 16 : (rows <= 64 ? 64 : 64 * NQ);
+    constexpr bool COARSE = std::is_same_v<T, uint16_t>, FEW = !kSplit<T> && !COARSE;       // without a mask only; 64 rows or fewer come here
+    const int per = rows <= 16 && FEW ? 16 : (rows <= 64 ? 64 : 64 * NQ);
     a.tiles = (int)((rows + per - 1) / per);
     const int64_t step = a.splits > 1 ? B : dot_graphs(a);              // split launches are small by construction
     const size_t lds = 4 * S::TILE, lds_keyw = std::max<size_t>(16 * S::KTW * S::ROW, 512 + 4 * S::DT * 1024);
@@ -1667,12 +1731,12 @@ static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
         a.B = (int)std::min(step, B - b0);
         int rc = GATMI_OK;
 #define RUN(keyw, nq, split, bytes)                                                                                                      \
-    (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, keyw ? kFloats : kBits>, a, bytes, st)                   \
+    (a.bias ? dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, COARSE ? kNoMask : (keyw ? kFloats : kBits)>, a, bytes, st) \
             : dot_launch("dot_attn_fwd", dot_fwd_kernel<T, DP, keyw, nq, split, kNoMask>, a, bytes, st))
         if (per == 16) {
-            if constexpr (!kSplit<T>) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
+            if constexpr (FEW) rc = a.splits > 1 ? RUN(true, 1, true, lds_keyw) : RUN(true, 1, false, lds_keyw);
         } else if (per == 64) {
-            if constexpr (!kSplit<T>) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);          // parts: more rows than that
+            if constexpr (FEW) rc = a.splits > 1 ? RUN(false, 1, true, lds) : RUN(false, 1, false, lds);
         } else {
             if constexpr (NQ > 1) rc = a.splits > 1 ? RUN(false, NQ, true, lds) : RUN(false, NQ, false, lds);
         }
@@ -1690,6 +1754,12 @@ static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
     return GATMI_OK;
 }
 
+// bf16: whether P and dz are two numbers each.  Their rounding adds as much to the results' error as the rounding of the results; a mask adds up over
+// fewer entries, where it shows more (dq of 2 % masks is 1.5 times as far off as its own rounding), so masks have two.  Without a mask the second
+// number is cheap up to 1024 nodes and dear beyond; forward and backward, one - two numbers, in us: 16 x 1025 - 16 x 1024 nodes, 4 heads of 64: 157 - 155, of
+// 128: 345 - 310; 4 x 4096 nodes, 16 heads of 64: 1388 - 1879, of 128: 2868 - 4315.
+static bool dot_wide16(int64_t rows, int64_t Nq, int64_t Nk, bool mask) { return mask || rows <= 64 || Nk <= 64 || std::max(Nq, Nk) <= 1024; }
+
 #define GATMI_DOT_DISPATCH(RUN, parts)                                                             \
     if (dtype == GATMI_DTYPE_F32 && (parts)) {                                                     \
         if (D <= 32) return RUN(Split3, 32);                                                       \
@@ -1702,6 +1772,12 @@ static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
         if (D <= 32) return RUN(float, 32);                                                        \
         if (D <= 64) return RUN(float, 64);                                                        \
         return RUN(float, 128);                                                                    \
+    }                                                                                              \
+    if (dot_wide16((int64_t)Nq * (H / Hkv), Nq, Nk, bias != nullptr)) {                                             \
+        if (D <= 16) return RUN(Wide16, 16);                                                       \
+        if (D <= 32) return RUN(Wide16, 32);                                                       \
+        if (D <= 64) return RUN(Wide16, 64);                                                       \
+        return RUN(Wide16, 128);                                                                   \
     }                                                                                              \
     if (D <= 16) return RUN(uint16_t, 16);                                                         \
     if (D <= 32) return RUN(uint16_t, 32);                                                         \
@@ -1719,7 +1795,7 @@ extern "C" size_t gatmi_dot_attn_bwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk
 
 extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
                                   const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const float *bias, int64_t bias_batch,
-                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse, float *mask_words, float *planes, float *ws, void *stream) {
+                                  int64_t bias_row, const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, void *out_low, float *lse, float *mask_words, float *planes, float *ws, void *stream) {
     if (int rc = dot_check("dot_attn_fwd", B, Nq, Nk, H, Hkv, D, dtype)) return rc;
     GATMI_REQUIRE(std::isfinite(scale), GATMI_EINVAL, "dot_attn_fwd: scale %g", (double)scale);
     if (B == 0 || Nq == 0) return GATMI_OK;
@@ -1732,7 +1808,9 @@ extern "C" int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
     GATMI_REQUIRE(out, GATMI_EINVAL, "dot_attn_fwd: out is null");
     GATMI_REQUIRE_ALIGNED(out);
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq == 1, GATMI_EINVAL, "dot_attn_fwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
-    a.out = out; a.lse = lse; a.bias = Nk > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
+    GATMI_REQUIRE(!out_low || dtype == GATMI_DTYPE_BF16, GATMI_EINVAL, "dot_attn_fwd: out_low is for bf16");
+    GATMI_REQUIRE_ALIGNED(out_low);
+    a.out = out; a.out_low = static_cast<uint16_t *>(out_low); a.lse = lse; a.bias = Nk > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
     a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);      // above 0: -inf stays -inf
     a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hkv = Hkv; a.group = H / Hkv; a.D = D;
     const int64_t rows = (int64_t)Nq * a.group;
@@ -1778,6 +1856,8 @@ static int dot_bwd_run(DotArgs a, int64_t B, float *planes, float *ws, hipStream
     }
     a.splits = 1;
     constexpr int NQ = S::NQ, NK = S::nk(false), NKM = S::nk(true);
+    constexpr bool COARSE = std::is_same_v<T, uint16_t>, FEW = !kSplit<T> && !COARSE;       // as in the forward
+    constexpr int BITS = COARSE ? kNoMask : kBits;
     for (int pass = 0; pass < 2; ++pass) {
         const int64_t count = pass == 0 ? rows : a.Nk;
         if (count == 0) continue;
@@ -1791,11 +1871,11 @@ static int dot_bwd_run(DotArgs a, int64_t B, float *planes, float *ws, hipStream
             int rc = GATMI_OK;
 #define RUN(kernel, n, mask) dot_launch("dot_attn_bwd", kernel<T, DP, n, mask>, a, 4 * S::TILE, st)
             if (pass == 0) {
-                if (wide) rc = a.bias ? RUN(dot_bwd_q_kernel, NQ, kBits) : RUN(dot_bwd_q_kernel, NQ, kNoMask);
-                else if constexpr (!kSplit<T>) rc = a.bias ? RUN(dot_bwd_q_kernel, 1, kBits) : RUN(dot_bwd_q_kernel, 1, kNoMask);
+                if (wide) rc = a.bias ? RUN(dot_bwd_q_kernel, NQ, BITS) : RUN(dot_bwd_q_kernel, NQ, kNoMask);
+                else if constexpr (FEW) rc = a.bias ? RUN(dot_bwd_q_kernel, 1, BITS) : RUN(dot_bwd_q_kernel, 1, kNoMask);
             } else {
-                if (wide) rc = a.bias ? RUN(dot_bwd_kv_kernel, NKM, kBits) : RUN(dot_bwd_kv_kernel, NK, kNoMask);
-                else if constexpr (!kSplit<T>) rc = a.bias ? RUN(dot_bwd_kv_kernel, 1, kBits) : RUN(dot_bwd_kv_kernel, 1, kNoMask);
+                if (wide) rc = a.bias ? RUN(dot_bwd_kv_kernel, (COARSE ? NK : NKM), BITS) : RUN(dot_bwd_kv_kernel, NK, kNoMask);
+                else if constexpr (FEW) rc = a.bias ? RUN(dot_bwd_kv_kernel, 1, BITS) : RUN(dot_bwd_kv_kernel, 1, kNoMask);
             }
 #undef RUN
             if (rc) return rc;
@@ -1806,7 +1886,7 @@ static int dot_bwd_run(DotArgs a, int64_t B, float *planes, float *ws, hipStream
 }
 
 extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype, const void *q, const int64_t *q_stride,
-                                  const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const void *out, const void *dout,
+                                  const void *k, const int64_t *k_stride, const void *v, const int64_t *v_stride, const void *out, const void *out_low, const void *dout,
                                   const int64_t *dout_stride, const float *lse, const float *bias, int64_t bias_batch, int64_t bias_row,
                                   const int32_t *key_sizes, const int32_t *query_sizes, float scale, float *mask_words, float *planes, void *dq, void *dk, void *dv,
                                   float *delta, float *ws, void *stream) {
@@ -1830,6 +1910,9 @@ extern "C" int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, 
         GATMI_REQUIRE_ALIGNED(dv);
     }
     GATMI_REQUIRE(!bias || bias_row >= Nk || Nq <= 1, GATMI_EINVAL, "dot_attn_bwd: bias row stride %lld below Nk = %d", (long long)bias_row, Nk);
+    GATMI_REQUIRE(!out_low || dtype == GATMI_DTYPE_BF16, GATMI_EINVAL, "dot_attn_bwd: out_low is for bf16");
+    GATMI_REQUIRE_ALIGNED(out_low);
+    a.out_low = static_cast<uint16_t *>(const_cast<void *>(out_low));
     a.dq = dq; a.dk = dk; a.dv = dv; a.lse = const_cast<float *>(lse); a.delta = delta;
     a.bias = Nk > 0 && Nq > 0 ? bias : nullptr; a.bias_batch = bias_batch; a.bias_row = bias_row;
     a.key_sizes = key_sizes; a.query_sizes = query_sizes; a.scale = scale; a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);      // above 0: -inf stays -inf

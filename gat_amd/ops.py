@@ -914,7 +914,7 @@ def _attn_rows(t, width):
 
 
 def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
-    """(rows of q, k, v as the kernels read them, out with padded width, lse or None, the mask as bits or None, fp32 rows
+    """(rows of q, k, v as the kernels read them, out with padded width, what rounding took from it or None, lse or None, the mask as bits or None, fp32 rows
     in parts or None, bias strides)"""
     B, Nq, H, D = q.shape
     Nk, Hkv = k.shape[1], k.shape[2]
@@ -925,6 +925,7 @@ def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
     qr, kr, vr = _attn_rows(q, width), _attn_rows(k, width), _attn_rows(v, width)
     out = torch.empty((B, Nq, H, width), dtype=q.dtype, device=dev)
     lse = torch.empty((B, H, Nq), dtype=torch.float32, device=dev) if need else None
+    low = torch.empty_like(out) if need and dtype == _lib.DTYPE_BF16 else None
     ws = _scratch(_lib.lib.gatmi_dot_attn_fwd_ws_floats(B, Nq, Nk, H, Hkv, width), dev)
     strides, words = (0, Nk), None
     if bias is not None:
@@ -935,9 +936,9 @@ def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
     if dtype == _lib.DTYPE_F32:
         planes = _scratch(_lib.lib.gatmi_dot_attn_planes_floats(B, Nq, Nk, H, Hkv, width, dtype, need), dev)
     _launch(dev, "gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr), vr.data_ptr(), _strides(vr),
-            ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(lse), ptr(words),
+            ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(low), ptr(lse), ptr(words),
             ptr(planes), ptr(ws))
-    return qr, kr, vr, out, lse, words, planes, strides
+    return qr, kr, vr, out, low, lse, words, planes, strides
 
 
 class DotAttentionFn(torch.autograd.Function):
@@ -946,15 +947,15 @@ class DotAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, key_sizes, query_sizes, scale):
         D = q.shape[3]
-        qr, kr, vr, out, lse, words, planes, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
-        ctx.save_for_backward(qr, kr, vr, out, lse, bias, words, planes, key_sizes, query_sizes)
+        qr, kr, vr, out, low, lse, words, planes, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
+        ctx.save_for_backward(qr, kr, vr, out, low, lse, bias, words, planes, key_sizes, query_sizes)
         ctx.scale, ctx.D, ctx.bias_strides = scale, D, strides
         return out[..., :D] if out.shape[3] != D else out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qr, kr, vr, out, lse, bias, words, planes, key_sizes, query_sizes = ctx.saved_tensors
+        qr, kr, vr, out, low, lse, bias, words, planes, key_sizes, query_sizes = ctx.saved_tensors
         B, Nq, H, width = qr.shape
         Nk, Hkv = kr.shape[1], kr.shape[2]
         D = ctx.D
@@ -963,7 +964,7 @@ class DotAttentionFn(torch.autograd.Function):
         delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
         ws = None if planes is None else _scratch(_lib.lib.gatmi_dot_attn_bwd_ws_floats(B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype]), qr.device)
         _launch(qr.device, "gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr),
-                vr.data_ptr(), _strides(vr), out.data_ptr(), dr.data_ptr(), _strides(dr), lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
+                vr.data_ptr(), _strides(vr), out.data_ptr(), ptr(low), dr.data_ptr(), _strides(dr), lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
                 ptr(query_sizes), ctx.scale, ptr(words), ptr(planes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), ptr(ws))
         if width != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]

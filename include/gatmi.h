@@ -562,11 +562,13 @@ int gatmi_ipd_bwd(int64_t B, int32_t N, int32_t F, const float *dOut, const floa
  *   attended key gives zeros.
  *   fwd: lse [B, H, Nq] (log2 of the row's sum of exponentials; NULL when no backward follows).  ws: gatmi_dot_attn_fwd_ws_floats
  *   (0: may be NULL); few rows on many keys are split over the keys and joined.
+ *   out_low: optional, bf16 only: what rounding took from out (bf16, laid out as out), written by fwd, read by the bwd of the same call:
+ *   the gradients then do not carry the rounding of out.
  *   mask_words: gatmi_dot_attn_mask_floats floats (bias_batch 0: one mask), written by fwd, read by the bwd of the same call: the mask
  *   as bits.  NULL without a bias, and for a fwd of at most 16 rows Nq * H / Hkv that no bwd follows.
  *   planes: gatmi_dot_attn_planes_floats floats (0: NULL), asked with backward = 1 for a fwd that has lse; written by fwd, read by the
  *   bwd of the same call, which gets it where its fwd did: fp32 rows as three bf16 parts each, on which many rows are computed faster at
- *   fp32 accuracy (an infinity among them gives NaN).  NULL is allowed, and slower.
+ *   fp32 accuracy (an infinity, or a number above 3.38e38, among them gives NaN).  NULL is allowed, and slower.
  *   bwd: the probabilities are formed again from lse; dq [B, Nq, H, D], dk, dv [B, Nk, Hkv, D] contiguous, written whole; delta
  *   [B, H, Nq] and ws (gatmi_dot_attn_bwd_ws_floats; planes NULL: may be NULL) are scratch.  No atomics: the same bits every run. */
 size_t gatmi_dot_attn_mask_floats(int64_t B, int32_t Nq, int32_t Nk, int64_t bias_batch);
@@ -576,11 +578,11 @@ size_t gatmi_dot_attn_fwd_ws_floats(int64_t B, int32_t Nq, int32_t Nk, int32_t H
 int gatmi_dot_attn_fwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype,
                        const void *q, const int64_t *q_stride, const void *k, const int64_t *k_stride,
                        const void *v, const int64_t *v_stride, const float *bias, int64_t bias_batch, int64_t bias_row,
-                       const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, float *lse,
+                       const int32_t *key_sizes, const int32_t *query_sizes, float scale, void *out, void *out_low, float *lse,
                        float *mask_words, float *planes, float *ws, void *stream);
 int gatmi_dot_attn_bwd(int64_t B, int32_t Nq, int32_t Nk, int32_t H, int32_t Hkv, int32_t D, int32_t dtype,
                        const void *q, const int64_t *q_stride, const void *k, const int64_t *k_stride,
-                       const void *v, const int64_t *v_stride, const void *out, const void *dout, const int64_t *dout_stride,
+                       const void *v, const int64_t *v_stride, const void *out, const void *out_low, const void *dout, const int64_t *dout_stride,
                        const float *lse, const float *bias, int64_t bias_batch, int64_t bias_row,
                        const int32_t *key_sizes, const int32_t *query_sizes, float scale, float *mask_words, float *planes,
                        void *dq, void *dk, void *dv, float *delta, float *ws, void *stream);

@@ -15,13 +15,15 @@ def attention(q, k, v, bias=None, key_sizes=None, query_sizes=None, scale=None, 
     Scores: an fp32 dot product of D terms is off by (D + 2) u32 sum |q k|; scaling, bias, the change to base 2 and the subtraction of the
     row's lse are a few more roundings of numbers no larger than |z| + |lse|.  A numerator's relative error is the absolute error of
     its exponent, the row's normalisation has at most the largest of them: rho = 2 max_j e_ij.  Sums over n terms: n u32 of the sum
-    of magnitudes.  bf16: P and dz enter the second products rounded, results and the saved `out` (inside delta) are rounded.
+    of magnitudes.  bf16: results are rounded; P and dz enter the second products as two numbers each, rounded to
+    one for many rows (beyond 1024 nodes) without a mask; the saved `out` (inside delta) is two numbers.
     Underflow: an exponential below 2^-126 may be flushed to zero (its weight at most TINY off), and so may the two low parts of a dz
     that is computed as three bf16 (2 TINY)."""
     B, Nq, H, D = q.shape
     Nk, G = k.shape[1:3]
     scale = D ** -0.5 if scale is None else scale
     ur = U16 if bf16 else 0.0
+    up = 0.0 if not bf16 else U16 if bias is None and min(Nq * (H // G), Nk) > 64 and max(Nq, Nk) > 1024 else U16 ** 2
     z0 = lambda x: np.zeros(x.shape)
     res = {"out": [z0(q), z0(q)]}
     if dout is not None:
@@ -46,7 +48,8 @@ def attention(q, k, v, bias=None, key_sizes=None, query_sizes=None, scale=None, 
             rho = 2 * np.where(seen, e, 0.0).max(1, initial=0.0)[:, None] + (nk + 16) * U32
             out = p @ V
             pv = p @ abs(V)
-            e_out = (rho + ur) * pv + ur * abs(out) + (nk + 8) * U32 * pv + TINY * abs(V).sum(0)
+            e_sum = (rho + up) * pv + (nk + 8) * U32 * pv + TINY * abs(V).sum(0)
+            e_out = e_sum + ur * (abs(out) + e_sum)
             res["out"][0][b, :nq, h] = out
             res["out"][1][b, :nq, h] = e_out
             if dout is None:
@@ -55,10 +58,10 @@ def attention(q, k, v, bias=None, key_sizes=None, query_sizes=None, scale=None, 
             dp, delta = dO @ V.T, (dO * out).sum(1, keepdims=True)
             ds = p * (dp - delta)
             dpa = abs(dO) @ abs(V).T
-            e_delta = (D + 4) * U32 * (abs(dO) * abs(out)).sum(1, keepdims=True) + (abs(dO) * e_out).sum(1, keepdims=True)
+            e_delta = (D + 4) * U32 * (abs(dO) * abs(out)).sum(1, keepdims=True) + (abs(dO) * (e_sum + ur ** 2 * (abs(out) + e_sum))).sum(1, keepdims=True)
             e_ds = p * (rho * (abs(dp) + abs(delta)) + (D + 4) * U32 * dpa + e_delta + 4 * U32 * (abs(dp) + abs(delta)))
             e_ds = e_ds + TINY * (abs(dp) + abs(delta) + 2)
-            e_use = e_ds + ur * (abs(ds) + e_ds)
+            e_use = e_ds + up * (abs(ds) + e_ds)
             dq, dk, dv = scale * (ds @ K), scale * (ds.T @ Q), p.T @ dO
             adds = abs(ds) + e_ds
             res["dq"][0][b, :nq, h] = dq
@@ -67,7 +70,7 @@ def attention(q, k, v, bias=None, key_sizes=None, query_sizes=None, scale=None, 
             res["dk"][0][b, :nk, g] += dk
             res["dk"][1][b, :nk, g] += abs(scale) * (e_use.T @ abs(Q) + (n + 8) * U32 * (adds.T @ abs(Q)))
             res["dv"][0][b, :nk, g] += dv
-            res["dv"][1][b, :nk, g] += (p * (rho + ur) + 3 * TINY).T @ abs(dO) + (n + 8) * U32 * (p.T @ abs(dO))
+            res["dv"][1][b, :nk, g] += (p * (rho + up) + 3 * TINY).T @ abs(dO) + (n + 8) * U32 * (p.T @ abs(dO))
     for name in ("dq", "dk", "dv"):
         if name in res:
             res[name][1] += ur * (abs(res[name][0]) + res[name][1])

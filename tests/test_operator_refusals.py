@@ -59,15 +59,15 @@ def test_c_entry_points_refuse_before_any_launch():
     odd = (ctypes.c_int64 * 3)(33, 16, 8)
     P = 4096                                                       # a 16-byte aligned address that no accepted call below uses
 
-    def fwd(B=1, Nq=2, Nk=2, H=2, G=2, D=8, dt=0, q=P, qs=s3, k=P, bias=None, br=2, out=P, scale=1.0):
-        return lib.gatmi_dot_attn_fwd(B, Nq, Nk, H, G, D, dt, q, qs, k, s3, P, s3, bias, 0, br, None, None, scale, out, None, None, None, None, None)
+    def fwd(B=1, Nq=2, Nk=2, H=2, G=2, D=8, dt=0, q=P, qs=s3, k=P, bias=None, br=2, out=P, scale=1.0, low=None):
+        return lib.gatmi_dot_attn_fwd(B, Nq, Nk, H, G, D, dt, q, qs, k, s3, P, s3, bias, 0, br, None, None, scale, out, low, None, None, None, None, None)
 
     for rc, want, text in ((fwd(B=-1), -1, "B = -1"), (fwd(H=3), -1, "3 query heads"), (fwd(G=0), -1, "heads"), (fwd(D=6), -3, "head width 6"), (fwd(D=132), -3, "132"),
                            (fwd(D=12, dt=1), -3, "head width 12"), (fwd(dt=2), -1, "dtype"), (fwd(q=None), -1, "q is null"), (fwd(q=P + 4), -2, "aligned"), (fwd(qs=odd), -2, "aligned"),
-                           (fwd(k=None), -1, "k is null"), (fwd(bias=P, br=1), -1, "bias row stride"), (fwd(out=None), -1, "out is null"), (fwd(Nq=20, bias=P), -1, "mask words"), (fwd(Nq=2 ** 30, H=4, G=4), -4 - 1, "31 bits"), (fwd(scale=float("nan")), -1, "scale")):
+                           (fwd(k=None), -1, "k is null"), (fwd(bias=P, br=1), -1, "bias row stride"), (fwd(out=None), -1, "out is null"), (fwd(low=P), -1, "out_low is for bf16"), (fwd(Nq=20, bias=P), -1, "mask words"), (fwd(Nq=2 ** 30, H=4, G=4), -4 - 1, "31 bits"), (fwd(scale=float("nan")), -1, "scale")):
         assert rc == want, (rc, want, text)
     assert fwd(B=0) == 0 and fwd(Nq=0) == 0
-    rc = lib.gatmi_dot_attn_bwd(1, 2, 2, 2, 2, 8, 0, P, s3, P, s3, P, s3, P, P, s3, None, None, 0, 2, None, None, 1.0, None, None, P, P, P, P, None, None)
+    rc = lib.gatmi_dot_attn_bwd(1, 2, 2, 2, 2, 8, 0, P, s3, P, s3, P, s3, P, None, P, s3, None, None, 0, 2, None, None, 1.0, None, None, P, P, P, P, None, None)
     assert rc == -1 and "null" in _lib.last_error()
 
     def emb(bits=64, n=4, ld=8, rows=4, w=8, dt=0, ids=P):
