@@ -330,6 +330,35 @@ def test_captured_forward_and_backward():
         assert torch.equal(res_one, ops.dot_attention(one_query["q"], one_query["k"], one_query["v"]))
 
 
+def test_captured_masks_that_change_between_replays():
+    """One graph whose mask has few entries in one replay and many in the next, with fp32 rows in parts; eager work between."""
+    from gat_amd import graphs, ops
+    c = _case(2, 520, 520, 2, 2, 64, "f32", density=0.01)
+    q, k, v = (c[n].clone().requires_grad_() for n in ("q", "k", "v"))
+    e = _case(2, 520, 520, 2, 2, 64, "bf16", density=0.01)
+    eq, ek, ev = (e[n].clone().requires_grad_() for n in ("q", "k", "v"))
+
+    def step():
+        out = ops.dot_attention(q, k, v, c["bias"])
+        out16 = ops.dot_attention(eq, ek, ev, e["bias"])
+        return (out, *torch.autograd.grad(out, (q, k, v), c["dout"]), out16, *torch.autograd.grad(out16, (eq, ek, ev), e["dout"]))
+
+    replay, res = graphs.capture(step, fresh_dropout=False)
+    for seed, density in enumerate((0.01, 0.3, 0.002, 1.0, 0.05)):
+        n, m = (_case(2, 520, 520, 2, 2, 64, dt, density=density, seed=seed) for dt in ("f32", "bf16"))
+        with torch.no_grad():
+            for to, frm, leaves in ((c, n, (q, k, v)), (e, m, (eq, ek, ev))):
+                for a, b in zip(leaves, ("q", "k", "v")):
+                    a.copy_(frm[b])
+                to["bias"].copy_(frm["bias"])
+                to["dout"].copy_(frm["dout"])
+        replay()
+        torch.cuda.synchronize()
+        want = [_run(n)[x] for x in ("out", "dq", "dk", "dv")] + [_run(m)[x] for x in ("out", "dq", "dk", "dv")]
+        for i, (got, w) in enumerate(zip(res, want)):
+            assert torch.equal(got, w), (density, i)
+
+
 def test_gradient_against_differences():
     """d/dt of <out(x + t d), dout> from outputs at t = +-h: truncation is h^2 times a third derivative of order 1, rounding 1e-6 / h."""
     from gat_amd import ops
