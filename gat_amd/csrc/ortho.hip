@@ -410,6 +410,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(WideArgs a) {
 
 // MODE: what becomes of a product.
 constexpr int kNsGram = 0, kNsPoly = 1, kNsStep = 2, kNsLast = 3;
+// Stages in LDS.  The symmetric products have about one 128 x 128 block to a compute unit: three.  Tiles of 64 are so small that five of two
+// blocks fit (five steps in us, with two or three - with five: 512 x 2048: 299 - 293, 1024 x 4096: 546 - 516, 2 x 1024 x 1024: 475 - 454, 256 x 256: 126 - 129).
+template <int MODE> constexpr int ns_stages(int tile) { return tile == 64 ? 5 : (MODE == kNsGram || MODE == kNsPoly ? 3 : 2); }
 template <int MODE> struct NsMode { static constexpr bool SYM = MODE == kNsGram || MODE == kNsPoly; };
 
 template <int MODE>
@@ -444,10 +447,10 @@ __device__ __forceinline__ void ns_product(const _Float16 *U, const _Float16 *V,
                                              (__attribute__((address_space(3))) void *)(&buf[s][wave >> 1][r0 * 64]), 16, 0, 0);
         }
     };
-    // the loads of the other waves have to be in LDS too: each waits for its own (all but those of the newest stage) before the barrier
+    // the loads of the other waves have to be in LDS too: each waits for its own (all but those of the stages after the next) before the barrier
     auto arrived = [&](bool all) {
         if (all) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * LOADS) : "memory");
         __syncthreads();
     };
     const int wi = (wave >> 1) * WV, wj = (wave & 1) * WV;
@@ -457,7 +460,7 @@ __device__ __forceinline__ void ns_product(const _Float16 *U, const _Float16 *V,
 #pragma unroll
     for (int g = 0; g < STAGES - 1; ++g)
         if (k0 + g * kWK < k1) stage(g, k0 + g * kWK);
-    arrived(STAGES == 2 || k0 + kWK >= k1);
+    arrived(k0 + AHEAD > k1);
     int s = 0;
     for (int64_t k = k0; k < k1; k += kWK, s = s + 1 == STAGES ? 0 : s + 1) {
         const bool more = k + AHEAD < k1;
@@ -484,7 +487,7 @@ __device__ __forceinline__ void ns_product(const _Float16 *U, const _Float16 *V,
         for (int i = 0; i < F; ++i)
 #pragma unroll
             for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(uh[i], vh[j], acc[i][j], 0, 0, 0);
-        arrived(STAGES == 2 || !more);
+        arrived(!more);
     }
 }
 
@@ -544,8 +547,7 @@ __device__ __forceinline__ NsTile ns_tile(int ty, int64_t tile) {         // til
 template <int MODE, int WT, typename T, bool TALL>
 __global__ __launch_bounds__(256) void ns_gemm_kernel(WideArgs a) {
     constexpr int WV = WT / 2, F = WV / 16;
-    // The symmetric products have about one block to a compute unit: three stages.
-    constexpr int STAGES = NsMode<MODE>::SYM ? 3 : 2;
+    constexpr int STAGES = ns_stages<MODE>(WT);
     extern __shared__ __attribute__((aligned(16))) char ns_lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t b = blockIdx.z;
@@ -896,7 +898,7 @@ static int ns_gemm(const WideArgs &a, int64_t batch, hipStream_t st) {
         return dim3((unsigned)((SYM ? y * (y + 1) / 2 : y * x) * 16), 1, (unsigned)batch);
     };
     const bool wide = (SYM ? ty * (ty + 1) / 2 : ty * tx) * batch >= kTileBlocks;
-    const size_t lds = (SYM ? 3 : 2) * (wide ? 128 : 64) * 256;
+    const size_t lds = (size_t)ns_stages<MODE>(wide ? 128 : 64) * (wide ? 128 : 64) * 256;
     auto kernel = wide ? ns_gemm_kernel<MODE, 128, T, TALL> : ns_gemm_kernel<MODE, 64, T, TALL>;
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
