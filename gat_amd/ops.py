@@ -987,7 +987,7 @@ def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, s
     q [B,Nq,H,D], k and v [B,Nk,Hkv,D] (H a multiple of Hkv, D at most 128), fp32 or bf16; any strides (rows that are not
     16-byte aligned are copied once).  Nq = 1 answers for single nodes.  scale: D ** -0.5 unless given.
     bias_mat [B or 1, Nq, Nk] fp32 (or None): an entry not above -1e8 is not attended; it takes no gradient.
-    key_sizes, query_sizes: int32 [B] on the same device: rows behind a graph's own nodes are neither read nor given a
+    key_sizes, query_sizes: int32 [B] on the same device: rows behind a graph's own nodes take no part and get no
     gradient, and their outputs are zeros.  A row without an attended key gives zeros.  Rows of k and v inside key_sizes have to be
     finite also where the mask leaves them out.  The backward recomputes the probabilities and adds in a fixed order."""
     what = "dot_attention"

@@ -558,7 +558,7 @@ int gatmi_ipd_bwd(int64_t B, int32_t N, int32_t F, const float *dOut, const floa
  *   key/value head h / (H / Hkv).  out contiguous [B, Nq, H, D].
  *   bias: optional fp32 [B, Nq, Nk] with strides bias_batch (0: one mask for all graphs), bias_row, 1.  An entry whose bias is
  *   not above -1e8 is not attended.  key_sizes, query_sizes: optional int32 [B] on the device, clamped to [0, Nk] / [0, Nq]; keys behind
- *   theirs are not read, queries behind theirs give zeros and take no part in the gradients.  A row without an
+ *   theirs take no part, queries behind theirs give zeros and take no part in the gradients.  A row without an
  *   attended key gives zeros.
  *   fwd: lse [B, H, Nq] (log2 of the row's sum of exponentials; NULL when no backward follows).  ws: gatmi_dot_attn_fwd_ws_floats
  *   (0: may be NULL); few rows on many keys are split over the keys and joined.
