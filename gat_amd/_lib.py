@@ -156,12 +156,19 @@ def ptr(t):
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# index of the current device without the check that the GPU has been initialised, which a tensor on it answers
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def current_stream():
     """Handle of the HIP stream torch currently records on (the hipStream_t the kernels are enqueued
     on).  The raw accessor avoids building a torch.cuda.Stream object per call (about 10 us each, a
     visible share of a launch-bound step)."""
+    return stream_of(torch.cuda.current_device())
+
+
+def stream_of(index):
+    """The same for the device of that index."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream

@@ -881,11 +881,12 @@ def _same_device(what, t, *others):
 
 def _launch(device, name, *args):
     """One library call on `device`, on the stream torch currently records on there."""
-    if device.index == torch.cuda.current_device():
-        rc = getattr(_lib.lib, name)(*args, _lib.current_stream())
+    index = device.index
+    if index == _lib.current_device():
+        rc = getattr(_lib.lib, name)(*args, _lib.stream_of(index))
     else:
         with torch.cuda.device(device):
-            rc = getattr(_lib.lib, name)(*args, _lib.current_stream())
+            rc = getattr(_lib.lib, name)(*args, _lib.stream_of(index))
     if rc:
         _lib.check(rc, name)
 
@@ -1019,16 +1020,18 @@ def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, s
     return out[..., :D] if out.shape[3] != D else out
 
 
+_ID_BITS = {torch.int32: 32, torch.int64: 64}
+
+
 def _embed_forward(ids, table, scale):
     """(ids flat, scale * table[ids])"""
     rows, width = table.shape
-    flat = ids.reshape(-1)
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
     flat = flat if flat.is_contiguous() else flat.contiguous()
-    n = flat.numel()
     tb = table if table.stride(1) == 1 and table.stride(0) >= width else table.contiguous()
-    out = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
-    _launch(table.device, "gatmi_embed_fwd", flat.data_ptr(), 8 * flat.element_size(), n, tb.data_ptr(), tb.stride(0), rows, width, _FLOATS[table.dtype], scale,
-            out.data_ptr())
+    out = table.new_empty((*ids.shape, width))
+    _launch(table.device, "gatmi_embed_fwd", flat.data_ptr(), _ID_BITS[flat.dtype], flat.numel(), tb.data_ptr(), tb.stride(0), rows, width, _FLOATS[table.dtype],
+            scale, out.data_ptr())
     return flat, out
 
 
@@ -1047,12 +1050,11 @@ class EmbeddingFn(torch.autograd.Function):
     def backward(ctx, dout):
         (flat,) = ctx.saved_tensors
         n, rows, width = flat.numel(), ctx.rows, dout.shape[-1]
-        d = dout.reshape(n, width)
+        d = dout if dout.dim() == 2 else dout.reshape(n, width)
         d = d if d.stride(1) == 1 and d.stride(0) >= width else d.contiguous()
-        dev = dout.device
-        grad = torch.empty((rows, width), dtype=dout.dtype, device=dev)
-        ws = _scratch(_lib.lib.gatmi_embed_bwd_ws_floats(n, rows, width), dev)
-        _launch(dev, "gatmi_embed_bwd", flat.data_ptr(), 8 * flat.element_size(), n, d.data_ptr(), d.stride(0), rows, width, _FLOATS[dout.dtype], ctx.scale,
+        grad = d.new_empty((rows, width))
+        ws = _scratch(_lib.lib.gatmi_embed_bwd_ws_floats(n, rows, width), d.device)
+        _launch(d.device, "gatmi_embed_bwd", flat.data_ptr(), _ID_BITS[flat.dtype], n, d.data_ptr(), d.stride(0), rows, width, _FLOATS[d.dtype], ctx.scale,
                 grad.data_ptr(), ptr(ws))
         return None, grad, None
 
