@@ -891,6 +891,13 @@ def _launch(device, name, *args):
         _lib.check(rc, name)
 
 
+def _recorded():
+    """Whether somebody follows what is called: torch.jit.trace, or forward-mode differentiation.  An operator then goes through its
+    Function also where no gradient is asked: a trace records that as one node (of a bare launch it would keep the allocation of the
+    result only), and a tangent is refused instead of lost."""
+    return torch.jit.is_tracing() or torch.autograd.forward_ad._current_level >= 0
+
+
 def _scratch(floats, device):
     return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
 
@@ -948,9 +955,11 @@ class DotAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, key_sizes, query_sizes, scale):
         D = q.shape[3]
-        qr, kr, vr, out, low, lse, words, planes, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, True)
-        ctx.save_for_backward(qr, kr, vr, out, low, lse, bias, words, planes, key_sizes, query_sizes)
-        ctx.scale, ctx.D, ctx.bias_strides = scale, D, strides
+        need = any(ctx.needs_input_grad)
+        qr, kr, vr, out, low, lse, words, planes, strides = _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need)
+        if need:
+            ctx.save_for_backward(qr, kr, vr, out, low, lse, bias, words, planes, key_sizes, query_sizes)
+            ctx.scale, ctx.D, ctx.bias_strides = scale, D, strides
         return out[..., :D] if out.shape[3] != D else out
 
     @staticmethod
@@ -1014,7 +1023,7 @@ def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, s
             bias_mat = bias_mat.contiguous()
     scale = float(D) ** -0.5 if scale is None else float(scale)
     key_sizes, query_sizes = _sizes("key_sizes", key_sizes, B, dev), _sizes("query_sizes", query_sizes, B, dev)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) or _recorded():
         return DotAttentionFn.apply(q, k, v, bias_mat, key_sizes, query_sizes, scale)
     out = _dot_forward(q, k, v, bias_mat, key_sizes, query_sizes, scale, False)[3]
     return out[..., :D] if out.shape[3] != D else out
@@ -1069,7 +1078,7 @@ def embedding(ids, table, scale=1.0):
         raise ValueError("embedding: table is [rows, width], got %s" % (tuple(table.shape) if torch.is_tensor(table) else type(table),))
     _float_type("embedding", table)
     _same_device("embedding", table, ids)
-    if table.requires_grad and torch.is_grad_enabled():
+    if table.requires_grad and torch.is_grad_enabled() or _recorded():
         return EmbeddingFn.apply(ids, table, float(scale))
     return _embed_forward(ids, table, float(scale))[1]
 
@@ -1077,24 +1086,38 @@ def embedding(ids, table, scale=1.0):
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # a, b, c of the quintic usual for orthogonalised updates: steep at 0, and [0.7, 1.2] maps into itself
 
 
+def _newton_schulz(x, steps, eps, coefficients):
+    m, n = x.shape[-2:]
+    x3 = x.detach()
+    if x3.dim() != 3:
+        x3 = x3.reshape(math.prod(x.shape[:-2]), m, n)
+    if x3.stride(2) != 1 or x3.stride(1) < n:
+        x3 = x3.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a, b, c = coefficients
+    ws = _scratch(_lib.lib.gatmi_newton_schulz_ws_floats(x3.shape[0], m, n), x.device)
+    _launch(x.device, "gatmi_newton_schulz", x3.shape[0], m, n, x3.data_ptr(), x3.stride(0), x3.stride(1), _FLOATS[x.dtype], int(steps), float(a), float(b), float(c),
+            float(eps), out.data_ptr(), m * n, n, ptr(ws))
+    return out
+
+
+class NewtonSchulzFn(torch.autograd.Function):
+    """newton_schulz where it is recorded (see _recorded); it has no derivative."""
+
+    @staticmethod
+    def forward(ctx, x, steps, eps, coefficients):
+        out = _newton_schulz(x, steps, eps, coefficients)
+        ctx.mark_non_differentiable(out)
+        return out
+
+
 def newton_schulz(x, steps=5, eps=1e-7, coefficients=NEWTON_SCHULZ):
     """Every m x n matrix of x [..., m, n] (fp32 or bf16) with its singular values driven towards 1: from X = x / (|x|_F + eps), `steps`
     times X <- a X + b (X X^T) X + c (X X^T)^2 X, at fp32 accuracy whatever the type (gatmi_newton_schulz).  Outside autograd."""
     if not torch.is_tensor(x) or x.dim() < 2:
         raise ValueError("newton_schulz: x is [..., m, n], got %s" % (tuple(x.shape) if torch.is_tensor(x) else type(x),))
-    dtype = _float_type("newton_schulz", x)
+    _float_type("newton_schulz", x)
     _require_cuda(x)
-    shape = x.shape
-    m, n = shape[-2:]
-    x3 = x.detach()
-    if x3.dim() != 3:
-        x3 = x3.reshape(math.prod(shape[:-2]), m, n)
-    if x3.stride(2) != 1 or x3.stride(1) < n:
-        x3 = x3.contiguous()
-    dev = x.device
-    out = torch.empty(shape, dtype=x.dtype, device=dev)
-    a, b, c = coefficients
-    ws = _scratch(_lib.lib.gatmi_newton_schulz_ws_floats(x3.shape[0], m, n), dev)
-    _launch(dev, "gatmi_newton_schulz", x3.shape[0], m, n, x3.data_ptr(), x3.stride(0), x3.stride(1), dtype, int(steps), float(a), float(b), float(c), float(eps),
-            out.data_ptr(), m * n, n, ptr(ws))
-    return out
+    if _recorded():
+        return NewtonSchulzFn.apply(x, steps, eps, coefficients)
+    return _newton_schulz(x, steps, eps, coefficients)

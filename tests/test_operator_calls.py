@@ -36,3 +36,63 @@ def test_a_lookup_of_a_list_of_ids_only_allocates(launches):
         torch.autograd.grad(out, table, dout)
     assert [n for n in seen.names if "empty" not in n and "detach" not in n] == [] and sum("empty" in n for n in seen.names) == 2
     assert [n for n, _ in launches] == ["gatmi_embed_fwd", "gatmi_embed_fwd", "gatmi_embed_bwd"]
+
+
+def _calls():
+    """name -> (call of one tensor, that tensor)"""
+    from gat_amd import ops
+    g = torch.Generator().manual_seed(0)
+    rows, ids, sizes = torch.randn((2, 3, 4, 8), generator=g), torch.tensor([[1, 0], [3, -1]]), torch.tensor([3, 1], dtype=torch.int32)
+    mask = torch.zeros((1, 3, 3))
+    return {"queries": (lambda x: ops.dot_attention(x, rows, rows, mask, key_sizes=sizes), rows), "keys": (lambda x: ops.dot_attention(rows, x, rows), rows),
+            "values": (lambda x: ops.dot_attention(rows, rows, x, scale=2.0), rows), "odd width": (lambda x: ops.dot_attention(x, x, x), rows[..., :7]),
+            "embedding": (lambda x: ops.embedding(ids, x, 0.5), rows[0, 0]), "newton_schulz": (lambda x: ops.newton_schulz(x, 3), rows),
+            "newton_schulz of one": (lambda x: ops.newton_schulz(x, coefficients=(1.5, -0.5, 0.0)), rows[0, 0])}
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+def test_tangents_are_refused(launches, name):
+    import torch.autograd.forward_ad as forward_ad
+    call, x = _calls()[name]
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        launches.clear()
+        call(x)                                                                       # without a tangent the level changes nothing
+        assert len(launches) == 1
+
+
+@pytest.mark.parametrize("name", list(_calls()))
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_a_trace_keeps_the_launch(launches, name):
+    call, x = _calls()[name]
+    shape = call(x).shape
+    traced = torch.jit.trace(call, x, check_trace=False)
+    want = launches[0][0]
+    launches.clear()
+    assert traced(x + 1).shape == shape
+    with torch.no_grad():
+        assert traced(x + 1).shape == shape
+    assert [n for n, _ in launches] == [want, want]
+
+
+def test_no_gradient_saves_nothing_for_one(launches):
+    """Recorded without a gradient asked, the attention takes what serving takes: no row sums, no bits of a small mask."""
+    import torch.autograd.forward_ad as forward_ad
+    from gat_amd import ops
+    q, mask = torch.zeros((1, 2, 1, 8)), torch.zeros((1, 2, 2))
+    ops.dot_attention(q, q, q, mask)
+    with forward_ad.dual_level():
+        ops.dot_attention(q, q, q, mask)
+    (_, plain), (_, recorded) = launches
+    pointers = lambda args: [a is None for a in args[7:]]
+    assert pointers(plain) == pointers(recorded)
+
+
+def test_newton_schulz_takes_no_gradient_recorded_or_not(launches):
+    import torch.autograd.forward_ad as forward_ad
+    from gat_amd import ops
+    x = torch.zeros((4, 4), requires_grad=True)
+    assert not ops.newton_schulz(x).requires_grad
+    with forward_ad.dual_level():
+        assert not ops.newton_schulz(x).requires_grad
