@@ -906,16 +906,18 @@ _Int64x3 = ctypes.c_int64 * 3
 
 
 def _strides(t):
-    s = t.stride()
-    return _Int64x3(s[0], s[1], s[2])
+    """Element strides of graph, node and head; that of a dimension of size 1, which torch leaves as it came, is 0."""
+    n, s = t.shape, t.stride()
+    return _Int64x3(s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
 def _attn_rows(t, width):
     """t [B, N, heads, D] as rows the kernels take: D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
     if t.shape[3] != width:
         return torch.nn.functional.pad(t, (0, width - t.shape[3]))
-    s, low = t.stride(), 15 // t.element_size()                    # strides are multiples of 4 (fp32) or 8 (bf16) elements
-    if s[3] == 1 and not ((s[0] | s[1] | s[2]) & low) and not (t.data_ptr() & 15):
+    n, s, low = t.shape, t.stride(), 15 // t.element_size()        # strides are multiples of 4 (fp32) or 8 (bf16) elements
+    apart = (s[0] if n[0] > 1 else 0) | (s[1] if n[1] > 1 else 0) | (s[2] if n[2] > 1 else 0)
+    if s[3] == 1 and not (apart & low) and not (t.data_ptr() & 15):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

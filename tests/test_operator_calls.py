@@ -96,3 +96,28 @@ def test_newton_schulz_takes_no_gradient_recorded_or_not(launches):
     assert not ops.newton_schulz(x).requires_grad
     with forward_ad.dual_level():
         assert not ops.newton_schulz(x).requires_grad
+
+
+def _odd_strides(dtype):
+    """name -> [B, N, heads, 8] rows with a dimension of size 1 whose stride divides nothing"""
+    base = torch.arange(2 * 5 * 3 * 9, dtype=torch.float32).to(dtype)
+    v = lambda *a: torch.as_strided(base, *a)
+    return {"one query of one graph": base[:9].reshape(1, 1, 9)[..., :8].unsqueeze(2), "one graph": v((1, 5, 2, 8), (77, 16, 8, 1)), "one node": v((3, 1, 2, 8), (16, 3, 8, 1)),
+            "one head": v((2, 5, 1, 8), (40, 8, 5, 1)), "one head, not aligned": v((2, 5, 1, 8), (40, 8, 5, 1), 1), "one of all, not aligned": v((1, 1, 1, 8), (9, 7, 5, 1), 3),
+            "one head, rows 9 apart": v((2, 5, 1, 8), (45, 9, 3, 1))}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", list(_odd_strides(torch.float32)))
+def test_strides_of_dimensions_of_size_one_do_not_matter(name, dtype):
+    from gat_amd import _lib, ops
+    t = _odd_strides(dtype)[name]
+    rows = ops._attn_rows(t, 8)
+    B, N, H, D = rows.shape
+    strides = ops._strides(rows)
+    assert torch.equal(rows, t)
+    assert rows.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in strides)
+    assert torch.equal(torch.as_strided(rows, rows.shape, (*strides, 1)), t)
+    # the library takes them: it gets as far as the missing result
+    rc = _lib.lib.gatmi_dot_attn_fwd(B, N, N, H, H, D, ops._FLOATS[dtype], *(rows.data_ptr(), strides) * 3, None, 0, N, None, None, 1.0, None, None, None, None, None, None, None)
+    assert rc == -1 and "out is null" in _lib.last_error()

@@ -24,3 +24,24 @@ def test_traced_calls_compute_what_eager_ones_do():
         args = [torch.randn(t.shape, device=dev, generator=g) for t in (q, k, table, x)]
         for a, b in zip(traced(*args), call(*args)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_odd_strides_of_dimensions_of_size_one(dtype):
+    """One query of one graph out of a wider row, one head, one node: as their contiguous copies, gradients included."""
+    from gat_amd import ops
+    dev = torch.device("cuda:0")
+    base = torch.randn(4096, device=dev).to(dtype)
+    v = lambda *a: torch.as_strided(base, *a)
+    k = torch.randn((1, 30, 1, 8), device=dev).to(dtype)
+    cases = [(base[:9].reshape(1, 1, 9)[..., :8].unsqueeze(2), k), (v((1, 5, 1, 8), (77, 16, 3, 1)), v((1, 30, 1, 8), (3, 8, 5, 1))), (v((3, 1, 2, 8), (16, 3, 8, 1)), v((3, 20, 1, 8), (160, 8, 7, 1))),
+             (v((2, 5, 1, 8), (40, 8, 5, 1), 1), v((2, 6, 1, 8), (48, 8, 1, 1)))]
+    for q, k in cases:
+        got, want = [], []
+        for res, leaves in ((got, (q, k)), (want, (q.contiguous().clone(), k.contiguous().clone()))):
+            q_, k_ = (t.detach().requires_grad_() for t in leaves)
+            out = ops.dot_attention(q_, k_, k_)
+            dout = torch.as_strided(base, out.shape, (out.stride(0), out.stride(1), 3 if out.shape[2] == 1 else out.stride(2), 1), 64)
+            res += [ops.dot_attention(*leaves, leaves[1]), out, *torch.autograd.grad(out, (q_, k_), dout)]
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
