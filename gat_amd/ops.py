@@ -914,7 +914,9 @@ def _strides(t):
 def _attn_rows(t, width):
     """t [B, N, heads, D] as rows the kernels take: D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
     if t.shape[3] != width:
-        return torch.nn.functional.pad(t, (0, width - t.shape[3]))
+        rows = t.new_zeros((*t.shape[:3], width))                  # not pad(t): it keeps the order that the dimensions have in memory
+        rows[..., :t.shape[3]] = t
+        return rows
     n, s, low = t.shape, t.stride(), 15 // t.element_size()        # strides are multiples of 4 (fp32) or 8 (bf16) elements
     apart = (s[0] if n[0] > 1 else 0) | (s[1] if n[1] > 1 else 0) | (s[2] if n[2] > 1 else 0)
     if s[3] == 1 and not (apart & low) and not (t.data_ptr() & 15):

@@ -121,3 +121,25 @@ def test_strides_of_dimensions_of_size_one_do_not_matter(name, dtype):
     # the library takes them: it gets as far as the missing result
     rc = _lib.lib.gatmi_dot_attn_fwd(B, N, N, H, H, D, ops._FLOATS[dtype], *(rows.data_ptr(), strides) * 3, None, 0, N, None, None, 1.0, None, None, None, None, None, None, None)
     assert rc == -1 and "out is null" in _lib.last_error()
+
+
+def _orders():
+    """name -> (turned, order): x.permute(*turned).contiguous().permute(*order) is x with its dimensions in another order in memory"""
+    return {"heads first": ((0, 2, 1, 3), (0, 2, 1, 3)), "nodes fastest": ((0, 2, 3, 1), (0, 3, 1, 2)), "graphs fastest": ((1, 2, 3, 0), (3, 0, 1, 2)), "width first": ((3, 0, 1, 2), (1, 2, 3, 0)),
+            "heads fastest": ((0, 1, 3, 2), (0, 1, 3, 2))}
+
+
+@pytest.mark.parametrize("D", [4, 8, 13, 100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("order", list(_orders()))
+def test_rows_in_any_order_become_rows_of_the_kernels(order, dtype, D):
+    from gat_amd import ops
+    turned, back = _orders()[order]
+    unit = 4 if dtype == torch.float32 else 8
+    width = (D + unit - 1) // unit * unit
+    x = torch.randn((2, 40, 3, D)).to(dtype)
+    t = x.permute(*turned).contiguous().permute(*back)
+    assert torch.equal(t, x)
+    rows = ops._attn_rows(t, width)
+    assert rows.stride(3) == 1 and rows.data_ptr() % 16 == 0 and all(s % unit == 0 for s in ops._strides(rows))
+    assert torch.equal(rows[..., :D], x) and (rows[..., D:] == 0).all()

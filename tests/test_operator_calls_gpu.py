@@ -45,3 +45,22 @@ def test_odd_strides_of_dimensions_of_size_one(dtype):
             res += [ops.dot_attention(*leaves, leaves[1]), out, *torch.autograd.grad(out, (q_, k_), dout)]
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [13, 16, 100])
+@pytest.mark.parametrize("turned,back", [((0, 2, 1, 3), (0, 2, 1, 3)), ((0, 2, 3, 1), (0, 3, 1, 2)), ((3, 0, 1, 2), (1, 2, 3, 0)), ((0, 1, 3, 2), (0, 1, 3, 2))])
+def test_rows_and_gradients_in_any_order_of_dimensions(turned, back, D, dtype):
+    """Rows, and the gradient of a result that is read in another order, as their contiguous copies."""
+    from gat_amd import ops
+    dev = torch.device("cuda:0")
+    g = torch.Generator(device=dev).manual_seed(D)
+    q, k, dout = (torch.randn((2, 45, h, D), device=dev, generator=g).to(dtype) for h in (4, 2, 4))
+    got, want = [], []
+    for res, other in ((got, lambda t: t.permute(*turned).contiguous().permute(*back)), (want, lambda t: t)):
+        q_, k_ = (other(t).detach().requires_grad_() for t in (q, k))
+        out = ops.dot_attention(q_, k_, k_)
+        read = out.permute(*turned).contiguous() if res is got else out
+        res += [ops.dot_attention(other(q), other(k), other(k)), out, *torch.autograd.grad(read, (q_, k_), dout.permute(*turned).contiguous() if res is got else dout)]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
