@@ -323,10 +323,13 @@ class DotHeads(nn.Module):
     scale <q_i, k_j> in place of f_1 + f_2):  act(softmax(q k^T / sqrt(D) + bias_mat) v + bias).
     W [F, H + 2 G, D]: the query kernels of the H heads, then the key and the value kernels of the G = kv_heads shared heads (H
     unless given); bias [H, D]; W_res / b_res as in GATHeads.  One projection, one attention launch for all heads.
-    storage="bf16": the rows the attention reads are rounded to bf16 (sums and softmax stay fp32)."""
+    storage="bf16": the rows the attention reads are rounded to bf16 (sums and softmax stay fp32).
+    Arguments in the order of GATHeads; what GATHeads does not have is given by name."""
 
-    def __init__(self, f_in, heads, width, kv_heads=None, residual=False, device=None, storage="f32"):
+    def __init__(self, f_in, heads, width, residual=False, device=None, storage="f32", *, kv_heads=None):
         super().__init__()
+        if residual not in (False, True):
+            raise ValueError("residual is True or False, got %r" % (residual,))
         if storage not in ("f32", "bf16"):
             raise ValueError("storage must be 'f32' or 'bf16'")
         self.f_in, self.heads, self.width = int(f_in), int(heads), int(width)
@@ -347,13 +350,19 @@ class DotHeads(nn.Module):
             if self.has_res:
                 self.W_res.uniform_(-lim, lim)
 
-    def forward(self, seq, bias_mat, activation="elu", reduce="concat", sizes=None):
-        """seq [B,N,F], bias_mat [B or 1,N,N] or None, sizes int32 [B]: nodes of each graph (rows behind them give act(bias))."""
+    def forward(self, seq, bias_mat, activation="elu", reduce="concat", in_drop=0.0, coef_drop=0.0, training=None, *, sizes=None):
+        """seq [B,N,F], bias_mat [B or 1,N,N] or None, sizes int32 [B]: nodes of each graph (rows behind them give act(bias)).
+        in_drop drops seq in training, as in GATHeads; the coefficients are never dropped: coef_drop is refused in training."""
+        training = self.training if training is None else training
+        if training and coef_drop != 0.0:
+            raise ValueError("dot-product heads have no dropout of the coefficients (coef_drop = %r)" % (coef_drop,))
         act = _activation_name(activation)
         if reduce not in ("concat", "mean"):
             raise ValueError("reduce must be 'concat' or 'mean'")
         if act != "identity" and reduce == "mean":
             raise ValueError("mean over heads is defined for the identity activation (models/sp_gat.py:30-32)")
+        if training and in_drop != 0.0:
+            seq = torch.nn.functional.dropout(seq, in_drop, True)
         B, N, F = seq.shape
         H, G, D = self.heads, self.kv_heads, self.width
         rows = ops.tall_linear(seq, self.W.reshape(F, -1).t()).reshape(B, N, H + 2 * G, D)
@@ -367,17 +376,18 @@ class DotHeads(nn.Module):
         return out.reshape(B, N, H, D).mean(2) if reduce == "mean" else out
 
 
-def dot_attn_heads(seq, out_sz, bias_mat, activation, n_heads, reduce="concat", in_drop=0.0, residual=False, sizes=None):
-    """n_heads dot-product heads over bias_mat, variables from the active VariableStore; a non-zero in_drop drops seq."""
-    if in_drop != 0.0:
-        seq = torch.nn.functional.dropout(seq, in_drop, True)
+def dot_attn_heads(seq, out_sz, bias_mat, activation, n_heads, reduce="concat", in_drop=0.0, coef_drop=0.0,
+                   residual=False, training=True, *, sizes=None):
+    """attn_heads with dot-product scores: n_heads heads over bias_mat, variables from the active VariableStore; coef_drop is refused."""
     m = default_store().next_heads(seq.shape[-1], n_heads, out_sz, residual, seq.device, DotHeads)
-    return m(seq, bias_mat, activation, reduce, sizes)
+    return m(seq, bias_mat, activation, reduce, in_drop, coef_drop, training, sizes=sizes)
 
 
-def dot_attn_head(seq, out_sz, bias_mat, activation, in_drop=0.0, residual=False):
-    """attn_head (utils/layers.py:6) with dot-product scores: seq [B,N,F], bias_mat [B,N,N] additive mask; returns [B,N,out_sz]."""
-    return dot_attn_heads(seq, out_sz, bias_mat, activation, 1, "concat", in_drop, residual)
+def dot_attn_head(seq, out_sz, bias_mat, activation, in_drop=0.0, coef_drop=0.0, residual=False):
+    """attn_head (utils/layers.py:6) with dot-product scores: seq [B,N,F], bias_mat [B,N,N] additive mask; returns [B,N,out_sz].
+    There is no dropout of the coefficients: a non-zero coef_drop is refused."""
+    training = in_drop != 0.0 or coef_drop != 0.0
+    return dot_attn_heads(seq, out_sz, bias_mat, activation, 1, "concat", in_drop, coef_drop, residual, training)
 
 
 class NodeEmbedding(nn.Module):

@@ -1,4 +1,6 @@
 """CPU tests: what ops.dot_attention, ops.embedding and ops.newton_schulz do around their launches, which are replaced by a list of them."""
+import inspect
+
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -143,3 +145,29 @@ def test_rows_in_any_order_become_rows_of_the_kernels(order, dtype, D):
     rows = ops._attn_rows(t, width)
     assert rows.stride(3) == 1 and rows.data_ptr() % 16 == 0 and all(s % unit == 0 for s in ops._strides(rows))
     assert torch.equal(rows[..., :D], x) and (rows[..., D:] == 0).all()
+
+
+def test_layers_take_the_arguments_of_their_kin_in_the_same_order():
+    """A call that is moved over from the additive heads means the same by position."""
+    from gat_amd import layers
+    names = lambda f: [n for n, p in inspect.signature(f).parameters.items() if p.kind == p.POSITIONAL_OR_KEYWORD]
+    assert names(layers.dot_attn_head) == names(layers.attn_head)
+    assert names(layers.dot_attn_heads) == names(layers.attn_heads)
+    assert names(layers.DotHeads.__init__) == names(layers.GATHeads.__init__)
+    ours, theirs = names(layers.DotHeads.forward), names(layers.GATHeads.forward)
+    assert ours[3:] == theirs[3:len(ours)] and theirs[len(ours):] == ["seed"]                  # the mask has a name of its own; no seed: torch drops the input
+
+
+def test_dropout_of_the_coefficients_is_refused():
+    from gat_amd import layers
+    x, store = torch.zeros((1, 3, 8)), layers.VariableStore()
+    with layers.variable_scope(store):
+        for call in (lambda: layers.dot_attn_head(x, 8, None, layers.elu, 0.6, 0.6), lambda: layers.dot_attn_head(x, 8, None, layers.elu, coef_drop=0.6),
+                     lambda: layers.dot_attn_heads(x, 8, None, "elu", 2, "concat", 0.0, 0.6), lambda: layers.DotHeads(8, 2, 8)(x, None, coef_drop=0.1)):
+            store.layers = torch.nn.ModuleList()
+            store.begin()
+            with pytest.raises(ValueError, match="coef_drop"):
+                call()
+            assert not any(m.has_res for m in store.layers)
+    with pytest.raises(ValueError, match="residual"):
+        layers.DotHeads(8, 4, 8, 2)                                                            # not the number of shared heads

@@ -64,3 +64,26 @@ def test_rows_and_gradients_in_any_order_of_dimensions(turned, back, D, dtype):
         res += [ops.dot_attention(other(q), other(k), other(k)), out, *torch.autograd.grad(read, (q_, k_), dout.permute(*turned).contiguous() if res is got else dout)]
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_dot_heads_drop_their_input_in_training_only():
+    from gat_amd import layers
+    dev = torch.device("cuda:0")
+    store, x = layers.VariableStore(), torch.randn((2, 30, 16), device=dev)
+
+    def call(*args, **kw):
+        store.begin()
+        with layers.variable_scope(store):
+            return layers.dot_attn_heads(x, 8, None, "elu", 2, "concat", *args, **kw)
+    want = call()
+    assert torch.equal(call(0.5, 0.6, False, False), want) and torch.equal(call(0.5, training=False), want)
+    torch.manual_seed(1)
+    a = call(0.5)
+    torch.manual_seed(1)
+    dropped = torch.nn.functional.dropout(x, 0.5, True)
+    m = store.layers[0]
+    assert not torch.equal(a, want) and torch.equal(a, m(dropped, None))
+    m.eval()
+    assert torch.equal(m(x, None, "elu", "concat", 0.5, 0.6), want)
+    sizes = torch.tensor([30, 7], device=dev, dtype=torch.int32)
+    assert torch.equal(call(sizes=sizes), m(x, None, sizes=sizes))
