@@ -87,3 +87,31 @@ def test_dot_heads_drop_their_input_in_training_only():
     assert torch.equal(m(x, None, "elu", "concat", 0.5, 0.6), want)
     sizes = torch.tensor([30, 7], device=dev, dtype=torch.int32)
     assert torch.equal(call(sizes=sizes), m(x, None, sizes=sizes))
+
+
+def test_masks_of_few_entries_captured_with_rows_that_are_not_finite_where_nothing_attends():
+    """The walk over single entries does not touch rows that no query attends: replayed twice, dk compared too."""
+    from gat_amd import graphs, ops
+    from tests.test_dot_attention_gpu import _case, _run
+    c = _case(2, 600, 600, 2, 2, 16, "f32", density=0.003, seed=2)
+    never = (c["bias"] < -1e8).all(1)[0]                                 # keys of the first graph that no query attends
+    assert never.any() and not never.all()
+    want = _run(c)
+    q, k, v = (c[n].clone().requires_grad_() for n in ("q", "k", "v"))
+    with torch.no_grad():
+        k[0, never], v[0, never] = float("nan"), float("inf")
+
+    def step():
+        out = ops.dot_attention(q, k, v, c["bias"])
+        return (out, *torch.autograd.grad(out, (q, k, v), c["dout"]))
+
+    replay, res = graphs.capture(step, fresh_dropout=False)
+    for _ in range(2):
+        for t in res:
+            t.fill_(7.0)
+        replay()
+        torch.cuda.synchronize()
+        for got, n in zip(res, ("out", "dq", "dk", "dv")):
+            assert torch.equal(got, want[n]), n
+        _run(c)
+    assert (res[2][0, never] == 0).all() and (res[3][0, never] == 0).all()
