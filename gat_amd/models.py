@@ -109,6 +109,7 @@ class Muon(torch.optim.Optimizer):
     params: (parameter, head axis) pairs as matrix_parameters gives them, or plain 2-d [out, in] parameters.  A 3-d kernel
     [F, H, D] (head axis 1) is one F x D matrix per head, as the reference creates them (tf.layers.conv1d per head,
     utils/layers.py:11); [H, F, D] has head axis 0.  Matrices of one shape share one call.  What is not a matrix goes to TFAdam.
+    The momentum is held in fp32, also that of bf16 parameters: 0.05 m would be lost beside m in 8 bits after some steps.
     step() only enqueues: it can be captured (gat_amd.graphs.capture); lr is then frozen."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
@@ -123,6 +124,14 @@ class Muon(torch.optim.Optimizer):
         super().__init__([dict(params=ps, head_axis=axis) for axis, ps in by_axis.items()],
                          dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]                       # torch has rounded the momentum to the type of its parameter
+        names = [n for group in state_dict["param_groups"] for n in group["params"]]
+        for n, p in zip(names, (p for group in self.param_groups for p in group["params"])):
+            if n in saved:
+                self.state[p]["m"] = saved[n]["m"].detach().to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -135,8 +144,8 @@ class Muon(torch.optim.Optimizer):
                 continue
             for p in ps:
                 if "m" not in self.state[p]:
-                    self.state[p]["m"] = torch.zeros_like(p)
-            gs, ms = [p.grad for p in ps], [self.state[p]["m"] for p in ps]
+                    self.state[p]["m"] = torch.zeros_like(p, dtype=torch.float32)
+            gs, ms = [p.grad.float() for p in ps], [self.state[p]["m"] for p in ps]
             torch._foreach_mul_(ms, group["momentum"])
             torch._foreach_add_(ms, gs)
             us = torch._foreach_add(gs, ms, alpha=group["momentum"]) if group["nesterov"] else ms

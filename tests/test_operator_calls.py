@@ -171,3 +171,43 @@ def test_dropout_of_the_coefficients_is_refused():
             assert not any(m.has_res for m in store.layers)
     with pytest.raises(ValueError, match="residual"):
         layers.DotHeads(8, 4, 8, 2)                                                            # not the number of shared heads
+
+
+def _muon(monkeypatch, made):
+    """models.Muon with its orthogonalisation replaced by the identity, whose inputs are kept."""
+    from gat_amd import models, ops
+
+    def same(x, steps=5, **kw):
+        made.append(x.clone())
+        return x.clone()
+    monkeypatch.setattr(ops, "newton_schulz", same)
+    return models.Muon
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_keeps_the_momentum_of_bf16_parameters_in_fp32(monkeypatch, nesterov):
+    """A constant gradient: m_k = g (1 - 0.95^k) / 0.05.  In fp32 a step rounds twice, 2^-24 of m each, the factor itself is rounded (2^-25), and
+    0.95 carries that on, 20 times in all: 50 * 2^-24 at the most, and 3 * 2^-24 more in the sum that is handed on.  (In bf16 m stays where a step
+    changes it by less than half of its last place, up to some hundredths short.)"""
+    made = []
+    Muon = _muon(monkeypatch, made)
+    p = torch.nn.Parameter(torch.zeros((3, 5), dtype=torch.bfloat16))
+    opt = Muon([p], lr=0.0, nesterov=nesterov)
+    g = torch.randn((3, 5), generator=torch.Generator().manual_seed(0)).to(torch.bfloat16)
+    for _ in range(150):
+        p.grad = g.clone()
+        opt.step()
+    m = g.double() * (1 - 0.95 ** 150) / 0.05
+    want = g.double() + 0.95 * m if nesterov else m
+    assert opt.state[p]["m"].dtype == torch.float32 and made[-1].dtype == torch.float32
+    assert ((opt.state[p]["m"].double() - m).abs() <= 50 * 2.0 ** -24 * m.abs()).all()
+    assert ((made[-1][0].double() - want).abs() <= 53 * 2.0 ** -24 * want.abs()).all()
+    # saved and loaded it stays as it is
+    other = Muon([torch.nn.Parameter(p.detach().clone())], lr=0.0, nesterov=nesterov)
+    other.load_state_dict(opt.state_dict())
+    (q,) = other.param_groups[0]["params"]
+    q.grad = g.clone()
+    assert torch.equal(other.state[q]["m"], opt.state[p]["m"]) and other.state[q]["m"].data_ptr() != opt.state[p]["m"].data_ptr()
+    for o in (opt, other):
+        o.step()
+    assert torch.equal(other.state[q]["m"], opt.state[p]["m"])

@@ -1,6 +1,9 @@
 """GPU tests of calls of ops.dot_attention, ops.embedding and ops.newton_schulz as documented but off the common path."""
+import numpy as np
 import pytest
 import torch
+
+from tests import attn_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +118,46 @@ def test_masks_of_few_entries_captured_with_rows_that_are_not_finite_where_nothi
             assert torch.equal(got, want[n]), n
         _run(c)
     assert (res[2][0, never] == 0).all() and (res[3][0, never] == 0).all()
+
+
+def test_muon_on_bf16_parameters_eager_and_captured():
+    """Three steps against the formula: the momentum in fp32, each step's weights rounded to bf16 twice (decay, update), 2^-8 of what they are."""
+    from gat_amd import graphs
+    from gat_amd.models import Muon
+    dev = torch.device("cuda:0")
+    rng = np.random.default_rng(3)
+    bf = lambda a: torch.tensor(a, dtype=torch.float32).to(torch.bfloat16)
+    start = [bf(rng.normal(0, 1, (20, 70))), bf(rng.normal(0, 1, (30, 4, 12)))]
+    grads = [[bf(rng.normal(0, 1, t.shape)).to(dev) for t in start] for _ in range(3)]
+
+    def make():
+        ps = [torch.nn.Parameter(t.to(dev)) for t in start]
+        return ps, Muon([(ps[0], None), (ps[1], 1)], lr=0.1, momentum=0.9, weight_decay=0.5)
+
+    ps, opt = make()
+    ref, mom, slack = [t.double().numpy() for t in start], [0.0, 0.0], [0.0, 0.0]
+    for gs in grads:
+        for i, (p, g) in enumerate(zip(ps, gs)):
+            p.grad = g.clone()
+            mom[i] = 0.9 * mom[i] + g.double().cpu().numpy()
+            u = g.double().cpu().numpy() + 0.9 * mom[i]
+            rate = lambda m: 0.1 * max(1.0, m.shape[0] / m.shape[1]) ** 0.5 * attn_ref.newton_schulz(m)
+            before = abs(ref[i])
+            ref[i] = ref[i] * 0.95 - (rate(u) if i == 0 else np.stack([rate(u[:, h].T).T for h in range(4)], 1))
+            slack[i] = 0.95 * slack[i] + 2.0 ** -8 * (before + slack[i] + abs(ref[i])) * 1.01 + 1e-4
+        opt.step()
+    for p, r, e in zip(ps, ref, slack):
+        assert p.dtype == torch.bfloat16
+        attn_ref.within(p.detach().double().cpu().numpy(), r, e, "weights")
+    qs, other = make()
+    for q, g in zip(qs, grads[0]):
+        q.grad = g.clone()
+    other.step()                                                         # the state is made eagerly
+    replay, _ = graphs.capture(other.step, warmup=0, fresh_dropout=False)
+    for gs in grads[1:]:
+        for q, g in zip(qs, gs):
+            q.grad.copy_(g)
+        replay()
+        torch.cuda.synchronize()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)
