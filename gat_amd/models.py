@@ -106,23 +106,38 @@ def matrix_parameters(module):
 class Muon(torch.optim.Optimizer):
     """Momentum whose update of every matrix is orthogonalised (ops.newton_schulz) before it is applied:
         m = momentum m + g;  u = g + momentum m (nesterov) or m;  W -= lr sqrt(max(1, out / in)) orth(u);  W *= 1 - lr weight_decay first.
-    params: (parameter, head axis) pairs as matrix_parameters gives them, or plain 2-d [out, in] parameters.  A 3-d kernel
+    params: (parameter, head axis) pairs as matrix_parameters gives them, plain 2-d [out, in] parameters, or dicts of a group.  A 3-d kernel
     [F, H, D] (head axis 1) is one F x D matrix per head, as the reference creates them (tf.layers.conv1d per head,
     utils/layers.py:11); [H, F, D] has head axis 0.  Matrices of one shape share one call.  What is not a matrix goes to TFAdam.
     The momentum is held in fp32, also that of bf16 parameters: 0.05 m would be lost beside m in 8 bits after some steps.
     step() only enqueues: it can be captured (gat_amd.graphs.capture); lr is then frozen."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
-        if lr < 0.0 or not 0.0 <= momentum < 1.0 or weight_decay < 0.0 or steps < 1:
-            raise ValueError("Muon: lr = %r, momentum = %r, weight_decay = %r, steps = %r" % (lr, momentum, weight_decay, steps))
-        by_axis = {}
+        by_axis, groups = {}, []
         for entry in params:
-            p, axis = entry if isinstance(entry, (tuple, list)) else (entry, None)
+            if isinstance(entry, dict):
+                groups.append(entry)
+            else:
+                by_axis.setdefault(entry[1] if isinstance(entry, (tuple, list)) else None, []).append(entry)
+        super().__init__([dict(params=entries) for entries in by_axis.values()] + groups,
+                         dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+
+    def add_param_group(self, group):
+        """group: a dict with "params" as the constructor takes them, all of one head axis, and what differs from the defaults."""
+        group = dict(group)
+        entries = group["params"]
+        entries = [entries] if torch.is_tensor(entries) else list(entries)
+        pairs = [tuple(e) if isinstance(e, (tuple, list)) else (e, group.get("head_axis")) for e in entries]
+        lr, momentum, decay, steps = (group.get(n, self.defaults[n]) for n in ("lr", "momentum", "weight_decay", "steps"))
+        if lr < 0.0 or not 0.0 <= momentum < 1.0 or decay < 0.0 or steps < 1:
+            raise ValueError("Muon: lr = %r, momentum = %r, weight_decay = %r, steps = %r" % (lr, momentum, decay, steps))
+        if len({axis for _, axis in pairs}) > 1:
+            raise ValueError("Muon: the parameters of a group have one head axis")
+        for p, axis in pairs:
             if p.dim() != (2 if axis is None else 3) or axis not in (None, 0, 1):
                 raise ValueError("Muon: a parameter of shape %s with head axis %r is not a matrix or a set of them" % (tuple(p.shape), axis))
-            by_axis.setdefault(axis, []).append(p)
-        super().__init__([dict(params=ps, head_axis=axis) for axis, ps in by_axis.items()],
-                         dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+        group["params"], group["head_axis"] = [p for p, _ in pairs], pairs[0][1] if pairs else None
+        super().add_param_group(group)
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)

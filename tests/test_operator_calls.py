@@ -211,3 +211,25 @@ def test_muon_keeps_the_momentum_of_bf16_parameters_in_fp32(monkeypatch, nestero
     for o in (opt, other):
         o.step()
     assert torch.equal(other.state[q]["m"], opt.state[p]["m"])
+
+
+def test_muon_groups_added_later_and_given_as_dicts(monkeypatch):
+    made = []
+    Muon = _muon(monkeypatch, made)
+    t = lambda *s: torch.nn.Parameter(torch.ones(s))
+    a, b, c, d = t(3, 4), t(5, 2, 3), t(2, 5), t(2, 6, 3)
+    opt = Muon([a, {"params": [(b, 1)], "lr": 0.5}])
+    opt.add_param_group({"params": c, "momentum": 0.0})
+    opt.add_param_group({"params": [(d, 0)]})
+    assert [(g["head_axis"], g["lr"], g["momentum"]) for g in opt.param_groups] == [(None, 0.02, 0.95), (1, 0.5, 0.95), (None, 0.02, 0.0), (0, 0.02, 0.95)]
+    for p in (a, b, c, d):
+        p.grad = torch.full_like(p, 2.0)
+    opt.step()
+    assert [tuple(x.shape) for x in made] == [(1, 3, 4), (1, 2, 5, 3), (1, 2, 5), (1, 2, 6, 3)]
+    assert torch.allclose(c, torch.full_like(c, 1.0 - 0.02 * 2.0)) and torch.allclose(b, torch.full_like(b, 1.0 - 0.5 * 3.9))
+    for bad in ({"params": [t(2, 2, 2)]}, {"params": [(t(2, 2), 0)]}, {"params": [t(4, 4)], "momentum": 1.0}, {"params": [(t(2, 2, 2), 1), t(3, 3)]}):
+        with pytest.raises(ValueError):
+            opt.add_param_group(bad)
+    assert len(opt.param_groups) == 4
+    opt.load_state_dict(opt.state_dict())
+    opt.step()
