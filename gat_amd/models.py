@@ -129,13 +129,15 @@ class Muon(torch.optim.Optimizer):
         entries = [entries] if torch.is_tensor(entries) else list(entries)
         pairs = [tuple(e) if isinstance(e, (tuple, list)) else (e, group.get("head_axis")) for e in entries]
         lr, momentum, decay, steps = (group.get(n, self.defaults[n]) for n in ("lr", "momentum", "weight_decay", "steps"))
-        if lr < 0.0 or not 0.0 <= momentum < 1.0 or decay < 0.0 or steps < 1:
+        if lr < 0.0 or not 0.0 <= momentum < 1.0 or decay < 0.0 or not 1 <= steps <= 32:                 # 32: the kernels' most
             raise ValueError("Muon: lr = %r, momentum = %r, weight_decay = %r, steps = %r" % (lr, momentum, decay, steps))
         if len({axis for _, axis in pairs}) > 1:
             raise ValueError("Muon: the parameters of a group have one head axis")
         for p, axis in pairs:
             if p.dim() != (2 if axis is None else 3) or axis not in (None, 0, 1):
                 raise ValueError("Muon: a parameter of shape %s with head axis %r is not a matrix or a set of them" % (tuple(p.shape), axis))
+            if p.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError("Muon: a parameter is %s, fp32 or bf16 expected" % (p.dtype,))
         group["params"], group["head_axis"] = [p for p, _ in pairs], pairs[0][1] if pairs else None
         super().add_param_group(group)
 
@@ -154,7 +156,7 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            ps = [p for p in group["params"] if p.grad is not None]
+            ps = [p for p in group["params"] if p.grad is not None and p.numel()]
             if not ps:
                 continue
             for p in ps:

@@ -233,3 +233,23 @@ def test_muon_groups_added_later_and_given_as_dicts(monkeypatch):
     assert len(opt.param_groups) == 4
     opt.load_state_dict(opt.state_dict())
     opt.step()
+
+
+def test_muon_refuses_what_its_step_cannot_do_when_it_is_made(monkeypatch):
+    """Types and counts that ops.newton_schulz refuses: not in the middle of a step, when momentum and decay have been applied."""
+    Muon = _muon(monkeypatch, [])
+    t = lambda dtype: torch.nn.Parameter(torch.ones((3, 4), dtype=dtype))
+    for dtype in (torch.float16, torch.float64):
+        with pytest.raises(ValueError, match="fp32 or bf16"):
+            Muon([t(dtype)])
+    with pytest.raises(ValueError, match="steps"):
+        Muon([t(torch.float32)], steps=33)
+    from gat_amd import _lib
+    P = 4096                                                       # never read: the counts are refused before any launch
+    for steps, rc in ((0, -1), (33, -1)):
+        assert _lib.lib.gatmi_newton_schulz(1, 4, 4, P, 16, 4, 0, steps, 3.4445, -4.775, 2.0315, 1e-7, P, 16, 4, P, None) == rc
+    empty = torch.nn.Parameter(torch.ones((3, 0)))
+    opt = Muon([empty, t(torch.bfloat16)], steps=32)
+    for p in opt.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    opt.step()                                                     # a matrix without entries has nothing to update
