@@ -110,7 +110,7 @@ class Muon(torch.optim.Optimizer):
     [F, H, D] (head axis 1) is one F x D matrix per head, as the reference creates them (tf.layers.conv1d per head,
     utils/layers.py:11); [H, F, D] has head axis 0.  Matrices of one shape share one call.  What is not a matrix goes to TFAdam.
     The momentum is held in fp32, also that of bf16 parameters: 0.05 m would be lost beside m in 8 bits after some steps.
-    step() only enqueues: it can be captured (gat_amd.graphs.capture); lr is then frozen."""
+    step() only enqueues: from the second step on it can be captured (gat_amd.graphs.capture warms up first); lr is then frozen."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
         by_axis, groups = {}, []
@@ -159,9 +159,11 @@ class Muon(torch.optim.Optimizer):
             ps = [p for p in group["params"] if p.grad is not None and p.numel()]
             if not ps:
                 continue
-            for p in ps:
-                if "m" not in self.state[p]:
-                    self.state[p]["m"] = torch.zeros_like(p, dtype=torch.float32)
+            fresh = [p for p in ps if "m" not in self.state[p]]
+            if fresh and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Muon: the first step of a parameter makes its momentum and cannot be captured; take one before")
+            for p in fresh:
+                self.state[p]["m"] = torch.zeros_like(p, dtype=torch.float32)
             gs, ms = [p.grad.float() for p in ps], [self.state[p]["m"] for p in ps]
             torch._foreach_mul_(ms, group["momentum"])
             torch._foreach_add_(ms, gs)

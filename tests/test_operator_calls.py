@@ -253,3 +253,21 @@ def test_muon_refuses_what_its_step_cannot_do_when_it_is_made(monkeypatch):
     for p in opt.param_groups[0]["params"]:
         p.grad = torch.ones_like(p)
     opt.step()                                                     # a matrix without entries has nothing to update
+
+
+def test_muon_does_not_make_its_momentum_inside_a_capture(monkeypatch):
+    """The zeros it starts from would be part of the graph, and every replay would start from them."""
+    Muon = _muon(monkeypatch, [])
+    p = torch.nn.Parameter(torch.ones((3, 4)))
+    opt = Muon([p])
+    p.grad = torch.ones_like(p)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step()
+    assert not opt.state[p] and (p == 1.0).all()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    opt.step()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    opt.step()
+    assert torch.allclose(opt.state[p]["m"], torch.full_like(p, 1.95))

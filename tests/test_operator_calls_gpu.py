@@ -161,3 +161,21 @@ def test_muon_on_bf16_parameters_eager_and_captured():
         torch.cuda.synchronize()
     for p, q in zip(ps, qs):
         assert torch.equal(p, q)
+
+
+def test_muon_captured_before_its_first_step_is_refused():
+    from gat_amd.models import Muon
+    p = torch.nn.Parameter(torch.randn(8, 4, device="cuda:0"))
+    p.grad = torch.randn_like(p)
+    opt, graph = Muon([p]), torch.cuda.CUDAGraph()
+    before, x = p.detach().clone(), torch.zeros(4, device="cuda:0")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p, before) and (x == 1.0).all()
+    opt.step()
+    assert not torch.equal(p, before)
