@@ -864,17 +864,23 @@ _FLOATS = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 def _float_type(what, t, *others):
     """Code of the one dtype (fp32 or bf16) that all tensors share."""
-    code = _FLOATS.get(t.dtype)
-    if code is None or any(o.dtype != t.dtype for o in others):
+    dtype = t.dtype
+    code = _FLOATS.get(dtype)
+    for o in others:
+        if o.dtype != dtype:
+            code = None
+    if code is None:
         raise TypeError("%s: fp32 or bf16 tensors of one type expected, got %s" % (what, ", ".join(str(o.dtype) for o in (t, *others))))
     return code
 
 
 def _same_device(what, t, *others):
-    _require_cuda(t, *others)
     dev = t.device
+    if not t.is_cuda:
+        _require_cuda(t)
     for o in others:
         if o is not None and o.device != dev:
+            _require_cuda(o)
             raise ValueError("%s: tensors on different devices: %s and %s" % (what, dev, o.device))
     return dev
 
@@ -891,11 +897,14 @@ def _launch(device, name, *args):
         _lib.check(rc, name)
 
 
+_is_tracing, _forward_ad = torch._C._is_tracing, torch.autograd.forward_ad
+
+
 def _recorded():
     """Whether somebody follows what is called: torch.jit.trace, or forward-mode differentiation.  An operator then goes through its
     Function also where no gradient is asked: a trace records that as one node (of a bare launch it would keep the allocation of the
     result only), and a tangent is refused instead of lost."""
-    return torch.jit.is_tracing() or torch.autograd.forward_ad._current_level >= 0
+    return _is_tracing() or _forward_ad._current_level >= 0
 
 
 def _scratch(floats, device):
@@ -912,17 +921,18 @@ def _strides(t):
 
 
 def _attn_rows(t, width):
-    """t [B, N, heads, D] as rows the kernels take: D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
+    """(t [B, N, heads, D] as rows the kernels take, their strides): D zero-padded to `width`, contiguous, 16-byte aligned (a view where it already is)."""
     if t.shape[3] != width:
         rows = t.new_zeros((*t.shape[:3], width))                  # not pad(t): it keeps the order that the dimensions have in memory
         rows[..., :t.shape[3]] = t
-        return rows
-    n, s, low = t.shape, t.stride(), 15 // t.element_size()        # strides are multiples of 4 (fp32) or 8 (bf16) elements
-    apart = (s[0] if n[0] > 1 else 0) | (s[1] if n[1] > 1 else 0) | (s[2] if n[2] > 1 else 0)
-    if s[3] == 1 and not (apart & low) and not (t.data_ptr() & 15):
-        return t
+        return rows, _strides(rows)
+    strides = _strides(t)
+    low = 15 // t.element_size()                                   # strides are multiples of 4 (fp32) or 8 (bf16) elements
+    if t.stride(3) == 1 and not ((strides[0] | strides[1] | strides[2]) & low) and not (t.data_ptr() & 15):
+        return t, strides
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    t = t if t.data_ptr() % 16 == 0 else t.clone()
+    return t, _strides(t)
 
 
 def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
@@ -934,7 +944,7 @@ def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
     unit = 4 if dtype == _lib.DTYPE_F32 else 8
     width = (D + unit - 1) // unit * unit
     dev = q.device
-    qr, kr, vr = _attn_rows(q, width), _attn_rows(k, width), _attn_rows(v, width)
+    (qr, qs), (kr, ks), (vr, vs) = _attn_rows(q, width), _attn_rows(k, width), _attn_rows(v, width)
     out = torch.empty((B, Nq, H, width), dtype=q.dtype, device=dev)
     lse = torch.empty((B, H, Nq), dtype=torch.float32, device=dev) if need else None
     low = torch.empty_like(out) if need and dtype == _lib.DTYPE_BF16 else None
@@ -947,7 +957,7 @@ def _dot_forward(q, k, v, bias, key_sizes, query_sizes, scale, need):
     planes = None
     if dtype == _lib.DTYPE_F32:
         planes = _scratch(_lib.lib.gatmi_dot_attn_planes_floats(B, Nq, Nk, H, Hkv, width, dtype, need), dev)
-    _launch(dev, "gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr), vr.data_ptr(), _strides(vr),
+    _launch(dev, "gatmi_dot_attn_fwd", B, Nq, Nk, H, Hkv, width, dtype, qr.data_ptr(), qs, kr.data_ptr(), ks, vr.data_ptr(), vs,
             ptr(bias), *strides, ptr(key_sizes), ptr(query_sizes), scale, out.data_ptr(), ptr(low), ptr(lse), ptr(words),
             ptr(planes), ptr(ws))
     return qr, kr, vr, out, low, lse, words, planes, strides
@@ -973,12 +983,12 @@ class DotAttentionFn(torch.autograd.Function):
         B, Nq, H, width = qr.shape
         Nk, Hkv = kr.shape[1], kr.shape[2]
         D = ctx.D
-        dr = _attn_rows(dout, width)
+        dr, ds = _attn_rows(dout, width)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (qr, kr, vr))
         delta = torch.empty(lse.shape, dtype=torch.float32, device=lse.device)
         ws = None if planes is None else _scratch(_lib.lib.gatmi_dot_attn_bwd_ws_floats(B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype]), qr.device)
         _launch(qr.device, "gatmi_dot_attn_bwd", B, Nq, Nk, H, Hkv, width, _FLOATS[qr.dtype], qr.data_ptr(), _strides(qr), kr.data_ptr(), _strides(kr),
-                vr.data_ptr(), _strides(vr), out.data_ptr(), ptr(low), dr.data_ptr(), _strides(dr), lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
+                vr.data_ptr(), _strides(vr), out.data_ptr(), ptr(low), dr.data_ptr(), ds, lse.data_ptr(), ptr(bias), *ctx.bias_strides, ptr(key_sizes),
                 ptr(query_sizes), ctx.scale, ptr(words), ptr(planes), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), ptr(ws))
         if width != D:
             dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
