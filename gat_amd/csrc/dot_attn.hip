@@ -16,17 +16,17 @@
 // Matrix instructions: v_mfma_f32_16x16x4_f32 and v_mfma_f32_16x16x32_bf16, sums in fp32.  The scores are formed transposed (keys down, queries
 // across the lanes): a lane then holds four consecutive keys of ONE query, the softmax statistics are one register each,
 // and the probabilities sit in the operand layout of the second product as they are: they never go through LDS.  For that
-// product bf16 rows have P and dz as two bf16 each, high and low (Wide16), or, of many rows without a mask, rounded to one (uint16_t: half a step of 2^-8, as its
-// other operand has and its result is stored with).
+// product bf16 rows have P and dz as two bf16 each, high and low (Wide16), or, beyond 1024 nodes without a mask, rounded to one (uint16_t: half a step of 2^-8, as its
+// other operand has and its result is stored with; see dot_wide16).
 //
 // A mask with few entries is walked entry by entry (dot_entries_*), a denser one in tiles, without the 16 x 16 parts that it leaves empty.
 //
 // What the tiles measure, forward / dq / dk, dv: 4 graphs of 2048 to 4096 nodes, 16 heads on 4 of 128, bf16: 520 / 655 / 1180 us, 594 / 708 / 524
-// TFLOP/s of products (a large bf16 product reaches 1140): the matrix instructions wait for LDS reads, most of all in dk, dv with
-// two operands that are read column-wise.  16 x 1024 nodes, 4 heads of 64, fp32: 92 / 121 / 164 us, 187 / 213 / 210 TFLOP/s of fp32 accuracy (a
+// TFLOP/s of products (a large bf16 product reaches 1140).  Matrix units 37 / 45 / 29 % busy, vector units 49 / 41 / 22 %, LDS 28 / 30 / 24 %: none is
+// full, 1.6 waves a SIMD wait for their own reads (33 / 34 / 64 % of their time), most of all in dk, dv with two operands that are read column-wise.  16 x 1024 nodes, 4 heads of 64, fp32: 92 / 121 / 164 us, 187 / 213 / 210 TFLOP/s of fp32 accuracy (a
 // large fp32 product: 153).  1024 graphs of 246 nodes, 8 heads of 8, 10 % attended: 375 / 419 / 589 us for 2 / 3 / 4 products of 8 wide operands each:
-// exponentials, masks and the bits' tests in the vector units, which the fp32 matrix instructions share, take the time.
-// One query on 98000 keys, 8 heads on 2 of 64, bf16, two graphs: 20.2 us, 5.0 TB/s (a large copy: 4.7).
+// matrix instructions (45 to 58 % of the cycles) and exponentials, masks and the bits' tests (51 to 36 %) share the SIMDs and nearly fill them.
+// One query on 98000 keys, 8 heads on 2 of 64, two graphs: 20.2 us in bf16, 5.0 TB/s (a large copy: 4.7), with the join 24; 51 in fp32 with the join, 4.0 TB/s.
 //
 // fp32 rows are computed in one of two ways.  A few rows: on v_mfma_f32_16x16x4_f32 (256 flop / clock / CU, which the vector units cannot use
 // meanwhile).  Otherwise (Split3): every number x is split exactly into three bf16, h + m + l with 8 bits each, and a product is the six
@@ -1614,12 +1614,18 @@ static int dot_launch(const char *what, K kernel, const DotArgs &a, size_t lds, 
 
 using namespace gatmi;
 
-// Masks of fewer entries than this are never walked entry by entry: finding out and the idle launches would cost more.
+// Masks of fewer entries than this are never walked entry by entry.  Finding out (the count, launches that return at once) costs 8 to 20 us a forward and
+// backward, 50 and 90 of 1024 masks.  Never - found out, in us, of masks that end in tiles (10 %): fp32 64 graphs of 128 nodes, 4 heads of 8: 33 - 46, 16 of 246, 4 of 64:
+// 92 - 103, 50 of 246, 6 of 64: 239 - 259, one of 400, 8 of 8: 69 - 78, 1024 of 246, 8 of 8: 1401 - 1451; bf16 50 of 246: 105 - 122, 1024 of 246: 863 - 950.
+// Of masks that are walked (1 %): fp32 34 - 46, 94 - 53, 245 - 128, 72 - 45, 1382 - 560; bf16 114 - 92, 919 - 808.  Graphs of so few nodes come as
+// connectivity thresholded to 10 % and more, so they keep the tiles without asking; a batch of very sparse ones pays for it.
 constexpr int64_t kEntriesMask = 512 * 512;
 static bool dot_maybe_entries(int64_t Nq, int64_t Nk) { return Nq * Nk >= kEntriesMask; }
 // "Few" is one entry of 16 for fp32, of 64 for bf16.  Forward and backward in us, 16 graphs of 1024 nodes, 4 heads, tiles - entries:
 //   fp32, 8 wide: 0.2 % 168 - 39, 1.6 % 213 - 70, 6.4 % 211 - 154;  64 wide: 392 - 90, 438 - 189, 433 - 440;  128 wide: 1101 - 137, 1112 - 353, 1080 - 863
 //   bf16, 64 wide: 0.2 % 175 - 87, 1.6 % 179 - 176, 3.2 % 165 - 254;  128 wide: 290 - 105, 306 - 236, 288 - 372
+// Entries are counted over the whole mask.  A row's are walked one after the other, so long rows take longer than tiles do: 2708 nodes with 5 entries a
+// row, 8 heads of 8, fp32: 281 - 57; as many with a power law (longest row 514): 326 - 286; with one full row and column: 319 - 993.
 static int64_t dot_entries_share(int32_t dtype) { return dtype == GATMI_DTYPE_F32 ? 16 : 64; }
 
 // floats that hold the words of `graphs` masks (rows, then columns), with the counts and flags of large ones
@@ -1754,10 +1760,12 @@ static int dot_fwd_run(DotArgs a, int64_t B, float *planes, hipStream_t st) {
     return GATMI_OK;
 }
 
-// bf16: whether P and dz are two numbers each.  Their rounding adds as much to the results' error as the rounding of the results; a mask adds up over
-// fewer entries, where it shows more (dq of 2 % masks is 1.5 times as far off as its own rounding), so masks have two.  Without a mask the second
-// number is cheap up to 1024 nodes and dear beyond; forward and backward, one - two numbers, in us: 16 x 1025 - 16 x 1024 nodes, 4 heads of 64: 157 - 155, of
-// 128: 345 - 310; 4 x 4096 nodes, 16 heads of 64: 1388 - 1879, of 128: 2868 - 4315.
+// bf16: whether P and dz are two numbers each.  Rounded to one they add as much to the results' error as the rounding of the results does (1.41 times it
+// together), whatever the number of nodes; over a mask's fewer entries it shows more (dq of 2 % masks: 1.53 times), so masks always have two.  Without a
+// mask the second number costs up to half of the time at any size.  Forward and backward, one - two numbers, in us: 16 graphs of 1024, 4 heads of 64:
+// 117 - 145, of 128: 194 - 270; 4 of 1024, 16 heads on 4 of 128: 374 - 347; 4 of 1536: 626 - 620; 8 of 1536, 4 heads of 128: 257 - 353; 8 of 2048: 340 - 501; 4 of
+// 2048, 16 on 4 of 128: 881 - 979; 4 of 4096, 16 on 4 of 64: 1299 - 1749, of 128: 2539 - 3772.  So the border is a choice: up to 1024 nodes, the
+// sizes of whole small graphs, the accuracy of a single rounding; beyond, where this is most of a step, the time.
 static bool dot_wide16(int64_t rows, int64_t Nq, int64_t Nk, bool mask) { return mask || rows <= 64 || Nk <= 64 || std::max(Nq, Nk) <= 1024; }
 
 #define GATMI_DOT_DISPATCH(RUN, parts)                                                             \

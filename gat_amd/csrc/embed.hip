@@ -418,7 +418,8 @@ __global__ __launch_bounds__(256) void embed_seg_kernel(SegArgs a) {
 
 // The first fill_blocks blocks fill the rows without a bit with zeros.  In the others a lane group looks at a chunk: where a run starts in
 // it and goes on behind it, the group adds its partial rows, or, of a run over more than kShortRun chunks, the block does: its groups
-// take consecutive shares, their sums are added in order.
+// take consecutive shares, their sums are added in order.  That one block is what a run of most tokens waits for: the gradient of 4 million tokens on one row of
+// 100 fp32 takes 1987 us, spread over 2.4 million rows 1042.
 template <typename T, int E, int L>
 __global__ __launch_bounds__(256) void embed_join_kernel(SegArgs a, uint32_t join_blocks, uint32_t fill_blocks) {
     constexpr int GROUPS = 256 / L;

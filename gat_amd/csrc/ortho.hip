@@ -14,7 +14,8 @@
 //   operand v is kept as hi + lo, two fp16 numbers of 11 bits each, and hi hi + hi lo + lo hi is summed in fp32 (relative error 2^-22;
 //   the missing lo lo is below it).  fp16 has few exponent bits, but the iteration bounds its operands: entries of X, X X^T and of the
 //   polynomial are below kMaxEntry (checked on the host for the given coefficients), so that one fixed scale
-//   2^13 keeps hi in range and lo of every entry that matters above the subnormals.  Where |x|_F is not far above eps, X is tiny: it is
+//   2^13 keeps hi in range and lo of every entry that matters above the subnormals: an entry is kept to 2^-22 of itself or 2^-38 of
+//   |X|_F, whichever is larger.  Where |x|_F is not far above eps, X is tiny: it is
 //   then kept times 2^e with e falling from step to step as X can grow (NsShift).  3 products at 16 times the rate of fp32's.
 //   `small` (n <= 64, at most 128 long): all steps in one block's LDS, one launch.  `wide` (n > 64): a launch per product; X X^T and its square
 //   are symmetric: only tiles on and above the diagonal are formed, each is stored twice.

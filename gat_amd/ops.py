@@ -1013,7 +1013,11 @@ def dot_attention(q, k, v, bias_mat=None, *, key_sizes=None, query_sizes=None, s
     bias_mat [B or 1, Nq, Nk] fp32 (or None): an entry not above -1e8 is not attended; it takes no gradient.
     key_sizes, query_sizes: int32 [B] on the same device: rows behind a graph's own nodes take no part and get no
     gradient, and their outputs are zeros.  A row without an attended key gives zeros.  Rows of k and v inside key_sizes have to be
-    finite also where the mask leaves them out.  The backward recomputes the probabilities and adds in a fixed order."""
+    finite also where the mask leaves them out.  The backward recomputes the probabilities and adds in a fixed order.
+    bf16 results are rounded once; without a mask and with more than 1024 queries or keys the probabilities are rounded too, and the
+    error is 1.4 times as large.  fp32 rows wider than 16, of many queries and keys, are computed as three bf16 parts each, at fp32
+    accuracy: an infinity, or a number above 3.38e38, among them gives NaN, and with gradients 6 more bytes per element of q, k and v
+    are held until the backward."""
     what = "dot_attention"
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not torch.is_tensor(t) or t.dim() != 4:
@@ -1127,7 +1131,8 @@ class NewtonSchulzFn(torch.autograd.Function):
 
 def newton_schulz(x, steps=5, eps=1e-7, coefficients=NEWTON_SCHULZ):
     """Every m x n matrix of x [..., m, n] (fp32 or bf16) with its singular values driven towards 1: from X = x / (|x|_F + eps), `steps`
-    times X <- a X + b (X X^T) X + c (X X^T)^2 X, at fp32 accuracy whatever the type (gatmi_newton_schulz).  Outside autograd."""
+    times X <- a X + b (X X^T) X + c (X X^T)^2 X, whatever the type at fp32 accuracy of the norm: single entries are good to
+    2^-38 |X|_F (gatmi_newton_schulz).  Outside autograd."""
     if not torch.is_tensor(x) or x.dim() < 2:
         raise ValueError("newton_schulz: x is [..., m, n], got %s" % (tuple(x.shape) if torch.is_tensor(x) else type(x),))
     _float_type("newton_schulz", x)

@@ -569,6 +569,8 @@ int gatmi_ipd_bwd(int64_t B, int32_t N, int32_t F, const float *dOut, const floa
  *   planes: gatmi_dot_attn_planes_floats floats (0: NULL), asked with backward = 1 for a fwd that has lse; written by fwd, read by the
  *   bwd of the same call, which gets it where its fwd did: fp32 rows as three bf16 parts each, on which many rows are computed faster at
  *   fp32 accuracy (an infinity, or a number above 3.38e38, among them gives NaN).  NULL is allowed, and slower.
+ *   bf16: results are rounded once; without a bias, with more than 64 rows Nq * H / Hkv and 64 keys and more than 1024 queries or keys,
+ *   the probabilities and their gradients are rounded to bf16 too (error 1.4 times as large, about two thirds of the time).
  *   bwd: the probabilities are formed again from lse; dq [B, Nq, H, D], dk, dv [B, Nk, Hkv, D] contiguous, written whole; delta
  *   [B, H, Nq] and ws (gatmi_dot_attn_bwd_ws_floats; planes NULL: may be NULL) are scratch.  No atomics: the same bits every run. */
 size_t gatmi_dot_attn_mask_floats(int64_t B, int32_t Nq, int32_t Nk, int64_t bias_batch);
@@ -600,7 +602,8 @@ int gatmi_embed_bwd(const void *ids, int32_t id_bits, int64_t tokens, const void
 
 /* Newton-Schulz orthogonalisation of a batch of m x n matrices (an update's singular values driven towards 1): from
  * X = x / (|x|_F + eps), `steps` (1..32) times X <- a X + b (X X^T) X + c (X X^T)^2 X.  x, out: fp32 or bf16, element
- * (i, j) of matrix b at b * batch stride + i * row stride + j; fp32 accuracy throughout, one rounding at the end.
+ * (i, j) of matrix b at b * batch stride + i * row stride + j; products at fp32 accuracy of the norm (entries are kept to 2^-38 |X|_F;
+ * to fp64's where the shorter side is at most 64 and the longer above 128), one rounding at the end.
  * GATMI_EUNSUPPORTED when (a, b, c) let the iteration's entries pass 7.5 within `steps`. */
 size_t gatmi_newton_schulz_ws_floats(int64_t batch, int64_t m, int64_t n);
 int gatmi_newton_schulz(int64_t batch, int64_t m, int64_t n, const void *x, int64_t x_batch, int64_t x_row, int32_t dtype,
