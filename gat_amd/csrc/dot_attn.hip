@@ -1357,7 +1357,9 @@ __device__ __forceinline__ float dot8(const float (&x)[8], const float (&y)[8]) 
     for (int k = 0; k < 8; ++k) s = fmaf(x[k], y[k], s);
     return group_sum<DL>(s);
 }
-// each(entry, whether its bias is other than 0) for the attended ones among the first n, every WS-th word from `first` on
+// each(entry, whether its bias is other than 0) for the attended ones among the first n, every WS-th word from `first` on.
+// The entry's bit of the second word is taken with the lowest bit of `bits`, not with a shift: hipcc (ROCm 7.2) put the amount of that 64-bit shift into
+// the last register of the wave, from where the hardware reads it wrong in all but a SIMD's first wave (tests/test_shift_amounts.py).
 template <int WS, typename F>
 __device__ __forceinline__ void walk_entries(const ulonglong2 *words, int n, int first, F each) {
     const int count = (n + 63) / 64;
@@ -1368,10 +1370,8 @@ __device__ __forceinline__ void walk_entries(const ulonglong2 *words, int n, int
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int base = (w0 + u * WS) * 64;
-            for (uint64_t bits = x[u].x & first_bits(n - base); bits; bits &= bits - 1) {
-                const int e = __builtin_ctzll(bits);
-                each(base + e, (x[u].y >> e & 1) != 0);
-            }
+            for (uint64_t bits = x[u].x & first_bits(n - base); bits; bits &= bits - 1)
+                each(base + __builtin_ctzll(bits), (x[u].y & bits & -bits) != 0);
         }
     }
 }

@@ -179,3 +179,13 @@ def test_muon_captured_before_its_first_step_is_refused():
     assert torch.equal(p, before) and (x == 1.0).all()
     opt.step()
     assert not torch.equal(p, before)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [8, 16, 32, 64, 97, 128])
+@pytest.mark.parametrize("Nq,Nk,H,G", [(1400, 190, 8, 1), (190, 1400, 8, 8)])
+def test_soft_masks_of_few_entries_on_more_rows_than_run_at_once(Nq, Nk, H, G, D, dtype):
+    """Biases other than 0, and so many queries, or keys, that every SIMD has several waves of the walk over single entries."""
+    from tests.test_dot_attention_gpu import _case, _check
+    _check(_case(2, Nq, Nk, H, G, D, dtype, density=0.01, soft=True, shared_mask=D == 32, seed=D + Nq), dtype, what="%d wide" % D)
+    _check(_case(2, Nq, Nk, H, G, D, dtype, density=0.01, soft=True, seed=D + Nq), dtype, grad=False, what="%d wide, forward alone" % D)
