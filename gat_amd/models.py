@@ -146,7 +146,7 @@ class Muon(torch.optim.Optimizer):
         saved = state_dict["state"]                       # torch has rounded the momentum to the type of its parameter
         names = [n for group in state_dict["param_groups"] for n in group["params"]]
         for n, p in zip(names, (p for group in self.param_groups for p in group["params"])):
-            if n in saved:
+            if "m" in saved.get(n, ()):
                 self.state[p]["m"] = saved[n]["m"].detach().to(device=p.device, dtype=torch.float32, copy=True)
 
     @torch.no_grad()

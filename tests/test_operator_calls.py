@@ -270,3 +270,17 @@ def test_muon_does_not_make_its_momentum_inside_a_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     opt.step()
     assert torch.allclose(opt.state[p]["m"], torch.full_like(p, 1.95))
+
+
+def test_muon_loads_a_state_without_momentum(monkeypatch):
+    """As it is saved after a step that was refused, or before the first one."""
+    Muon = _muon(monkeypatch, [])
+    p = torch.nn.Parameter(torch.ones((3, 4)))
+    opt = Muon([p])
+    opt.state[p]                                                   # an entry, but nothing in it
+    other = Muon([torch.nn.Parameter(torch.ones((3, 4)))])
+    other.load_state_dict(opt.state_dict())
+    (q,) = other.param_groups[0]["params"]
+    q.grad = torch.ones_like(q)
+    other.step()
+    assert torch.allclose(other.state[q]["m"], torch.ones_like(q))
